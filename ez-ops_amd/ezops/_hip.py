@@ -64,6 +64,14 @@ SIGNATURES: dict[str, tuple] = {
                                             _f32, _p, _sz, _p]),
     "ezops_qk_norm_rope_bf16": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _p,
                                        _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64, _f32, _p]),
+    "ezops_paged_batch_plan": (_i32, [_p] * 10 + [_i64] * 6 + [_p]),
+    "ezops_qk_norm_mrope_bf16": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _p, _i32, _p, _p, _i32, _p, _i64, _p, _i32,
+                                        _p, _p, _p, _i64, _i64, _p, _p] + [_i64] * 5 + [_f32, _p]),
+    "ezops_linear_attn_prefill_workspace_size": (_sz, [_i64] * 6),
+    "ezops_linear_attn_prefill_bf16": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _p, _p, _p, _p, _i64, _p] + [_i64] * 6
+                                       + [_f32, _p, _sz, _p]),
+    "ezops_linear_attn_decode_bf16": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _p, _p, _i64, _p, _i64, _i64, _i64, _i64,
+                                             _f32, _p]),
     "ezops_o_proj_ffn_workspace_size": (_sz, [_i64, _i64, _i64, _i64]),
     "ezops_o_proj_ffn_bf16": (_i32, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _f32, _p, _sz, _p]),
     "ezops_qwen3_layer_workspace_size": (_sz, [C.POINTER(Qwen3LayerParams)]),
@@ -134,6 +142,18 @@ def call(name: str, *args) -> None:
         raise RuntimeError(f"{name} failed ({rc}): {msg}")
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def call_on(device: torch.device, name: str, *args) -> None:
+    """``call`` with the tensors' device as the current one and its stream as the last argument."""
+    if device.index == _current_device():
+        call(name, *args, stream(device))
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, stream(device))
+
+
 def size(name: str, *args) -> int:
     return int(_fn(name)(*args))
 
@@ -178,6 +198,25 @@ def check(t: torch.Tensor, name: str, shape: tuple, dtype: torch.dtype) -> None:
         raise ValueError(f"{name}: expected dtype {dtype}, got {t.dtype}")
     if not t.is_contiguous():
         raise ValueError(f"{name}: must be contiguous")
+
+
+def check_rows(t: torch.Tensor, name: str, shape: tuple, dtype: torch.dtype) -> int:
+    """``check`` for a tensor whose rows (all dims behind the first) are contiguous and may lie apart, as slices of
+    a packed projection do; returns the distance of the rows in elements."""
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.dtype != dtype:
+        raise ValueError(f"{name}: expected dtype {dtype}, got {t.dtype}")
+    n = 1
+    for size_, stride_ in zip(reversed(shape[1:]), reversed(t.stride()[1:])):
+        if size_ != 1 and stride_ != n:
+            raise ValueError(f"{name}: the dims behind the first must be contiguous, got strides {t.stride()}")
+        n *= size_
+    if shape[0] <= 1:
+        return n
+    if t.stride(0) < n:
+        raise ValueError(f"{name}: rows must not overlap, got a row stride of {t.stride(0)} elements for {n}")
+    return t.stride(0)
 
 
 class Workspace:

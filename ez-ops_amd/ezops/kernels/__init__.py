@@ -5,6 +5,9 @@ from . import (  # noqa: F401
     fused_o_proj_ffn,
     fused_qk_norm_rope,
     gemv,
+    linear_attn,
+    paged_batch_plan,
+    qk_norm_mrope,
     qwen3_dense_decode,
     reduce,
     rmsnorm,

@@ -191,6 +191,99 @@ int ezops_qk_norm_rope_bf16(const void* q, int64_t q_bstride, const void* k, int
                             const int32_t* positions, int64_t pos_offset, float eps,
                             hipStream_t stream);
 
+/* Batch plan of a ragged step over a paged cache, on the GPU: sequence b brings
+ * q_lens[b] new tokens on top of past_lens[b] cached rows (past_lens NULL = 0;
+ * negative lengths count as 0).  The new tokens of all sequences lie back to back
+ * in T rows (tokens past row T are cut off).  With P = page_size, M = max_pages:
+ *   cu_seqlens [B+1]   first row of every sequence, then the number of rows used
+ *   kv_lens [B]        past + new tokens, at most M * P
+ *   positions [T]      past + i for token i of its sequence; -1 behind the last
+ *   slot_mapping [T]   int64: page id * P + position % P; -1 behind the last, at
+ *                      positions from M * P on, and where the page is missing
+ *   block_table [B, M] entries below ceil(past / P) are read and kept; those from
+ *                      there up to ceil(kv_len / P) are entered, the others left alone
+ * New pages are taken in order from free_pages[num_free], from index free_span[0]
+ * (head) up to free_span[1] (tail): sequence 0's pages first, in position order.
+ * Where the list ends, and for ids outside [0, num_pages), -1 is entered and the
+ * rows have no slot.  free_span_out [3] = head behind the pages taken, tail, and the
+ * pages needed: the plan is whole if needed <= tail - head.  free_span is not
+ * changed (free_span_out is another buffer), so a call with the same inputs gives
+ * the same plan.  B <= 4096, T < 2^30, M * P <= 2^30, num_pages < 2^31; page_size a
+ * power of two in [32, 2^20].  cu_seqlens and past_lens are what
+ * ezops_prefill_attn_bf16 takes, block_table and kv_lens what
+ * ezops_paged_attn_decode_bf16 takes.
+ * No counterpart in the reference (one contiguous cache,
+ * ezops/ops/attn_decode.py:60-61). */
+int ezops_paged_batch_plan(const int32_t* q_lens, const int32_t* past_lens, int32_t* block_table,
+                           const int32_t* free_pages, const int32_t* free_span, int32_t* cu_seqlens,
+                           int32_t* kv_lens, int32_t* positions, int64_t* slot_mapping,
+                           int32_t* free_span_out, int64_t B, int64_t T, int64_t page_size,
+                           int64_t max_pages, int64_t num_pages, int64_t num_free, hipStream_t stream);
+
+/* QK RMSNorm + rotary positions with several axes + paged cache write for T packed
+ * tokens (text, images, video).  q [T, H, D], k / v [T, Hkv, D] bf16 with token
+ * strides q_stride, k_stride, v_stride (elements); norm = 0: no RMSNorm, else over
+ * every q and k head with q_norm_w / k_norm_w [D] (NULL = unit).  positions [axes, T]
+ * int32, axes in [1, 4]; pair (i, i + D/2) turns by the position of its axis:
+ * sections [axes] (host memory) holds the number of pairs of each axis, D/2 in
+ * sum, as consecutive runs or (interleaved) pair i to axis i % axes while
+ * i < axes * sections[i % axes], else to axis 0.  cos / sin [S, D] in the HF layout
+ * (both halves equal; the first D/2 columns are read), bf16 or (table_f32) fp32.
+ * q_out [T, H, D]; k goes to k_out [T, Hkv, D] (may be NULL with a cache) and, with
+ * caches [num_pages, Hkv, page_size, D], with v to slot slot_mapping[t] =
+ * page * page_size + offset; slots outside the pool are skipped, and two tokens
+ * must not share one.  A token with a position outside [0, S) on any axis writes
+ * nothing.  q_out may be q (q_stride = H * D), k_out k.  D even, at most 512;
+ * page_size a power of two in [32, 2^20].
+ * No counterpart in the reference, which turns one token per sequence by one
+ * position (ezops/ops/fused_qk_norm_rope.py:7-169). */
+int ezops_qk_norm_mrope_bf16(const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                             const void* v, int64_t v_stride, const void* q_norm_w,
+                             const void* k_norm_w, int norm, const void* cos, const void* sin,
+                             int table_f32, const int32_t* positions, int64_t axes,
+                             const int64_t* sections, int interleaved, const int64_t* slot_mapping,
+                             void* K_cache, void* V_cache, int64_t num_pages, int64_t page_size,
+                             void* q_out, void* k_out, int64_t T, int64_t H, int64_t Hkv, int64_t D,
+                             int64_t S, float eps, hipStream_t stream);
+
+/* Linear attention with a decay per kv head over packed prompts:
+ *   S_t = exp(log_decay[kv head]) S_{t-1} + k_t v_t^T,  o_t = scale * q_t^T S_t
+ * q [T, H, D], k / v [T, Hkv, D] bf16 with token strides (elements, multiples of 8);
+ * sequence b owns rows cu_seqlens[b] .. cu_seqlens[b+1]-1 (clamped into [0, T]; the
+ * offsets must not decrease), of which the first max_q_len count (0 = T).  out
+ * [T, H, D] bf16.  state [num_slots, Hkv, D, D] fp32 (NULL: none, every sequence
+ * starts from zero and leaves no state): sequence b continues from slot
+ * state_slots[b] (NULL = slot b) if past_lens[b] > 0 (past_lens NULL = 0 for all),
+ * starts from zero otherwise, and leaves its last state there; a sequence without
+ * tokens leaves it alone.  A sequence whose slot is outside the pool, or that an
+ * earlier sequence of the batch holds already, is left out whole (no row of out and
+ * no state is written); rows of no sequence are not written.  log_decay [Hkv] fp32,
+ * at most 0 (-inf: no memory).  H / Hkv in {1, 2, 4, 8, 16}, D in {64, 128}; q, k, v,
+ * out, state and workspace 16-byte aligned; B <= 65536, T < 2^30; scale <= 0 selects
+ * 1/sqrt(D).  The workspace (ezops_linear_attn_prefill_workspace_size bytes, 0 for
+ * some shapes) need not be zero-filled.
+ * No counterpart in the reference (softmax attention only,
+ * ezops/ops/attn_decode.py:9-67). */
+size_t ezops_linear_attn_prefill_workspace_size(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t D,
+                                                int64_t max_q_len);
+int ezops_linear_attn_prefill_bf16(const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                                   const void* v, int64_t v_stride, const float* log_decay,
+                                   const int32_t* cu_seqlens, const int32_t* past_lens, float* state,
+                                   const int32_t* state_slots, int64_t num_slots, void* out, int64_t B,
+                                   int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t max_q_len,
+                                   float scale, void* workspace, size_t workspace_bytes,
+                                   hipStream_t stream);
+
+/* The recurrent form: one token per sequence, q [B, H, D], k / v [B, Hkv, D] (row
+ * strides in elements, multiples of 8), the state required and updated in place,
+ * slots as above.  out [B, H, D] bf16.
+ * No counterpart in the reference (softmax attention only,
+ * ezops/ops/attn_decode.py:9-67). */
+int ezops_linear_attn_decode_bf16(const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                                  const void* v, int64_t v_stride, const float* log_decay, float* state,
+                                  const int32_t* state_slots, int64_t num_slots, void* out, int64_t B,
+                                  int64_t H, int64_t Hkv, int64_t D, float scale, hipStream_t stream);
+
 /* Fused o_proj + post-norm + SwiGLU FFN (batch x 1 token), bf16:
  *   x2 = residual + attn @ Wo^T ; xn = rmsnorm(x2) * post_norm_w
  *   out = x2 + (silu(xn @ Wg^T) * (xn @ Wu^T)) @ Wd^T
@@ -333,7 +426,8 @@ int ezops_gemm_swiglu_bf16(const void* X, int64_t ldx, const void* Wgu, void* Y,
  *   uint16 kernel   kernel id (1 gemv_rows, 2 gemv_valu, 3 linear_scalar, 4 linear_mfma,
  *                   5 attn_split, 6 attn_combine, 7 prefill_attn, 8 silu_mul,
  *                   9 qk_norm_rope, 10 rmsnorm_f32, 11 rmsnorm_bf16, 12 softmax, 13 sum,
- *                   14 gemm)
+ *                   14 gemm, 15 batch_plan, 16 qk_norm_mrope, 17 linear_attn_prefill,
+ *                   18 linear_attn_decode, 19 linear_attn_state)
  *   uint16 wave     wave index in its block;  uint32 block  blockIdx.x
  * ezops_profile_reset clears the buffers; ezops_profile_read copies up to
  * `capacity` records to host memory and returns how many (both synchronise
