@@ -10,6 +10,8 @@
 // A sequence's state lives in a pool of slots.  A sequence whose slot lies
 // outside the pool, or that an earlier sequence of the batch holds already, is
 // left out whole: nothing of it is read or written, so equal slots make no race.
+#include <type_traits>
+
 #include "common.h"
 #include "internal.h"
 #include "prof.h"
@@ -30,9 +32,29 @@ struct LinAttnArgs {
   const int32_t *cu, *past;   // prefill: [B + 1], [B] or NULL
   uint16_t* out;              // [T, H, D]
   int64_t T, num_slots, max_q;
+  int64_t seg, segments;      // prefill: tokens per segment, segment numbers
+  float* ws;                  // prefill: [segments, Hkv, D, D] or NULL (one segment a sequence)
   int B, H, Hkv;
   float scale;
 };
+
+// What a state keeps over n tokens, lambda^n S: where lambda^n > 1/2 as S + (lambda^n - 1) S, so that
+// the factor's own rounding does not build up over many steps as that of lambda^n itself would (a
+// state that is all but kept adds it up 1 / (1 - lambda^n) times); below that as the plain product,
+// which the sum would cancel in.
+struct Keep {
+  float m;
+  bool near;
+};
+__device__ __forceinline__ Keep keep_over(float log_decay, float n) {
+  const float m = expm1f(log_decay * n);
+  return m > -0.5f ? Keep{m, true} : Keep{expf(log_decay * n), false};
+}
+// lambda^n S + x
+__device__ __forceinline__ float decayed(const Keep& k, float S, float x) {
+  const float y = fmaf(k.m, S, x);
+  return k.near ? S + y : y;
+}
 
 // Slot of sequence b, -1 if it has none: outside the pool, or held by an earlier
 // sequence.  Every thread of the block calls it (barrier inside).
@@ -47,47 +69,499 @@ __device__ __forceinline__ int slot_of(const LinAttnArgs& a, int b) {
   return s < 0 || s >= a.num_slots || dup ? -1 : s;
 }
 
-// One block per (sequence, kv head), thread = column of v: its column of the state
-// in D registers, token by token.
+// ---- prompts: the chunked form ------------------------------------------
+// A chunk of 64 tokens with state S before it, everything decayed relative to
+// one of its ends, so that only powers n >= 0 appear:
+//   o_i   = scale (lambda^{i+1} S^T q_i + sum_{j<=i} lambda^{i-j} (q_i . k_j) v_j)
+//   S_out = lambda^n S + sum_j lambda^{n-1-j} k_j v_j^T
+// A sequence is cut into segments of `seg` tokens that end at its end; only the
+// first chunk of its first segment can be short, and it is filled up with zero
+// tokens at its front, which leaves every power below the same for all chunks.
+//
+// With one segment a sequence the output kernel alone runs (state from the pool,
+// state to the pool).  Otherwise: the state kernel sums every segment but the last
+// from zero into the workspace, the scan turns these sums into the state before
+// each segment, and the output kernel starts each segment from there.
+//
+// Matrix layout (v_mfma_f32_32x32x16_bf16: lane 32h+i holds A[i][8h..8h+7] and
+// B[8h..8h+7][i]; register r of lane 32h+j holds C[8(r/4)+4h+r%4][j]).  Wave w owns
+// columns 32w..32w+31 of v, of the state and of the outputs:
+//   P^T = K Q^T         keys x queries; its registers are the B operand of the next
+//                       product as they are, if the token slots 8h..8h+7 of a 16-key
+//                       step mean keys 4h..4h+3 and 8+4h..8+4h+3
+//   O^T += V^T P^T      A = V^T by transposing LDS reads in that token order
+//   S   += K^T (w V)    the same V registers, weighted, are the B operand; A = K^T by
+//                       transposing reads whose dims come in the order that makes
+//                       registers 8u..8u+7 of S dims 16u+8h..+7:
+//   O^T += S^T Q^T      S's registers are the A operand with the dims in natural order,
+//                       so one set of Q registers serves both products
+// The three 32 x 32 blocks of P are shared out among the waves and handed round through LDS.
+// fp32 operands (P, S, w V) are given to the matrix cores in bf16 parts: two for P and
+// S, whose products end in one bf16 rounding (2^-16 of a term against 2^-8), three for
+// w V, whose sums are the fp32 state (2^-24).
+constexpr int kC = 64;  // tokens per chunk
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef int i32x2_t __attribute__((ext_vector_type(2)));
+
+// 16-byte chunk c of row `key` of an LDS tile lies at chunk c ^ swizzle(key): the row
+// reads (32 rows, one chunk) and the transposing reads (4 rows x 64 bytes per half
+// wave) both spread over all banks.
 template <int D>
-__global__ __launch_bounds__(D) void linear_attn_prefill_kernel(LinAttnArgs a) {
-  EZ_PROF_WAVE(kProfLinAttnPrefill);
-  __shared__ float ks[D], qs[16][D];
-  const int b = blockIdx.x / a.Hkv, kvh = blockIdx.x % a.Hkv, tid = threadIdx.x, G = a.H / a.Hkv;
-  const int64_t t0 = min(max(int64_t(a.cu[b]), int64_t(0)), a.T);
-  const int64_t t1 = min(min(int64_t(a.cu[b + 1]), a.T), t0 + a.max_q);
-  int slot = -1;
-  if (a.state) {
-    slot = slot_of<D>(a, b);
-    if (slot < 0) return;
+__device__ __forceinline__ int swizzle(int key) {
+  return D == 128 ? ((key & 3) << 2) | ((key >> 2) & 3) : (((key >> 1) & 1) << 2) | ((key >> 2) & 3);
+}
+
+// LDS reads as asm blocks that end in their own wait: the compiler would make an
+// ordinary read wait for the next chunk's LDS DMA as well.
+// All dims of 32 token rows (N = D / 16 steps), `a` = this lane's first chunk.
+template <int OFF>
+__device__ __forceinline__ void lds_row(uint32_t a, bf16x8_t (&r)[8]) {
+  asm volatile(
+      "ds_read_b128 %0, %8 offset:%16\n\tds_read_b128 %1, %9 offset:%16\n\t"
+      "ds_read_b128 %2, %10 offset:%16\n\tds_read_b128 %3, %11 offset:%16\n\t"
+      "ds_read_b128 %4, %12 offset:%16\n\tds_read_b128 %5, %13 offset:%16\n\t"
+      "ds_read_b128 %6, %14 offset:%16\n\tds_read_b128 %7, %15 offset:%16\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
+      : "v"(a), "v"(a ^ 32), "v"(a ^ 64), "v"(a ^ 96), "v"(a ^ 128), "v"(a ^ 160), "v"(a ^ 192), "v"(a ^ 224), "i"(OFF));
+}
+template <int OFF>
+__device__ __forceinline__ void lds_row(uint32_t a, bf16x8_t (&r)[4]) {
+  asm volatile(
+      "ds_read_b128 %0, %4 offset:%8\n\tds_read_b128 %1, %5 offset:%8\n\t"
+      "ds_read_b128 %2, %6 offset:%8\n\tds_read_b128 %3, %7 offset:%8\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3])
+      : "v"(a), "v"(a ^ 32), "v"(a ^ 64), "v"(a ^ 96), "i"(OFF));
+}
+// Transposing reads (ds_read_b64_tr_b16: in each 16-lane group, lane m receives element
+// m % 4 of the 8-byte rows that lanes m/4, 4 + m/4, 8 + m/4 and 12 + m/4 address): tokens
+// 16s + 4h..+3 and 8 further on (row pitch P bytes) of 32 dims a tile.
+// One 32-dim tile, all four 16-token steps.
+template <int P>
+__device__ __forceinline__ void lds_tr_steps(uint32_t a, i32x2_t (&r)[8]) {
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8 offset:%10\n\tds_read_b64_tr_b16 %1, %9 offset:%11\n\t"
+      "ds_read_b64_tr_b16 %2, %8 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+      "ds_read_b64_tr_b16 %4, %8 offset:%14\n\tds_read_b64_tr_b16 %5, %9 offset:%15\n\t"
+      "ds_read_b64_tr_b16 %6, %8 offset:%16\n\tds_read_b64_tr_b16 %7, %9 offset:%17\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
+      : "v"(a), "v"(a ^ 32), "i"(0), "i"(8 * P), "i"(16 * P), "i"(24 * P), "i"(32 * P), "i"(40 * P), "i"(48 * P),
+        "i"(56 * P));
+}
+// One 16-token step, all 32-dim tiles.
+template <int OFF, int P>
+__device__ __forceinline__ void lds_tr_tiles(uint32_t a, i32x2_t (&r)[8]) {
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8 offset:%16\n\tds_read_b64_tr_b16 %1, %9 offset:%17\n\t"
+      "ds_read_b64_tr_b16 %2, %10 offset:%16\n\tds_read_b64_tr_b16 %3, %11 offset:%17\n\t"
+      "ds_read_b64_tr_b16 %4, %12 offset:%16\n\tds_read_b64_tr_b16 %5, %13 offset:%17\n\t"
+      "ds_read_b64_tr_b16 %6, %14 offset:%16\n\tds_read_b64_tr_b16 %7, %15 offset:%17\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
+      : "v"(a), "v"(a ^ 32), "v"(a ^ 64), "v"(a ^ 96), "v"(a ^ 128), "v"(a ^ 160), "v"(a ^ 192), "v"(a ^ 224), "i"(OFF),
+        "i"(OFF + 8 * P));
+}
+template <int OFF, int P>
+__device__ __forceinline__ void lds_tr_tiles(uint32_t a, i32x2_t (&r)[4]) {
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %4 offset:%8\n\tds_read_b64_tr_b16 %1, %5 offset:%9\n\t"
+      "ds_read_b64_tr_b16 %2, %6 offset:%8\n\tds_read_b64_tr_b16 %3, %7 offset:%9\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3])
+      : "v"(a), "v"(a ^ 32), "v"(a ^ 64), "v"(a ^ 96), "i"(OFF), "i"(OFF + 8 * P));
+}
+// Four 1 KiB fragments in a row (16 bytes a lane).
+__device__ __forceinline__ void lds_frags4(uint32_t a, bf16x8_t (&r)[4]) {
+  asm volatile(
+      "ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:1024\n\tds_read_b128 %2, %4 offset:2048\n\t"
+      "ds_read_b128 %3, %4 offset:3072\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3])
+      : "v"(a));
+}
+__device__ __forceinline__ void lds_write_frags4(uint32_t a, const bf16x8_t (&r)[4]) {
+  asm volatile(
+      "ds_write_b128 %0, %1\n\tds_write_b128 %0, %2 offset:1024\n\tds_write_b128 %0, %3 offset:2048\n\t"
+      "ds_write_b128 %0, %4 offset:3072\n\ts_waitcnt lgkmcnt(0)"
+      :
+      : "v"(a), "v"(r[0]), "v"(r[1]), "v"(r[2]), "v"(r[3])
+      : "memory");
+}
+__device__ __forceinline__ bf16x8_t join(const i32x2_t& x, const i32x2_t& y) {
+  return as_bf16x8(make_uint4(uint32_t(x[0]), uint32_t(x[1]), uint32_t(y[0]), uint32_t(y[1])));
+}
+
+// The next bf16 part of eight values: returned rounded, and taken off them.
+__device__ __forceinline__ bf16x8_t take_part(float (&x)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    w[e] = cvt_bf2(x[2 * e], x[2 * e + 1]);
+    x[2 * e] -= bf_lo(w[e]);
+    x[2 * e + 1] -= bf_hi(w[e]);
   }
-  if (t0 >= t1) return;
-  float* st = a.state ? a.state + (int64_t(slot) * a.Hkv + kvh) * D * D + tid : nullptr;
-  const bool cont = st && a.past && a.past[b] > 0;
-  const float lambda = __expf(a.log_decay[kvh]);
-  float S[D];
+  return as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
+}
+__device__ __forceinline__ bf16x8_t last_part(const float (&x)[8]) {
+  return as_bf16x8(make_uint4(cvt_bf2(x[0], x[1]), cvt_bf2(x[2], x[3]), cvt_bf2(x[4], x[5]), cvt_bf2(x[6], x[7])));
+}
+
+// An LDS address of this chunk's buffer.  Opaque to the compiler, which would else keep every
+// address derived from it in a register of its own throughout the loop.
+__device__ __forceinline__ uint32_t lds_at(uint32_t base, uint32_t off) {
+  uint32_t a = base + off;
+  asm volatile("" : "+v"(a));
+  return a;
+}
+
+// lambda^n, n >= 0, from log2(lambda); lambda^0 = 1 for lambda = 0 too.
+__device__ __forceinline__ float power(float g2, int n) { return n == 0 ? 1.f : __builtin_amdgcn_exp2f(g2 * float(n)); }
+
+// Segment numbers: sequence b's segments are numbers cu[b] / seg + b, + 1, ...: distinct
+// for distinct sequences, and at most T / seg + B in all, so the host knows the grid.
+struct Segment {
+  int b, s, count;     // sequence, index in it, its number of segments
+  int slot;            // state slot (-1: no pool)
+  bool cont;           // the sequence starts from its stored state
+  int64_t row;         // first row of the segment
+  int len, before;     // tokens, tokens of the segment before it
+};
+
+// Finds segment number `id`; false if there is none (every thread agrees).  Contains barriers.
+template <int THREADS>
+__device__ __forceinline__ bool find_segment(const LinAttnArgs& a, int64_t id, Segment& g) {
+  __shared__ int64_t s_row[2];
+  __shared__ int s_slot, s_past;
+  int count = 0;  // sequences whose first segment number is at most id: the last of them is ours
+  for (int c0 = 0; c0 < a.B; c0 += THREADS) {
+    const int c = c0 + threadIdx.x;
+    bool in = false;
+    if (c < a.B) {
+      const int64_t r = min(max(int64_t(a.cu[c]), int64_t(0)), a.T);
+      in = r / a.seg + c <= id;
+    }
+    count += __syncthreads_count(in);
+  }
+  const int b = count - 1;
+  if (b < 0) return false;
+  if (threadIdx.x == 0) {
+    s_row[0] = min(max(int64_t(a.cu[b]), int64_t(0)), a.T);
+    s_row[1] = min(int64_t(a.cu[b + 1]), a.T);
+    s_slot = a.state ? (a.state_slots ? a.state_slots[b] : b) : -1;
+    s_past = a.past ? a.past[b] : 0;
+  }
+  __syncthreads();
+  const int64_t r0 = s_row[0], n = min(s_row[1] - r0, a.max_q);
+  int slot = s_slot;
+  if (a.state) {
+    int dup = slot < 0 || slot >= a.num_slots;
+    if (a.state_slots)
+      for (int c = threadIdx.x; c < b; c += THREADS) dup |= a.state_slots[c] == slot;
+    if (__syncthreads_or(dup)) return false;
+  }
+  const int64_t s = id - (r0 / a.seg + b);
+  if (n <= 0 || s < 0 || s * a.seg >= n) return false;
+  const int cnt = int((n + a.seg - 1) / a.seg);
+  const int first = int(n - int64_t(cnt - 1) * a.seg);  // 1 .. seg
+  g.b = b;
+  g.s = int(s);
+  g.count = cnt;
+  g.slot = slot;
+  g.cont = a.state && s_past > 0;
+  g.row = r0 + (s ? first + (s - 1) * a.seg : 0);
+  g.len = s ? int(a.seg) : first;
+  g.before = s > 1 ? int(a.seg) : first;
+  return true;
+}
+
+// OUT: the outputs of a segment (and, of a sequence's last one, its last state);
+// otherwise the sum of a segment from a zero state.  Block = (segment, kv head).
+template <int D, bool OUT>
+__global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void linear_attn_chunk_kernel(LinAttnArgs a) {
+  EZ_PROF_WAVE(OUT ? kProfLinAttnPrefill : kProfLinAttnState);
+  constexpr int THREADS = 2 * D, NT = D / 32, NK = D / 16, P = 2 * D;  // P: bytes of an LDS row
+  constexpr int TILE = kC * P, LPT = TILE / 16 / THREADS;
+  __shared__ __align__(16) uint16_t Ks[2][kC * D], Vs[2][kC * D];
+  __shared__ __align__(16) uint16_t Ps[OUT ? 3 * 4 * 512 : 8];  // block of P x (16-key step, part) x lane x 8
+  const int64_t id = blockIdx.x / a.Hkv;
+  const int kvh = blockIdx.x % a.Hkv;
+  Segment sg;
+  if (!find_segment<THREADS>(a, id, sg)) return;
+  if (!OUT && sg.s == sg.count - 1) return;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int h = lane >> 5, j = lane & 31;
+  const int chunks = (sg.len + kC - 1) / kC, pad = chunks * kC - sg.len;
+  const float g = a.log_decay[kvh], g2 = g * 1.4426950408889634f;
+
+  // state of this wave's columns: register r of tile t = S[32t + 16(r/8) + 8h + r%8][32w + j]
+  f32x16_t S[NT];
 #pragma unroll
-  for (int i = 0; i < D; ++i) S[i] = cont ? st[i * D] : 0.f;
-  for (int64_t t = t0; t < t1; ++t) {
-    __syncthreads();
-    ks[tid] = bf2f(a.k[t * a.k_rs + kvh * D + tid]);
-    for (int g = 0; g < G; ++g) qs[g][tid] = bf2f(a.q[t * a.q_rs + (kvh * G + g) * D + tid]);
-    const float v = bf2f(a.v[t * a.v_rs + kvh * D + tid]);
-    __syncthreads();
+  for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int i = 0; i < D; ++i) S[i] = lambda * S[i] + ks[i] * v;
-    for (int g = 0; g < G; ++g) {
-      float o = 0.f;
+    for (int r = 0; r < 16; ++r) S[t][r] = 0.f;
+  const int64_t elem = int64_t(8 * h) * D + 32 * w + j;
+  float* pool = sg.slot >= 0 ? a.state + (int64_t(sg.slot) * a.Hkv + kvh) * D * D + elem : nullptr;
+  float* ws = a.ws + (id * a.Hkv + kvh) * D * D + elem;
+  if (OUT && (sg.s > 0 || sg.cont)) {
+    const float* src = sg.count > 1 ? ws : pool;
 #pragma unroll
-      for (int i = 0; i < D; ++i) o += qs[g][i] * S[i];
-      a.out[(t * a.H + kvh * G + g) * D + tid] = f2bf(o * a.scale);
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) S[t][r] = src[(32 * t + 16 * (r >> 3) + (r & 7)) * D];
+  }
+
+  // powers: wv[e] = lambda^(15 - token) of the tokens of a 16-token step; pm = scale * lambda^(query - key)
+  // of this wave's block of P: on the diagonal (blocks 0 and 2) or below it (block 1)
+  const bool diag = D == 64 ? w == 0 : w != 1;
+  float wv[8], pm[16];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) wv[e] = power(g2, 15 - (8 * (e >> 2) + 4 * h + (e & 3)));
+  if constexpr (OUT) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int ago = (diag ? 0 : 32) + j - (8 * (r >> 2) + 4 * h + (r & 3));
+      pm[r] = ago >= 0 ? a.scale * power(g2, max(ago, 0)) : 0.f;
     }
   }
-  if (st) {
+
+  // staging: LDS chunk p = THREADS c + tid holds 16-byte chunk (p % (D/8)) ^ swizzle of row
+  // p / (D/8).  Buffer loads: rows in front of the segment lie past the resource's end as
+  // unsigned offsets and read as zeros.
+  constexpr int RPL = THREADS / (D / 8);  // rows per load of the block: 16, which the swizzle does not see
+  static_assert(RPL == 16 && LPT * RPL == kC, "staging covers the chunk");
+  const int srow = tid / (D / 8), sch = (tid % (D / 8)) ^ swizzle<D>(srow);
+  const uint32_t krow = uint32_t(srow) * uint32_t(2 * a.k_rs) + 16 * sch;
+  const uint32_t vrow = uint32_t(srow) * uint32_t(2 * a.v_rs) + 16 * sch;
+  auto load_chunk = [&](int c) {
+    const int r0 = c * kC - pad;  // first row of the chunk in the segment; negative in a short first chunk
+    const int rb = max(r0, 0), back = rb - r0, rows = kC - back;
+    const uint16_t* kp = a.k + (sg.row + rb) * a.k_rs + kvh * D;
+    const uint16_t* vp = a.v + (sg.row + rb) * a.v_rs + kvh * D;
+    const auto kres = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(kp), 0, int(rows * 2 * a.k_rs), 0x00020000);
+    const auto vres = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(vp), 0, int(rows * 2 * a.v_rs), 0x00020000);
 #pragma unroll
-    for (int i = 0; i < D; ++i) st[i * D] = S[i];
+    for (int i = 0; i < LPT; ++i) {
+      const int at = (i * THREADS + w * kWave) * 8;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(kres, (__attribute__((address_space(3))) void*)(&Ks[c & 1][at]), 16,
+                                               krow + uint32_t(i * RPL - back) * uint32_t(2 * a.k_rs), 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(vres, (__attribute__((address_space(3))) void*)(&Vs[c & 1][at]), 16,
+                                               vrow + uint32_t(i * RPL - back) * uint32_t(2 * a.v_rs), 0, 0, 0);
+    }
+  };
+
+  // LDS read addresses in buffer 0
+  const uint32_t kbase = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint16_t*)(&Ks[0][0])));
+  const uint32_t vbase = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint16_t*)(&Vs[0][0])));
+  const uint32_t krd = kbase + uint32_t(j * P + ((h ^ swizzle<D>(j)) << 4));
+  const int mm = lane & 15, g1 = (lane >> 4) & 1, trow = 4 * h + (mm >> 2), gm = mm & 3;
+  const int kg = ((gm & 1) << 1) | (gm >> 1);  // dim groups 0, 2, 1, 3
+  const uint32_t ktr = kbase + uint32_t(trow * P + (((2 * g1 + (kg >> 1)) ^ swizzle<D>(trow)) << 4) + 8 * (kg & 1));
+  const uint32_t vtr = vbase + uint32_t(trow * P + (((4 * w + 2 * g1 + (gm >> 1)) ^ swizzle<D>(trow)) << 4) + 8 * (gm & 1));
+
+  const uint32_t pfr = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint16_t*)(&Ps[0]))) +
+                       uint32_t(lane * 16);
+
+  const int G = a.H / a.Hkv;
+  bf16x8_t q[2][NK];  // queries of the chunk's two halves, the next head's as soon as these are used
+  auto load_q = [&](int c, int hg) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint16_t* qp =
+          a.q + (sg.row + max(c * kC - pad + 32 * t + j, 0)) * a.q_rs + (kvh * G + hg) * D + 8 * h;
+#pragma unroll
+      for (int s = 0; s < NK; ++s) q[t][s] = as_bf16x8(*reinterpret_cast<const uint4*>(qp + 16 * s));
+    }
+  };
+  // one 32 x 32 block of P (keys of half KT) into LDS slot `blk`
+  auto make_p = [&](auto ktc, const bf16x8_t(&qt)[NK], uint32_t buf, int blk) {
+    constexpr int KT = decltype(ktc)::value;
+    bf16x8_t kf[NK], pf[4];
+    lds_row<KT * 32 * P>(lds_at(krd, buf), kf);
+    f32x16_t st;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) st[r] = 0.f;
+#pragma unroll
+    for (int s = 0; s < NK; ++s) st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[s], qt[s], st, 0, 0, 0);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int r = 8 * u + e;
+        // keys behind the query give nothing, whatever they hold
+        x[e] = !diag || j >= 8 * (r >> 2) + 4 * h + (r & 3) ? st[r] * pm[r] : 0.f;
+      }
+      pf[2 * u] = take_part(x);
+      pf[2 * u + 1] = last_part(x);
+    }
+    lds_write_frags4(pfr + 4096 * blk, pf);
+  };
+  if constexpr (OUT) load_q(0, 0);
+  load_chunk(0);
+  wait_vm<0>();
+  __syncthreads();
+  for (int c = 0; c < chunks; ++c) {
+    const uint32_t buf = uint32_t(c & 1) * TILE;
+    const int r0 = c * kC - pad;
+    if (c + 1 < chunks) load_chunk(c + 1);
+    i32x2_t vf[8];
+    lds_tr_steps<P>(lds_at(vtr, buf), vf);
+    if constexpr (OUT) {
+      for (int hg = 0; hg < G; ++hg) {
+        const int hq = kvh * G + hg;
+        if (w == 0) make_p(std::integral_constant<int, 0>{}, q[0], buf, 0);
+        if (w == 1) make_p(std::integral_constant<int, 0>{}, q[1], buf, 1);
+        if (w == (D == 64 ? 0 : 2)) make_p(std::integral_constant<int, 1>{}, q[1], buf, 2);
+        __builtin_amdgcn_sched_barrier(0);
+        // what the state gives, scaled by lambda^(i+1) of the query.  The parts of S are made anew for
+        // every head (S is opaque here): kept, they would take the registers of S a second time.
+#pragma unroll
+        for (int t = 0; t < NT; ++t) asm volatile("" : "+v"(S[t]));
+        f32x16_t o[2];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[0][r] = o[1][r] = 0.f;
+#pragma unroll
+        for (int s = 0; s < NK; ++s) {
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = S[s >> 1][8 * (s & 1) + e];
+          const bf16x8_t hi = take_part(x), lo = last_part(x);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi, q[t][s], o[t], 0, 0, 0);
+            o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lo, q[t][s], o[t], 0, 0, 0);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if (hg + 1 < G) load_q(c, hg + 1);
+        else if (c + 1 < chunks) load_q(c + 1, 0);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const float f = a.scale * power(g2, max(r0 + 32 * t + j - max(r0, 0) + 1, 0));
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[t][r] *= f;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        __syncthreads();  // P is there
+        // what the chunk's own tokens give
+#pragma unroll
+        for (int blk = 0; blk < 3; ++blk) {
+          bf16x8_t pf[4];
+          lds_frags4(pfr + 4096 * blk, pf);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int t = blk > 0, step = 2 * (blk == 2) + u;
+            const bf16x8_t va = join(vf[2 * step], vf[2 * step + 1]);
+            o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, pf[2 * u], o[t], 0, 0, 0);
+            o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, pf[2 * u + 1], o[t], 0, 0, 0);
+          }
+        }
+        if (hg + 1 < G) __syncthreads();  // P has been read
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int row = r0 + 32 * t + j;
+          if (row >= 0) {
+            uint16_t* op = a.out + ((sg.row + row) * a.H + hq) * D + 32 * w + 4 * h;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              *reinterpret_cast<uint2*>(op + 8 * e) = make_uint2(cvt_bf2(o[t][4 * e], o[t][4 * e + 1]),
+                                                                 cvt_bf2(o[t][4 * e + 2], o[t][4 * e + 3]));
+          }
+        }
+      }
+    }
+    const Keep keep = keep_over(g, float(min(r0 + kC, kC)));
+    if (keep.near) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) S[t][r] = fmaf(S[t][r], keep.m, S[t][r]);
+    } else {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) S[t][r] *= keep.m;
+    }
+    auto add_step = [&](auto sc) {
+      constexpr int s = decltype(sc)::value;
+      float x[8];
+      float f = power(g2, 48 - 16 * s);
+      asm volatile("" : "+v"(f));  // keeps the products f * wv out of registers of their own
+      unpack8(__builtin_bit_cast(uint4, join(vf[2 * s], vf[2 * s + 1])), x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] *= wv[e] * f;
+      const bf16x8_t hi = take_part(x), mid = take_part(x), lo = last_part(x);
+      i32x2_t kf[2 * NT];
+      lds_tr_tiles<16 * s * P, P>(lds_at(ktr, buf), kf);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const bf16x8_t ka = join(kf[2 * t], kf[2 * t + 1]);
+        S[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka, lo, S[t], 0, 0, 0);
+        S[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka, mid, S[t], 0, 0, 0);
+        S[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka, hi, S[t], 0, 0, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    add_step(std::integral_constant<int, 0>{});
+    add_step(std::integral_constant<int, 1>{});
+    add_step(std::integral_constant<int, 2>{});
+    add_step(std::integral_constant<int, 3>{});
+    wait_vm<0>();  // the next chunk has landed
+    __syncthreads();
+  }
+  float* dst = OUT ? (sg.s == sg.count - 1 ? pool : nullptr) : id + 1 < a.segments ? ws + int64_t(a.Hkv) * D * D : nullptr;
+  if (dst) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dst[(32 * t + 16 * (r >> 3) + (r & 7)) * D] = S[t][r];
   }
 }
+
+// The workspace's slot of segment s > 0 holds the sum of segment s - 1; becomes the state
+// before segment s.  Slot 0 gets the stored state where the sequence continues (the output
+// kernel's last segment overwrites the pool while its first may still have to start).
+// Block = (sequence, kv head, 1024 elements).
+template <int D>
+__global__ __launch_bounds__(256) void linear_attn_scan_kernel(LinAttnArgs a) {
+  EZ_PROF_WAVE(kProfLinAttnState);
+  constexpr int PARTS = D * D / 1024;
+  const int part = blockIdx.x % PARTS, kvh = blockIdx.x / PARTS % a.Hkv, b = blockIdx.x / PARTS / a.Hkv;
+  const int64_t r0 = min(max(int64_t(a.cu[b]), int64_t(0)), a.T);
+  const int64_t n = min(min(int64_t(a.cu[b + 1]), a.T) - r0, a.max_q);
+  if (n <= a.seg) return;
+  int slot = -1;
+  if (a.state) {
+    slot = slot_of<256>(a, b);
+    if (slot < 0) return;
+  }
+  const int64_t cnt = (n + a.seg - 1) / a.seg, id = r0 / a.seg + b;
+  const int64_t last = min(cnt, a.segments - id);  // a table of decreasing offsets must not lead past the workspace
+  const int64_t at = int64_t(part) * 1024 + 4 * threadIdx.x, step = int64_t(a.Hkv) * D * D;
+  float* ws = a.ws + (id * a.Hkv + kvh) * D * D + at;
+  float4 S = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (slot >= 0 && a.past && a.past[b] > 0) {
+    S = *reinterpret_cast<const float4*>(a.state + (int64_t(slot) * a.Hkv + kvh) * D * D + at);
+    *reinterpret_cast<float4*>(ws) = S;
+  }
+  const float g = a.log_decay[kvh];
+  const Keep first = keep_over(g, float(n - (cnt - 1) * a.seg)), rest = keep_over(g, float(a.seg));
+  for (int64_t s = 1; s < last; ++s) {
+    float4* p = reinterpret_cast<float4*>(ws + s * step);
+    const Keep f = s == 1 ? first : rest;
+    const float4 x = *p;
+    S.x = decayed(f, S.x, x.x);
+    S.y = decayed(f, S.y, x.y);
+    S.z = decayed(f, S.z, x.z);
+    S.w = decayed(f, S.w, x.w);
+    *p = S;
+  }
+}
+
+// Tokens per segment: as long as that still gives about 512 blocks (two a CU) over the
+// whole batch, at least a chunk.
+int64_t segment_tokens(int64_t T, int64_t Hkv) {
+  const int64_t want = (T * Hkv + 511) / 512;
+  return (want + kC - 1) / kC * kC;
+}
+int64_t segment_count(int64_t B, int64_t T, int64_t seg) { return T / seg + B; }
 
 // One token per sequence: block = (sequence, kv head, slice of VC columns of the
 // state), the slice in registers between its one read and its one write.
@@ -108,7 +582,7 @@ __global__ __launch_bounds__(256) void linear_attn_decode_kernel(LinAttnArgs a) 
   float4 S[NI];
 #pragma unroll
   for (int i = 0; i < NI; ++i) S[i] = st[(r0 + i * RPI) * (D / 4)];
-  const float lambda = __expf(a.log_decay[kvh]);
+  const Keep keep = keep_over(a.log_decay[kvh], 1.f);
   for (int i = tid; i < D; i += 256) ks[i] = bf2f(a.k[b * a.k_rs + kvh * D + i]);
   for (int i = tid; i < G * D; i += 256) qs[i / D][i % D] = bf2f(a.q[b * a.q_rs + kvh * G * D + i]) * a.scale;
   const uint2 vr = *reinterpret_cast<const uint2*>(a.v + b * a.v_rs + kvh * D + sl * VC + 4 * c);
@@ -117,10 +591,10 @@ __global__ __launch_bounds__(256) void linear_attn_decode_kernel(LinAttnArgs a) 
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
     const float kk = ks[r0 + i * RPI];
-    S[i].x = lambda * S[i].x + kk * v.x;
-    S[i].y = lambda * S[i].y + kk * v.y;
-    S[i].z = lambda * S[i].z + kk * v.z;
-    S[i].w = lambda * S[i].w + kk * v.w;
+    S[i].x = decayed(keep, S[i].x, kk * v.x);
+    S[i].y = decayed(keep, S[i].y, kk * v.y);
+    S[i].z = decayed(keep, S[i].z, kk * v.z);
+    S[i].w = decayed(keep, S[i].w, kk * v.w);
     st[(r0 + i * RPI) * (D / 4)] = S[i];
   }
   for (int g = 0; g < G; ++g) {
@@ -165,7 +639,10 @@ int check_common(const LinAttnArgs& a, int64_t H, int64_t Hkv, int64_t D, const 
 
 extern "C" size_t ezops_linear_attn_prefill_workspace_size(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t D,
                                                            int64_t max_q_len) {
-  return 0;
+  if (B < 1 || T < 1 || Hkv < 1 || D < 1) return 0;
+  const int64_t seg = ez::segment_tokens(T, Hkv);
+  if ((max_q_len > 0 && max_q_len < T ? max_q_len : T) <= seg) return 0;
+  return size_t(ez::segment_count(B, T, seg)) * Hkv * D * D * sizeof(float);
 }
 
 extern "C" int ezops_linear_attn_prefill_bf16(const void* q, int64_t q_stride, const void* k, int64_t k_stride,
@@ -194,8 +671,30 @@ extern "C" int ezops_linear_attn_prefill_bf16(const void* q, int64_t q_stride, c
   EZ_REQUIRE(max_q_len >= 0, "linear_attn_prefill: max_q_len must be >= 0");
   a.B = int(B); a.H = int(H); a.Hkv = int(Hkv);
   a.scale = scale > 0.f ? scale : 1.f / sqrtf(float(D));
-  if (D == 64) hipLaunchKernelGGL(ez::linear_attn_prefill_kernel<64>, dim3(unsigned(B * Hkv)), dim3(64), 0, stream, a);
-  else hipLaunchKernelGGL(ez::linear_attn_prefill_kernel<128>, dim3(unsigned(B * Hkv)), dim3(128), 0, stream, a);
+  EZ_REQUIRE(q_stride < (1 << 23) && k_stride < (1 << 23) && v_stride < (1 << 23),
+             "linear_attn_prefill: token strides must be below 2^23");
+  a.seg = ez::segment_tokens(T, Hkv);
+  a.segments = ez::segment_count(B, T, a.seg);
+  const size_t need = ezops_linear_attn_prefill_workspace_size(B, T, H, Hkv, D, max_q_len);
+  EZ_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ez::aligned16(workspace)),
+             "linear_attn_prefill: needs a 16-byte aligned workspace of %zu bytes", need);
+  EZ_REQUIRE(a.segments * Hkv < (int64_t(1) << 31) && B * Hkv < (int64_t(1) << 27),
+             "linear_attn_prefill: too many sequences and heads for one launch");
+  a.ws = static_cast<float*>(workspace);
+  const dim3 grid(unsigned(a.segments * Hkv)), parts(unsigned(B * Hkv * (D * D / 1024)));
+  if (D == 64) {
+    if (need) {
+      hipLaunchKernelGGL((ez::linear_attn_chunk_kernel<64, false>), grid, dim3(128), 0, stream, a);
+      hipLaunchKernelGGL(ez::linear_attn_scan_kernel<64>, parts, dim3(256), 0, stream, a);
+    }
+    hipLaunchKernelGGL((ez::linear_attn_chunk_kernel<64, true>), grid, dim3(128), 0, stream, a);
+  } else {
+    if (need) {
+      hipLaunchKernelGGL((ez::linear_attn_chunk_kernel<128, false>), grid, dim3(256), 0, stream, a);
+      hipLaunchKernelGGL(ez::linear_attn_scan_kernel<128>, parts, dim3(256), 0, stream, a);
+    }
+    hipLaunchKernelGGL((ez::linear_attn_chunk_kernel<128, true>), grid, dim3(256), 0, stream, a);
+  }
   return ez::launch_status("linear_attn_prefill");
 }
 
