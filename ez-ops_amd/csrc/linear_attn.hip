@@ -32,7 +32,8 @@ struct LinAttnArgs {
   const int32_t *cu, *past;   // prefill: [B + 1], [B] or NULL
   uint16_t* out;              // [T, H, D]
   int64_t T, num_slots, max_q;
-  int64_t seg, segments;      // prefill: tokens per segment, segment numbers
+  int seg, seg_sh;            // prefill: tokens per segment (1 << seg_sh)
+  int segments;               // prefill: segment numbers
   float* ws;                  // prefill: [segments, Hkv, D, D] or NULL (one segment a sequence)
   int B, H, Hkv;
   float scale;
@@ -168,12 +169,16 @@ __device__ __forceinline__ void lds_tr_tiles(uint32_t a, i32x2_t (&r)[4]) {
       : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3])
       : "v"(a), "v"(a ^ 32), "v"(a ^ 64), "v"(a ^ 96), "i"(OFF), "i"(OFF + 8 * P));
 }
-// Four 1 KiB fragments in a row (16 bytes a lane).
-__device__ __forceinline__ void lds_frags4(uint32_t a, bf16x8_t (&r)[4]) {
+// Twelve 1 KiB fragments in a row (16 bytes a lane).
+__device__ __forceinline__ void lds_frags12(uint32_t a, bf16x8_t (&r)[12]) {
   asm volatile(
-      "ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:1024\n\tds_read_b128 %2, %4 offset:2048\n\t"
-      "ds_read_b128 %3, %4 offset:3072\n\ts_waitcnt lgkmcnt(0)"
-      : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3])
+      "ds_read_b128 %0, %12\n\tds_read_b128 %1, %12 offset:1024\n\tds_read_b128 %2, %12 offset:2048\n\t"
+      "ds_read_b128 %3, %12 offset:3072\n\tds_read_b128 %4, %12 offset:4096\n\tds_read_b128 %5, %12 offset:5120\n\t"
+      "ds_read_b128 %6, %12 offset:6144\n\tds_read_b128 %7, %12 offset:7168\n\tds_read_b128 %8, %12 offset:8192\n\t"
+      "ds_read_b128 %9, %12 offset:9216\n\tds_read_b128 %10, %12 offset:10240\n\t"
+      "ds_read_b128 %11, %12 offset:11264\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7]),
+        "=&v"(r[8]), "=&v"(r[9]), "=&v"(r[10]), "=&v"(r[11])
       : "v"(a));
 }
 __device__ __forceinline__ void lds_write_frags4(uint32_t a, const bf16x8_t (&r)[4]) {
@@ -221,53 +226,48 @@ struct Segment {
   int slot;            // state slot (-1: no pool)
   bool cont;           // the sequence starts from its stored state
   int64_t row;         // first row of the segment
-  int len, before;     // tokens, tokens of the segment before it
+  int len;             // tokens
 };
 
 // Finds segment number `id`; false if there is none (every thread agrees).  Contains barriers.
 template <int THREADS>
-__device__ __forceinline__ bool find_segment(const LinAttnArgs& a, int64_t id, Segment& g) {
-  __shared__ int64_t s_row[2];
-  __shared__ int s_slot, s_past;
+__device__ __forceinline__ bool find_segment(const LinAttnArgs& a, int id, Segment& g) {
+  __shared__ int s_row[2], s_slot, s_past;
+  const int T = int(a.T);
   int count = 0;  // sequences whose first segment number is at most id: the last of them is ours
   for (int c0 = 0; c0 < a.B; c0 += THREADS) {
     const int c = c0 + threadIdx.x;
     bool in = false;
-    if (c < a.B) {
-      const int64_t r = min(max(int64_t(a.cu[c]), int64_t(0)), a.T);
-      in = r / a.seg + c <= id;
-    }
+    if (c < a.B) in = (min(max(a.cu[c], 0), T) >> a.seg_sh) + c <= id;
     count += __syncthreads_count(in);
   }
   const int b = count - 1;
   if (b < 0) return false;
   if (threadIdx.x == 0) {
-    s_row[0] = min(max(int64_t(a.cu[b]), int64_t(0)), a.T);
-    s_row[1] = min(int64_t(a.cu[b + 1]), a.T);
+    s_row[0] = min(max(a.cu[b], 0), T);
+    s_row[1] = min(a.cu[b + 1], T);
     s_slot = a.state ? (a.state_slots ? a.state_slots[b] : b) : -1;
     s_past = a.past ? a.past[b] : 0;
   }
   __syncthreads();
-  const int64_t r0 = s_row[0], n = min(s_row[1] - r0, a.max_q);
-  int slot = s_slot;
+  const int r0 = s_row[0], n = min(s_row[1] - r0, int(a.max_q)), slot = s_slot;
   if (a.state) {
     int dup = slot < 0 || slot >= a.num_slots;
     if (a.state_slots)
       for (int c = threadIdx.x; c < b; c += THREADS) dup |= a.state_slots[c] == slot;
     if (__syncthreads_or(dup)) return false;
   }
-  const int64_t s = id - (r0 / a.seg + b);
-  if (n <= 0 || s < 0 || s * a.seg >= n) return false;
-  const int cnt = int((n + a.seg - 1) / a.seg);
-  const int first = int(n - int64_t(cnt - 1) * a.seg);  // 1 .. seg
+  const int s = id - ((r0 >> a.seg_sh) + b);
+  if (n <= 0 || s < 0 || s >= (n + a.seg - 1) >> a.seg_sh) return false;
+  const int cnt = (n + a.seg - 1) >> a.seg_sh;
+  const int first = n - ((cnt - 1) << a.seg_sh);  // 1 .. seg
   g.b = b;
-  g.s = int(s);
+  g.s = s;
   g.count = cnt;
   g.slot = slot;
   g.cont = a.state && s_past > 0;
-  g.row = r0 + (s ? first + (s - 1) * a.seg : 0);
-  g.len = s ? int(a.seg) : first;
-  g.before = s > 1 ? int(a.seg) : first;
+  g.row = r0 + (s ? first + ((s - 1) << a.seg_sh) : 0);
+  g.len = s ? a.seg : first;
   return true;
 }
 
@@ -278,9 +278,11 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
   EZ_PROF_WAVE(OUT ? kProfLinAttnPrefill : kProfLinAttnState);
   constexpr int THREADS = 2 * D, NT = D / 32, NK = D / 16, P = 2 * D;  // P: bytes of an LDS row
   constexpr int TILE = kC * P, LPT = TILE / 16 / THREADS;
-  __shared__ __align__(16) uint16_t Ks[2][kC * D], Vs[2][kC * D];
+  // K in two buffers (read up to the end of its chunk), V and Q in one each: they are in
+  // registers before the next ones are asked for.  76 KiB at D = 128: two blocks a CU.
+  __shared__ __align__(16) uint16_t Ks[2][kC * D], Vs[OUT ? 1 : 2][kC * D], Qs[OUT ? kC * D : 8];
   __shared__ __align__(16) uint16_t Ps[OUT ? 3 * 4 * 512 : 8];  // block of P x (16-key step, part) x lane x 8
-  const int64_t id = blockIdx.x / a.Hkv;
+  const int id = blockIdx.x / a.Hkv;
   const int kvh = blockIdx.x % a.Hkv;
   Segment sg;
   if (!find_segment<THREADS>(a, id, sg)) return;
@@ -298,7 +300,7 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
     for (int r = 0; r < 16; ++r) S[t][r] = 0.f;
   const int64_t elem = int64_t(8 * h) * D + 32 * w + j;
   float* pool = sg.slot >= 0 ? a.state + (int64_t(sg.slot) * a.Hkv + kvh) * D * D + elem : nullptr;
-  float* ws = a.ws + (id * a.Hkv + kvh) * D * D + elem;
+  float* ws = a.ws + (int64_t(id) * a.Hkv + kvh) * D * D + elem;
   if (OUT && (sg.s > 0 || sg.cont)) {
     const float* src = sg.count > 1 ? ws : pool;
 #pragma unroll
@@ -327,23 +329,22 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
   constexpr int RPL = THREADS / (D / 8);  // rows per load of the block: 16, which the swizzle does not see
   static_assert(RPL == 16 && LPT * RPL == kC, "staging covers the chunk");
   const int srow = tid / (D / 8), sch = (tid % (D / 8)) ^ swizzle<D>(srow);
-  const uint32_t krow = uint32_t(srow) * uint32_t(2 * a.k_rs) + 16 * sch;
-  const uint32_t vrow = uint32_t(srow) * uint32_t(2 * a.v_rs) + 16 * sch;
-  auto load_chunk = [&](int c) {
+  // head `hd` of chunk c's rows of x into LDS at `to`
+  auto load_tile = [&](const uint16_t* x, int64_t rs, int hd, int c, uint16_t* to) {
     const int r0 = c * kC - pad;  // first row of the chunk in the segment; negative in a short first chunk
-    const int rb = max(r0, 0), back = rb - r0, rows = kC - back;
-    const uint16_t* kp = a.k + (sg.row + rb) * a.k_rs + kvh * D;
-    const uint16_t* vp = a.v + (sg.row + rb) * a.v_rs + kvh * D;
-    const auto kres = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(kp), 0, int(rows * 2 * a.k_rs), 0x00020000);
-    const auto vres = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(vp), 0, int(rows * 2 * a.v_rs), 0x00020000);
+    const int rb = max(r0, 0), back = rb - r0;
+    const auto res = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(x + (sg.row + rb) * rs + hd * D), 0,
+                                                       int((kC - back) * 2 * rs), 0x00020000);
+    const uint32_t pitch = uint32_t(2 * rs), off = uint32_t(srow) * pitch + 16 * sch;
 #pragma unroll
-    for (int i = 0; i < LPT; ++i) {
-      const int at = (i * THREADS + w * kWave) * 8;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(kres, (__attribute__((address_space(3))) void*)(&Ks[c & 1][at]), 16,
-                                               krow + uint32_t(i * RPL - back) * uint32_t(2 * a.k_rs), 0, 0, 0);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(vres, (__attribute__((address_space(3))) void*)(&Vs[c & 1][at]), 16,
-                                               vrow + uint32_t(i * RPL - back) * uint32_t(2 * a.v_rs), 0, 0, 0);
-    }
+    for (int i = 0; i < LPT; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          res, (__attribute__((address_space(3))) void*)(to + (i * THREADS + w * kWave) * 8), 16,
+          off + uint32_t(i * RPL - back) * pitch, 0, 0, 0);
+  };
+  auto load_kv = [&](int c) {
+    load_tile(a.k, a.k_rs, kvh, c, Ks[c & 1]);
+    load_tile(a.v, a.v_rs, kvh, c, Vs[OUT ? 0 : c & 1]);
   };
 
   // LDS read addresses in buffer 0
@@ -358,17 +359,10 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
   const uint32_t pfr = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint16_t*)(&Ps[0]))) +
                        uint32_t(lane * 16);
 
+  const uint32_t qrd = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint16_t*)(&Qs[0]))) +
+                       uint32_t(j * P + ((h ^ swizzle<D>(j)) << 4));
+
   const int G = a.H / a.Hkv;
-  bf16x8_t q[2][NK];  // queries of the chunk's two halves, the next head's as soon as these are used
-  auto load_q = [&](int c, int hg) {
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const uint16_t* qp =
-          a.q + (sg.row + max(c * kC - pad + 32 * t + j, 0)) * a.q_rs + (kvh * G + hg) * D + 8 * h;
-#pragma unroll
-      for (int s = 0; s < NK; ++s) q[t][s] = as_bf16x8(*reinterpret_cast<const uint4*>(qp + 16 * s));
-    }
-  };
   // one 32 x 32 block of P (keys of half KT) into LDS slot `blk`
   auto make_p = [&](auto ktc, const bf16x8_t(&qt)[NK], uint32_t buf, int blk) {
     constexpr int KT = decltype(ktc)::value;
@@ -393,19 +387,23 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
     }
     lds_write_frags4(pfr + 4096 * blk, pf);
   };
-  if constexpr (OUT) load_q(0, 0);
-  load_chunk(0);
+  load_kv(0);
+  if constexpr (OUT) load_tile(a.q, a.q_rs, kvh * G, 0, Qs);
   wait_vm<0>();
   __syncthreads();
   for (int c = 0; c < chunks; ++c) {
     const uint32_t buf = uint32_t(c & 1) * TILE;
     const int r0 = c * kC - pad;
-    if (c + 1 < chunks) load_chunk(c + 1);
+    const bool more = c + 1 < chunks;
+    if (!OUT && more) load_kv(c + 1);
     i32x2_t vf[8];
-    lds_tr_steps<P>(lds_at(vtr, buf), vf);
+    lds_tr_steps<P>(lds_at(vtr, OUT ? 0 : buf), vf);
     if constexpr (OUT) {
       for (int hg = 0; hg < G; ++hg) {
         const int hq = kvh * G + hg;
+        bf16x8_t q[2][NK];
+        lds_row<0>(lds_at(qrd, 0), q[0]);
+        lds_row<32 * P>(lds_at(qrd, 0), q[1]);
         if (w == 0) make_p(std::integral_constant<int, 0>{}, q[0], buf, 0);
         if (w == 1) make_p(std::integral_constant<int, 0>{}, q[1], buf, 1);
         if (w == (D == 64 ? 0 : 2)) make_p(std::integral_constant<int, 1>{}, q[1], buf, 2);
@@ -423,15 +421,19 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] = S[s >> 1][8 * (s & 1) + e];
           const bf16x8_t hi = take_part(x), lo = last_part(x);
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi, q[t][s], o[t], 0, 0, 0);
-            o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lo, q[t][s], o[t], 0, 0, 0);
-          }
-          __builtin_amdgcn_sched_barrier(0);
+          o[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi, q[0][s], o[0], 0, 0, 0);
+          o[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi, q[1][s], o[1], 0, 0, 0);
+          o[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lo, q[0][s], o[0], 0, 0, 0);
+          o[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lo, q[1][s], o[1], 0, 0, 0);
         }
-        if (hg + 1 < G) load_q(c, hg + 1);
-        else if (c + 1 < chunks) load_q(c + 1, 0);
+        // the parts of the next step between the products of this one
+        __builtin_amdgcn_sched_group_barrier(0x2, 24, 0);
+#pragma unroll
+        for (int i = 0; i < 4 * NK; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x2, 6, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const float f = a.scale * power(g2, max(r0 + 32 * t + j - max(r0, 0) + 1, 0));
@@ -439,31 +441,42 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
           for (int r = 0; r < 16; ++r) o[t][r] *= f;
         }
         __builtin_amdgcn_sched_barrier(0);
-        __syncthreads();  // P is there
-        // what the chunk's own tokens give
+        __syncthreads();  // P is there; V and Q have been read
+        if (hg + 1 < G) load_tile(a.q, a.q_rs, hq + 1, c, Qs);
+        else if (more) load_tile(a.q, a.q_rs, kvh * G, c + 1, Qs);
+        if (hg == 0 && more) load_kv(c + 1);
+        // what the chunk's own tokens give: block 0 to the first queries, blocks 1 and 2 to the second
+        bf16x8_t pf[12];
+        lds_frags12(pfr, pf);
 #pragma unroll
-        for (int blk = 0; blk < 3; ++blk) {
-          bf16x8_t pf[4];
-          lds_frags4(pfr + 4096 * blk, pf);
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int t = blk > 0, step = 2 * (blk == 2) + u;
-            const bf16x8_t va = join(vf[2 * step], vf[2 * step + 1]);
-            o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, pf[2 * u], o[t], 0, 0, 0);
-            o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, pf[2 * u + 1], o[t], 0, 0, 0);
-          }
+        for (int i = 0; i < 4; ++i) {
+          const bf16x8_t v0 = join(vf[2 * (i >> 1)], vf[2 * (i >> 1) + 1]), v1 = join(vf[4 + 2 * (i >> 1)], vf[5 + 2 * (i >> 1)]);
+          o[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v0, pf[4 + i], o[1], 0, 0, 0);
+          o[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v0, pf[i], o[0], 0, 0, 0);
+          o[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v1, pf[8 + i], o[1], 0, 0, 0);
         }
-        if (hg + 1 < G) __syncthreads();  // P has been read
+        // o[t][4e + x] = O^T[column 8e + 4h + x][query j]: the lane halves swap groups, so that each stores
+        // 16 bytes: columns 16p + 8h..+7
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const int row = r0 + 32 * t + j;
-          if (row >= 0) {
-            uint16_t* op = a.out + ((sg.row + row) * a.H + hq) * D + 32 * w + 4 * h;
+          uint16_t* op = a.out + ((sg.row + max(row, 0)) * a.H + hq) * D + 32 * w + 8 * h;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              *reinterpret_cast<uint2*>(op + 8 * e) = make_uint2(cvt_bf2(o[t][4 * e], o[t][4 * e + 1]),
-                                                                 cvt_bf2(o[t][4 * e + 2], o[t][4 * e + 3]));
+          for (int p = 0; p < 2; ++p) {
+            const auto x = __builtin_amdgcn_permlane32_swap(cvt_bf2(o[t][8 * p], o[t][8 * p + 1]),
+                                                            cvt_bf2(o[t][8 * p + 4], o[t][8 * p + 5]), false, false);
+            const auto y = __builtin_amdgcn_permlane32_swap(cvt_bf2(o[t][8 * p + 2], o[t][8 * p + 3]),
+                                                            cvt_bf2(o[t][8 * p + 6], o[t][8 * p + 7]), false, false);
+            if (row >= 0) *reinterpret_cast<uint4*>(op + 16 * p) = make_uint4(x[0], y[0], x[1], y[1]);
           }
+        }
+        if (hg + 1 < G) {
+          // the next head's Q has landed: in front of it in the counter are this head's four stores (all
+          // there unless the chunk is short) and, once a chunk, the next K and V
+          if (r0 < 0) wait_vm<0>();
+          else if (hg == 0 && more) wait_vm<4 + 2 * LPT>();
+          else wait_vm<4>();
+          __syncthreads();  // ... and P has been read
         }
       }
     }
@@ -490,13 +503,12 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
       const bf16x8_t hi = take_part(x), mid = take_part(x), lo = last_part(x);
       i32x2_t kf[2 * NT];
       lds_tr_tiles<16 * s * P, P>(lds_at(ktr, buf), kf);
+      const bf16x8_t parts[3] = {lo, mid, hi};
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const bf16x8_t ka = join(kf[2 * t], kf[2 * t + 1]);
-        S[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka, lo, S[t], 0, 0, 0);
-        S[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka, mid, S[t], 0, 0, 0);
-        S[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka, hi, S[t], 0, 0, 0);
-      }
+      for (int i = 0; i < 3; ++i)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+          S[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(join(kf[2 * t], kf[2 * t + 1]), parts[i], S[t], 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
     };
     add_step(std::integral_constant<int, 0>{});
@@ -518,50 +530,60 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
 // The workspace's slot of segment s > 0 holds the sum of segment s - 1; becomes the state
 // before segment s.  Slot 0 gets the stored state where the sequence continues (the output
 // kernel's last segment overwrites the pool while its first may still have to start).
-// Block = (sequence, kv head, 1024 elements).
+// Block = (sequence, kv head, 256 elements), one element a thread: the chain over the segments is
+// short of work per step, so the chip is filled with threads, each eight loads ahead of its sums.
 template <int D>
 __global__ __launch_bounds__(256) void linear_attn_scan_kernel(LinAttnArgs a) {
   EZ_PROF_WAVE(kProfLinAttnState);
-  constexpr int PARTS = D * D / 1024;
+  constexpr int PARTS = D * D / 256, AHEAD = 8;
   const int part = blockIdx.x % PARTS, kvh = blockIdx.x / PARTS % a.Hkv, b = blockIdx.x / PARTS / a.Hkv;
-  const int64_t r0 = min(max(int64_t(a.cu[b]), int64_t(0)), a.T);
-  const int64_t n = min(min(int64_t(a.cu[b + 1]), a.T) - r0, a.max_q);
+  const int T = int(a.T), r0 = min(max(a.cu[b], 0), T), n = min(min(a.cu[b + 1], T) - r0, int(a.max_q));
   if (n <= a.seg) return;
   int slot = -1;
   if (a.state) {
     slot = slot_of<256>(a, b);
     if (slot < 0) return;
   }
-  const int64_t cnt = (n + a.seg - 1) / a.seg, id = r0 / a.seg + b;
-  const int64_t last = min(cnt, a.segments - id);  // a table of decreasing offsets must not lead past the workspace
-  const int64_t at = int64_t(part) * 1024 + 4 * threadIdx.x, step = int64_t(a.Hkv) * D * D;
-  float* ws = a.ws + (id * a.Hkv + kvh) * D * D + at;
-  float4 S = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int cnt = (n + a.seg - 1) >> a.seg_sh, id = (r0 >> a.seg_sh) + b;
+  const int last = min(cnt, a.segments - id);  // decreasing offsets must not lead past the workspace
+  if (last < 2) return;
+  const int at = part * 256 + int(threadIdx.x);
+  const int64_t step = int64_t(a.Hkv) * D * D;
+  float* ws = a.ws + (int64_t(id) * a.Hkv + kvh) * D * D + at;
+  auto load = [&](float(&x)[AHEAD], int s0) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) x[i] = ws[min(s0 + i, last - 1) * step];
+  };
+  float x[AHEAD], next[AHEAD];
+  load(x, 1);
+  float S = 0.f;
   if (slot >= 0 && a.past && a.past[b] > 0) {
-    S = *reinterpret_cast<const float4*>(a.state + (int64_t(slot) * a.Hkv + kvh) * D * D + at);
-    *reinterpret_cast<float4*>(ws) = S;
+    S = a.state[(int64_t(slot) * a.Hkv + kvh) * D * D + at];
+    ws[0] = S;
   }
   const float g = a.log_decay[kvh];
-  const Keep first = keep_over(g, float(n - (cnt - 1) * a.seg)), rest = keep_over(g, float(a.seg));
-  for (int64_t s = 1; s < last; ++s) {
-    float4* p = reinterpret_cast<float4*>(ws + s * step);
-    const Keep f = s == 1 ? first : rest;
-    const float4 x = *p;
-    S.x = decayed(f, S.x, x.x);
-    S.y = decayed(f, S.y, x.y);
-    S.z = decayed(f, S.z, x.z);
-    S.w = decayed(f, S.w, x.w);
-    *p = S;
+  const Keep first = keep_over(g, float(n - ((cnt - 1) << a.seg_sh))), rest = keep_over(g, float(a.seg));
+  for (int s0 = 1; s0 < last; s0 += AHEAD) {
+    load(next, s0 + AHEAD);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      if (s0 + i < last) {
+        S = decayed(s0 + i == 1 ? first : rest, S, x[i]);
+        ws[(s0 + i) * step] = S;
+      }
+      x[i] = next[i];
+    }
   }
 }
 
-// Tokens per segment: as long as that still gives about 512 blocks (two a CU) over the
-// whole batch, at least a chunk.
-int64_t segment_tokens(int64_t T, int64_t Hkv) {
-  const int64_t want = (T * Hkv + 511) / 512;
-  return (want + kC - 1) / kC * kC;
+// log2 of the tokens per segment: the longest segments that still give about 512 blocks over the whole
+// batch, at least a chunk.
+int segment_shift(int64_t T, int64_t Hkv) {
+  int sh = 6;
+  while ((T * Hkv) >> (sh + 1) >= 512) ++sh;
+  return sh;
 }
-int64_t segment_count(int64_t B, int64_t T, int64_t seg) { return T / seg + B; }
+int64_t segment_count(int64_t B, int64_t T, int sh) { return (T >> sh) + B; }
 
 // One token per sequence: block = (sequence, kv head, slice of VC columns of the
 // state), the slice in registers between its one read and its one write.
@@ -640,9 +662,9 @@ int check_common(const LinAttnArgs& a, int64_t H, int64_t Hkv, int64_t D, const 
 extern "C" size_t ezops_linear_attn_prefill_workspace_size(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t D,
                                                            int64_t max_q_len) {
   if (B < 1 || T < 1 || Hkv < 1 || D < 1) return 0;
-  const int64_t seg = ez::segment_tokens(T, Hkv);
-  if ((max_q_len > 0 && max_q_len < T ? max_q_len : T) <= seg) return 0;
-  return size_t(ez::segment_count(B, T, seg)) * Hkv * D * D * sizeof(float);
+  const int sh = ez::segment_shift(T, Hkv);
+  if ((max_q_len > 0 && max_q_len < T ? max_q_len : T) <= int64_t(1) << sh) return 0;
+  return size_t(ez::segment_count(B, T, sh)) * Hkv * D * D * sizeof(float);
 }
 
 extern "C" int ezops_linear_attn_prefill_bf16(const void* q, int64_t q_stride, const void* k, int64_t k_stride,
@@ -673,15 +695,17 @@ extern "C" int ezops_linear_attn_prefill_bf16(const void* q, int64_t q_stride, c
   a.scale = scale > 0.f ? scale : 1.f / sqrtf(float(D));
   EZ_REQUIRE(q_stride < (1 << 23) && k_stride < (1 << 23) && v_stride < (1 << 23),
              "linear_attn_prefill: token strides must be below 2^23");
-  a.seg = ez::segment_tokens(T, Hkv);
-  a.segments = ez::segment_count(B, T, a.seg);
+  a.seg_sh = ez::segment_shift(T, Hkv);
+  a.seg = 1 << a.seg_sh;
+  const int64_t segments = ez::segment_count(B, T, a.seg_sh);
   const size_t need = ezops_linear_attn_prefill_workspace_size(B, T, H, Hkv, D, max_q_len);
   EZ_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ez::aligned16(workspace)),
              "linear_attn_prefill: needs a 16-byte aligned workspace of %zu bytes", need);
-  EZ_REQUIRE(a.segments * Hkv < (int64_t(1) << 31) && B * Hkv < (int64_t(1) << 27),
+  EZ_REQUIRE(segments * Hkv < (int64_t(1) << 31) && B * Hkv < (int64_t(1) << 25),
              "linear_attn_prefill: too many sequences and heads for one launch");
+  a.segments = int(segments);
   a.ws = static_cast<float*>(workspace);
-  const dim3 grid(unsigned(a.segments * Hkv)), parts(unsigned(B * Hkv * (D * D / 1024)));
+  const dim3 grid(unsigned(segments * Hkv)), parts(unsigned(B * Hkv * (D * D / 256)));
   if (D == 64) {
     if (need) {
       hipLaunchKernelGGL((ez::linear_attn_chunk_kernel<64, false>), grid, dim3(128), 0, stream, a);
