@@ -51,6 +51,10 @@ __device__ __forceinline__ Keep keep_over(float log_decay, float n) {
   const float m = expm1f(log_decay * n);
   return m > -0.5f ? Keep{m, true} : Keep{expf(log_decay * n), false};
 }
+__device__ __forceinline__ Keep uniform(const Keep& k) {  // into scalar registers
+  return Keep{__int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(k.m))),
+              bool(__builtin_amdgcn_readfirstlane(int(k.near)))};
+}
 // lambda^n S + x
 __device__ __forceinline__ float decayed(const Keep& k, float S, float x) {
   const float y = fmaf(k.m, S, x);
@@ -169,6 +173,10 @@ __device__ __forceinline__ void lds_tr_tiles(uint32_t a, i32x2_t (&r)[4]) {
       : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3])
       : "v"(a), "v"(a ^ 32), "v"(a ^ 64), "v"(a ^ 96), "i"(OFF), "i"(OFF + 8 * P));
 }
+// A barrier without a wait: __syncthreads() waits for outstanding LDS DMA as well, which here is the next
+// chunk's.  LDS reads and writes in front of it have ended with waits of their own.
+__device__ __forceinline__ void block_barrier() { asm volatile("s_barrier" ::: "memory"); }
+
 // Twelve 1 KiB fragments in a row (16 bytes a lane).
 __device__ __forceinline__ void lds_frags12(uint32_t a, bf16x8_t (&r)[12]) {
   asm volatile(
@@ -187,6 +195,30 @@ __device__ __forceinline__ void lds_write_frags4(uint32_t a, const bf16x8_t (&r)
       "ds_write_b128 %0, %4 offset:3072\n\ts_waitcnt lgkmcnt(0)"
       :
       : "v"(a), "v"(r[0]), "v"(r[1]), "v"(r[2]), "v"(r[3])
+      : "memory");
+}
+// Register r: 8 (r / 4) + r % 4 floats below the address + 108.
+__device__ __forceinline__ void lds_weights(uint32_t a, float (&r)[16]) {
+  asm volatile(
+      "ds_read_b32 %0, %16 offset:108\n\tds_read_b32 %1, %16 offset:104\n\tds_read_b32 %2, %16 offset:100\n\t"
+      "ds_read_b32 %3, %16 offset:96\n\tds_read_b32 %4, %16 offset:76\n\tds_read_b32 %5, %16 offset:72\n\t"
+      "ds_read_b32 %6, %16 offset:68\n\tds_read_b32 %7, %16 offset:64\n\tds_read_b32 %8, %16 offset:44\n\t"
+      "ds_read_b32 %9, %16 offset:40\n\tds_read_b32 %10, %16 offset:36\n\tds_read_b32 %11, %16 offset:32\n\t"
+      "ds_read_b32 %12, %16 offset:12\n\tds_read_b32 %13, %16 offset:8\n\tds_read_b32 %14, %16 offset:4\n\t"
+      "ds_read_b32 %15, %16\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7]),
+        "=&v"(r[8]), "=&v"(r[9]), "=&v"(r[10]), "=&v"(r[11]), "=&v"(r[12]), "=&v"(r[13]), "=&v"(r[14]), "=&v"(r[15])
+      : "v"(a));
+}
+// A wave's own 32 rows of 64 bytes, written 16 bytes a lane at `wr` and `wr ^ 32` and read back at
+// `rd` and 1 KiB further on.
+__device__ __forceinline__ void lds_turn(uint32_t wr, uint32_t rd, const uint4& x, const uint4& y, u32x4_t (&r)[2]) {
+  const u32x4_t a = {x.x, x.y, x.z, x.w}, b = {y.x, y.y, y.z, y.w};
+  asm volatile(
+      "ds_write_b128 %2, %4\n\tds_write_b128 %3, %5\n\ts_waitcnt lgkmcnt(0)\n\t"
+      "ds_read_b128 %0, %6\n\tds_read_b128 %1, %6 offset:1024\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(r[0]), "=&v"(r[1])
+      : "v"(wr), "v"(wr ^ 32), "v"(a), "v"(b), "v"(rd)
       : "memory");
 }
 __device__ __forceinline__ bf16x8_t join(const i32x2_t& x, const i32x2_t& y) {
@@ -225,7 +257,7 @@ struct Segment {
   int b, s, count;     // sequence, index in it, its number of segments
   int slot;            // state slot (-1: no pool)
   bool cont;           // the sequence starts from its stored state
-  int64_t row;         // first row of the segment
+  int row;             // first row of the segment
   int len;             // tokens
 };
 
@@ -241,7 +273,7 @@ __device__ __forceinline__ bool find_segment(const LinAttnArgs& a, int id, Segme
     if (c < a.B) in = (min(max(a.cu[c], 0), T) >> a.seg_sh) + c <= id;
     count += __syncthreads_count(in);
   }
-  const int b = count - 1;
+  const int b = __builtin_amdgcn_readfirstlane(count) - 1;
   if (b < 0) return false;
   if (threadIdx.x == 0) {
     s_row[0] = min(max(a.cu[b], 0), T);
@@ -250,7 +282,10 @@ __device__ __forceinline__ bool find_segment(const LinAttnArgs& a, int id, Segme
     s_past = a.past ? a.past[b] : 0;
   }
   __syncthreads();
-  const int r0 = s_row[0], n = min(s_row[1] - r0, int(a.max_q)), slot = s_slot;
+  // out of LDS into scalar registers: every thread has the same
+  const int r0 = __builtin_amdgcn_readfirstlane(s_row[0]);
+  const int n = min(__builtin_amdgcn_readfirstlane(s_row[1]) - r0, int(a.max_q));
+  const int slot = __builtin_amdgcn_readfirstlane(s_slot);
   if (a.state) {
     int dup = slot < 0 || slot >= a.num_slots;
     if (a.state_slots)
@@ -265,7 +300,7 @@ __device__ __forceinline__ bool find_segment(const LinAttnArgs& a, int id, Segme
   g.s = s;
   g.count = cnt;
   g.slot = slot;
-  g.cont = a.state && s_past > 0;
+  g.cont = a.state && __builtin_amdgcn_readfirstlane(s_past) > 0;
   g.row = r0 + (s ? first + ((s - 1) << a.seg_sh) : 0);
   g.len = s ? a.seg : first;
   return true;
@@ -280,8 +315,9 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
   constexpr int TILE = kC * P, LPT = TILE / 16 / THREADS;
   // K in two buffers (read up to the end of its chunk), V and Q in one each: they are in
   // registers before the next ones are asked for.  76 KiB at D = 128: two blocks a CU.
-  __shared__ __align__(16) uint16_t Ks[2][kC * D], Vs[OUT ? 1 : 2][kC * D], Qs[OUT ? kC * D : 8];
-  __shared__ __align__(16) uint16_t Ps[OUT ? 3 * 4 * 512 : 8];  // block of P x (16-key step, part) x lane x 8
+  __shared__ __align__(1024) uint16_t Ks[2][kC * D], Vs[OUT ? 1 : 2][kC * D], Qs[OUT ? kC * D : 8];
+  __shared__ __align__(1024) uint16_t Ps[OUT ? 3 * 4 * 512 : 8];  // block of P x (16-key step, part) x lane x 8
+  __shared__ float pw[96];
   const int id = blockIdx.x / a.Hkv;
   const int kvh = blockIdx.x % a.Hkv;
   Segment sg;
@@ -290,7 +326,8 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
   const int tid = threadIdx.x, lane = tid & (kWave - 1), w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = lane >> 5, j = lane & 31;
   const int chunks = (sg.len + kC - 1) / kC, pad = chunks * kC - sg.len;
-  const float g = a.log_decay[kvh], g2 = g * 1.4426950408889634f;
+  const float g = a.log_decay[kvh];
+  const float g2 = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(g * 1.4426950408889634f)));
 
   // state of this wave's columns: register r of tile t = S[32t + 16(r/8) + 8h + r%8][32w + j]
   f32x16_t S[NT];
@@ -298,29 +335,21 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int r = 0; r < 16; ++r) S[t][r] = 0.f;
-  const int64_t elem = int64_t(8 * h) * D + 32 * w + j;
-  float* pool = sg.slot >= 0 ? a.state + (int64_t(sg.slot) * a.Hkv + kvh) * D * D + elem : nullptr;
-  float* ws = a.ws + (int64_t(id) * a.Hkv + kvh) * D * D + elem;
+  const int elem = 8 * h * D + 32 * w + j;
+  float* pool = sg.slot >= 0 ? a.state + (int64_t(sg.slot) * a.Hkv + kvh) * D * D : nullptr;
+  float* ws = a.ws + (int64_t(id) * a.Hkv + kvh) * D * D;
   if (OUT && (sg.s > 0 || sg.cont)) {
     const float* src = sg.count > 1 ? ws : pool;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) S[t][r] = src[(32 * t + 16 * (r >> 3) + (r & 7)) * D];
+      for (int r = 0; r < 16; ++r) S[t][r] = src[elem + (32 * t + 16 * (r >> 3) + (r & 7)) * D];
   }
 
-  // powers: wv[e] = lambda^(15 - token) of the tokens of a 16-token step; pm = scale * lambda^(query - key)
-  // of this wave's block of P: on the diagonal (blocks 0 and 2) or below it (block 1)
-  const bool diag = D == 64 ? w == 0 : w != 1;
-  float wv[8], pm[16];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) wv[e] = power(g2, 15 - (8 * (e >> 2) + 4 * h + (e & 3)));
+  // weights of P: pw[31 + n] = scale * lambda^n, 0 for n < 0 (keys behind the query); n = query - key in the
+  // blocks on the diagonal, 32 more in the one below it
   if constexpr (OUT) {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int ago = (diag ? 0 : 32) + j - (8 * (r >> 2) + 4 * h + (r & 3));
-      pm[r] = ago >= 0 ? a.scale * power(g2, max(ago, 0)) : 0.f;
-    }
+    if (tid < 96) pw[tid] = tid < 31 ? 0.f : a.scale * power(g2, tid - 31);
   }
 
   // staging: LDS chunk p = THREADS c + tid holds 16-byte chunk (p % (D/8)) ^ swizzle of row
@@ -362,17 +391,35 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
   const uint32_t qrd = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint16_t*)(&Qs[0]))) +
                        uint32_t(j * P + ((h ^ swizzle<D>(j)) << 4));
 
+  // register r wants n = j - 8 (r / 4) - 4 h - r % 4
+  const uint32_t pwrd = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const float*)(&pw[0]))) +
+                        uint32_t(4 * (31 + j - 4 * h - 27));
+  // the outputs on their way: row j of the wave's 2 KiB, 16-byte chunk c at c ^ (row / 4 % 4)
+  const uint32_t obase = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint16_t*)(&Ps[0]))) +
+                         uint32_t(w * 2048);
+  const uint32_t owr = obase + uint32_t(j * 64 + ((h ^ ((j >> 2) & 3)) << 4));
+  const uint32_t ord = obase + uint32_t((lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 4) & 3)) << 4));
+
   const int G = a.H / a.Hkv;
-  // one 32 x 32 block of P (keys of half KT) into LDS slot `blk`
-  auto make_p = [&](auto ktc, const bf16x8_t(&qt)[NK], uint32_t buf, int blk) {
-    constexpr int KT = decltype(ktc)::value;
-    bf16x8_t kf[NK], pf[4];
-    lds_row<KT * 32 * P>(lds_at(krd, buf), kf);
+  float* dst = OUT ? (sg.s == sg.count - 1 ? pool : nullptr) : id + 1 < a.segments ? ws + int64_t(a.Hkv) * D * D : nullptr;
+  const Keep keep_first = uniform(keep_over(g, float(kC - pad))), keep_full = uniform(keep_over(g, float(kC)));
+  // One 32 x 32 block of P (0: first keys and queries, 1: first keys, second queries, 2: second keys and
+  // queries), weighted, in two parts: the operand of the product with V, four fragments.
+  auto make_p = [&](int blk, uint32_t buf) {
     f32x16_t st;
 #pragma unroll
     for (int r = 0; r < 16; ++r) st[r] = 0.f;
+    {
+      bf16x8_t kf[NK], qf[NK];
+      lds_row<0>(lds_at(krd, buf + (blk >> 1) * 32 * P), kf);
+      lds_row<0>(lds_at(qrd, (blk > 0) * 32 * P), qf);
 #pragma unroll
-    for (int s = 0; s < NK; ++s) st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[s], qt[s], st, 0, 0, 0);
+      for (int s = 0; s < NK; ++s) st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[s], qf[s], st, 0, 0, 0);
+    }
+    const bool diag = blk != 1;
+    float pm[16];
+    lds_weights(lds_at(pwrd, diag ? 0 : 128), pm);
+    bf16x8_t pf[4];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       float x[8];
@@ -401,12 +448,14 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
     if constexpr (OUT) {
       for (int hg = 0; hg < G; ++hg) {
         const int hq = kvh * G + hg;
+        // blocks of P: wave w makes block w (0: first keys and queries, 1: first keys, second queries,
+        // 2: second keys and queries); of two waves the first makes block 2 too
+        if (w < 3) make_p(w, buf);
+        if (D == 64 && w == 0) make_p(2, buf);
+        __builtin_amdgcn_sched_barrier(0);
         bf16x8_t q[2][NK];
         lds_row<0>(lds_at(qrd, 0), q[0]);
         lds_row<32 * P>(lds_at(qrd, 0), q[1]);
-        if (w == 0) make_p(std::integral_constant<int, 0>{}, q[0], buf, 0);
-        if (w == 1) make_p(std::integral_constant<int, 0>{}, q[1], buf, 1);
-        if (w == (D == 64 ? 0 : 2)) make_p(std::integral_constant<int, 1>{}, q[1], buf, 2);
         __builtin_amdgcn_sched_barrier(0);
         // what the state gives, scaled by lambda^(i+1) of the query.  The parts of S are made anew for
         // every head (S is opaque here): kept, they would take the registers of S a second time.
@@ -441,33 +490,41 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
           for (int r = 0; r < 16; ++r) o[t][r] *= f;
         }
         __builtin_amdgcn_sched_barrier(0);
-        __syncthreads();  // P is there; V and Q have been read
+        block_barrier();  // P is there; V and Q have been read
         if (hg + 1 < G) load_tile(a.q, a.q_rs, hq + 1, c, Qs);
         else if (more) load_tile(a.q, a.q_rs, kvh * G, c + 1, Qs);
         if (hg == 0 && more) load_kv(c + 1);
         // what the chunk's own tokens give: block 0 to the first queries, blocks 1 and 2 to the second
-        bf16x8_t pf[12];
-        lds_frags12(pfr, pf);
+        bf16x8_t pa[12];
+        lds_frags12(pfr, pa);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const bf16x8_t v0 = join(vf[2 * (i >> 1)], vf[2 * (i >> 1) + 1]), v1 = join(vf[4 + 2 * (i >> 1)], vf[5 + 2 * (i >> 1)]);
-          o[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v0, pf[4 + i], o[1], 0, 0, 0);
-          o[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v0, pf[i], o[0], 0, 0, 0);
-          o[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v1, pf[8 + i], o[1], 0, 0, 0);
+          o[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v0, pa[4 + i], o[1], 0, 0, 0);
+          o[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v0, pa[i], o[0], 0, 0, 0);
+          o[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v1, pa[8 + i], o[1], 0, 0, 0);
         }
-        // o[t][4e + x] = O^T[column 8e + 4h + x][query j]: the lane halves swap groups, so that each stores
-        // 16 bytes: columns 16p + 8h..+7
+        block_barrier();  // P has been read: its place serves the outputs
+        // o[t][4e + x] = O^T[column 8e + 4h + x][query j]: the lane halves swap groups, so that each holds
+        // 16 bytes of a row, columns 16p + 8h..+7; through LDS to four lanes a row (stores of 64 lanes on
+        // 64 lines cost the address unit four times as much)
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const int row = r0 + 32 * t + j;
-          uint16_t* op = a.out + ((sg.row + max(row, 0)) * a.H + hq) * D + 32 * w + 8 * h;
+          uint4 x[2];
 #pragma unroll
           for (int p = 0; p < 2; ++p) {
-            const auto x = __builtin_amdgcn_permlane32_swap(cvt_bf2(o[t][8 * p], o[t][8 * p + 1]),
+            const auto u = __builtin_amdgcn_permlane32_swap(cvt_bf2(o[t][8 * p], o[t][8 * p + 1]),
                                                             cvt_bf2(o[t][8 * p + 4], o[t][8 * p + 5]), false, false);
-            const auto y = __builtin_amdgcn_permlane32_swap(cvt_bf2(o[t][8 * p + 2], o[t][8 * p + 3]),
+            const auto v = __builtin_amdgcn_permlane32_swap(cvt_bf2(o[t][8 * p + 2], o[t][8 * p + 3]),
                                                             cvt_bf2(o[t][8 * p + 6], o[t][8 * p + 7]), false, false);
-            if (row >= 0) *reinterpret_cast<uint4*>(op + 16 * p) = make_uint4(x[0], y[0], x[1], y[1]);
+            x[p] = make_uint4(u[0], v[0], u[1], v[1]);
+          }
+          u32x4_t y[2];
+          lds_turn(owr, ord, x[0], x[1], y);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int row = r0 + 32 * t + 16 * i + (lane >> 2);
+            if (row >= 0) *reinterpret_cast<u32x4_t*>(a.out + ((sg.row + row) * a.H + hq) * D + 32 * w + 8 * (lane & 3)) = y[i];
           }
         }
         if (hg + 1 < G) {
@@ -476,11 +533,12 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
           if (r0 < 0) wait_vm<0>();
           else if (hg == 0 && more) wait_vm<4 + 2 * LPT>();
           else wait_vm<4>();
-          __syncthreads();  // ... and P has been read
+          block_barrier();
         }
       }
     }
-    const Keep keep = keep_over(g, float(min(r0 + kC, kC)));
+    if (!more && !dst) break;  // nobody takes the state on
+    const Keep keep = r0 < 0 ? keep_first : keep_full;
     if (keep.near) {
 #pragma unroll
       for (int t = 0; t < NT; ++t)
@@ -492,7 +550,13 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
 #pragma unroll
         for (int r = 0; r < 16; ++r) S[t][r] *= keep.m;
     }
-    auto add_step = [&](auto sc) {
+    // weights lambda^(15 - token) of a 16-token step, made anew for every chunk: registers are short
+    float wv[8], gv = g2;
+    asm volatile("" : "+v"(gv));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) wv[e] = power(gv, 15 - (8 * (e >> 2) + 4 * h + (e & 3)));
+    bf16x8_t vp[2][3];  // the parts of w V of a 16-token step, and of the one after it
+    auto parts_of_v = [&](auto sc) {
       constexpr int s = decltype(sc)::value;
       float x[8];
       float f = power(g2, 48 - 16 * s);
@@ -500,30 +564,41 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
       unpack8(__builtin_bit_cast(uint4, join(vf[2 * s], vf[2 * s + 1])), x);
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] *= wv[e] * f;
-      const bf16x8_t hi = take_part(x), mid = take_part(x), lo = last_part(x);
+      vp[s & 1][0] = take_part(x);
+      vp[s & 1][1] = take_part(x);
+      vp[s & 1][2] = last_part(x);
+    };
+    auto add_step = [&](auto sc) {
+      constexpr int s = decltype(sc)::value;
       i32x2_t kf[2 * NT];
       lds_tr_tiles<16 * s * P, P>(lds_at(ktr, buf), kf);
-      const bf16x8_t parts[3] = {lo, mid, hi};
+      if constexpr (s < 3) parts_of_v(std::integral_constant<int, s + 1>{});
 #pragma unroll
-      for (int i = 0; i < 3; ++i)
+      for (int i = 2; i >= 0; --i)  // the smallest part first
 #pragma unroll
         for (int t = 0; t < NT; ++t)
-          S[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(join(kf[2 * t], kf[2 * t + 1]), parts[i], S[t], 0, 0, 0);
+          S[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(join(kf[2 * t], kf[2 * t + 1]), vp[s & 1][i], S[t], 0, 0, 0);
+      // the next step's parts between this step's products
+#pragma unroll
+      for (int i = 0; i < 3 * NT; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x2, 24 / NT, 0);
+      }
       __builtin_amdgcn_sched_barrier(0);
     };
+    parts_of_v(std::integral_constant<int, 0>{});
     add_step(std::integral_constant<int, 0>{});
     add_step(std::integral_constant<int, 1>{});
     add_step(std::integral_constant<int, 2>{});
     add_step(std::integral_constant<int, 3>{});
     wait_vm<0>();  // the next chunk has landed
-    __syncthreads();
+    block_barrier();
   }
-  float* dst = OUT ? (sg.s == sg.count - 1 ? pool : nullptr) : id + 1 < a.segments ? ws + int64_t(a.Hkv) * D * D : nullptr;
   if (dst) {
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) dst[(32 * t + 16 * (r >> 3) + (r & 7)) * D] = S[t][r];
+      for (int r = 0; r < 16; ++r) dst[elem + (32 * t + 16 * (r >> 3) + (r & 7)) * D] = S[t][r];
   }
 }
 
