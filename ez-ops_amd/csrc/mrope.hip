@@ -12,7 +12,9 @@
 // axis i % A while that axis has pairs left, else to axis 0.
 //
 // The work is memory traffic: q and k in and out, v into the cache, 2 D bytes a
-// head each; the table rows are shared by the heads of a token.
+// head each; the table rows are shared by the heads of a token.  Measured: 16384
+// tokens of 32 + 2 x 8 heads of 128 80 us, 5.1 TB/s (a large copy reaches 4.9); 4097
+// tokens of 16 + 2 x 8 17 us; 16 tokens 5.3 us, a launch and three dependent loads.
 #include "common.h"
 #include "internal.h"
 #include "prof.h"
@@ -136,7 +138,191 @@ __global__ __launch_bounds__(256) void qk_norm_mrope_kernel(MropeArgs a) {
   }
 }
 
+// Sum over the LPG lanes of a group (4, 8, 16 or 32 neighbours); every lane gets it.
+template <int LPG>
+__device__ __forceinline__ float group_sum(float v) {
+  v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0xB1, 0xF, 0xF, true));   // quad_perm [1,0,3,2]
+  v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x4E, 0xF, 0xF, true));   // quad_perm [2,3,0,1]
+  if constexpr (LPG >= 8)
+    v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x141, 0xF, 0xF, true));  // row_half_mirror
+  if constexpr (LPG >= 16)
+    v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x140, 0xF, 0xF, true));  // row_mirror
+  if constexpr (LPG >= 32) {
+    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  }
+  return v;
+}
+
+// Table entries of this lane's 8 pairs at row p.
+__device__ __forceinline__ void load8(const uint16_t* p, float (&f)[8]) { unpack8(*reinterpret_cast<const uint4*>(p), f); }
+__device__ __forceinline__ void load8(const float* p, float (&f)[8]) {
+  const float4 x = reinterpret_cast<const float4*>(p)[0], y = reinterpret_cast<const float4*>(p)[1];
+  f[0] = x.x; f[1] = x.y; f[2] = x.z; f[3] = x.w;
+  f[4] = y.x; f[5] = y.y; f[6] = y.z; f[7] = y.w;
+}
+
+// 16-byte accesses, with the non-temporal hint where NT.
+template <bool NT>
+__device__ __forceinline__ uint4 load16(const uint16_t* p) {
+  if constexpr (NT) return ld16_stream(p);
+  return *reinterpret_cast<const uint4*>(p);
+}
+template <bool NT>
+__device__ __forceinline__ void store16(uint16_t* p, const uint4& v) {
+  const u32x4_t x = {v.x, v.y, v.z, v.w};
+  if constexpr (NT) __builtin_nontemporal_store(x, reinterpret_cast<u32x4_t*>(p));
+  else *reinterpret_cast<u32x4_t*>(p) = x;
+}
+
+// D a multiple of 16 with everything on 16 bytes: a group of LPG lanes (the power of two from D / 16 on)
+// per token and HPT heads (q, then k, then with a cache v, which is only copied), lane l holding pairs
+// 8l..8l+7, so that rotation needs no exchange, the norm one sum over the group, and the table entries
+// (chosen by axis) are read once for all HPT heads.
+template <int LPG, int HPT, bool NT, class TAB>
+__global__ __launch_bounds__(256) void qk_norm_mrope_vec_kernel(MropeArgs a, uint32_t groups) {
+  EZ_PROF_WAVE(kProfQkMrope);
+  const int l = threadIdx.x % LPG;
+  const uint32_t g = blockIdx.x * (256 / LPG) + threadIdx.x / LPG;
+  const uint32_t tok = g / groups;
+  const int u0 = int(g - tok * groups) * HPT, half = a.D / 2;
+  const int heads = a.H + a.Hkv, units = heads + (a.Kc ? a.Hkv : 0);
+  const int64_t t = tok;
+  if (t >= a.T) return;
+  const bool lane_on = 8 * l < half;  // lanes behind the head's last pair only join the sums
+  const int at = lane_on ? 8 * l : 0;
+  uint4 x1[HPT], x2[HPT];
+#pragma unroll
+  for (int i = 0; i < HPT; ++i) {
+    const int u = min(u0 + i, units - 1);
+    const uint16_t* src = at + (u < a.H     ? a.q + t * a.q_rs + int64_t(u) * a.D
+                                : u < heads ? a.k + t * a.k_rs + int64_t(u - a.H) * a.D
+                                            : a.v + t * a.v_rs + int64_t(u - heads) * a.D);
+    x1[i] = load16<NT>(src);
+    x2[i] = load16<NT>(src + half);
+  }
+  int pos[kMaxAxes];
+  bool ok = true;
+#pragma unroll
+  for (int n = 0; n < kMaxAxes; ++n) {
+    pos[n] = n < a.A ? a.positions[n * a.T + t] : 0;
+    ok &= pos[n] >= 0 && pos[n] < a.S;
+  }
+  const int64_t slot = a.Kc ? a.slots[t] : -1;
+  const bool cached = slot >= 0 && slot < a.num_slots;
+  if (!ok) return;  // the whole group
+
+  float c[8], s[8];
+  load8(static_cast<const TAB*>(a.cos) + int64_t(pos[0]) * a.D + at, c);
+  load8(static_cast<const TAB*>(a.sin) + int64_t(pos[0]) * a.D + at, s);
+  if (a.A > 1) {
+    int ax[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ax[e] = axis_of(a, at + e);
+#pragma unroll
+    for (int n = 1; n < kMaxAxes; ++n) {
+      if (n < a.A) {
+        float cn[8], sn[8];
+        load8(static_cast<const TAB*>(a.cos) + int64_t(pos[n]) * a.D + at, cn);
+        load8(static_cast<const TAB*>(a.sin) + int64_t(pos[n]) * a.D + at, sn);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          c[e] = ax[e] == n ? cn[e] : c[e];
+          s[e] = ax[e] == n ? sn[e] : s[e];
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < HPT; ++i) {
+    const int u = u0 + i;  // the group as a whole has it or not
+    const bool is_q = u < a.H;
+    uint4 p1 = x1[i], p2 = x2[i];
+    if (u < heads) {
+      float y1[8], y2[8];
+      unpack8(x1[i], y1);
+      unpack8(x2[i], y2);
+      if (a.norm) {
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss += y1[e] * y1[e] + y2[e] * y2[e];
+        const float r = rsqrtf(group_sum<LPG>(lane_on ? ss : 0.f) / float(a.D) + a.eps);
+        const uint16_t* w = is_q ? a.qw : a.kw;
+        float w1[8], w2[8];
+        if (w) {
+          load8(w + at, w1);
+          load8(w + at + half, w2);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          y1[e] = __fmul_rn(y1[e], r);
+          y2[e] = __fmul_rn(y2[e], r);
+          if (w) {
+            y1[e] = __fmul_rn(y1[e], w1[e]);
+            y2[e] = __fmul_rn(y2[e], w2[e]);
+          }
+        }
+      }
+      float o1[8], o2[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        o1[e] = __fadd_rn(__fmul_rn(y1[e], c[e]), __fmul_rn(-y2[e], s[e]));
+        o2[e] = __fadd_rn(__fmul_rn(y2[e], c[e]), __fmul_rn(y1[e], s[e]));
+      }
+      p1 = make_uint4(pack_bf2(o1[0], o1[1]), pack_bf2(o1[2], o1[3]), pack_bf2(o1[4], o1[5]), pack_bf2(o1[6], o1[7]));
+      p2 = make_uint4(pack_bf2(o2[0], o2[1]), pack_bf2(o2[2], o2[3]), pack_bf2(o2[4], o2[5]), pack_bf2(o2[6], o2[7]));
+    }
+    if (lane_on && u < units) {
+      uint16_t* dst = is_q ? a.q_out + (t * a.H + u) * a.D : a.k_out && u < heads ? a.k_out + (t * a.Hkv + u - a.H) * a.D : nullptr;
+      if (dst) {
+        store16<NT>(dst + at, p1);
+        store16<NT>(dst + at + half, p2);
+      }
+      if (!is_q && cached) {
+        uint16_t* pool = u < heads ? a.Kc + slot_offset(a, slot, u - a.H) : a.Vc + slot_offset(a, slot, u - heads);
+        store16<NT>(pool + at, p1);
+        store16<NT>(pool + at + half, p2);
+      }
+    }
+  }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+bool vec_form(const MropeArgs& a) {
+  return a.D % 16 == 0 && a.q_rs % 8 == 0 && a.k_rs % 8 == 0 && a.v_rs % 8 == 0 && aligned16(a.q) && aligned16(a.k) &&
+         aligned16(a.v) && aligned16(a.qw) && aligned16(a.kw) && aligned16(a.cos) && aligned16(a.sin) && aligned16(a.Kc) &&
+         aligned16(a.Vc) && aligned16(a.q_out) && aligned16(a.k_out) && a.T * (a.H + 2 * a.Hkv) < (int64_t(1) << 31);
+}
+
+template <int LPG, int HPT, bool NT>
+void launch_vec(const MropeArgs& a, hipStream_t s) {
+  const uint32_t groups = uint32_t((a.H + (a.Kc ? 2 : 1) * a.Hkv + HPT - 1) / HPT);
+  const dim3 grid(unsigned((a.T * groups + 256 / LPG - 1) / (256 / LPG)));
+  if (a.table_f32) hipLaunchKernelGGL((qk_norm_mrope_vec_kernel<LPG, HPT, NT, float>), grid, dim3(256), 0, s, a, groups);
+  else hipLaunchKernelGGL((qk_norm_mrope_vec_kernel<LPG, HPT, NT, uint16_t>), grid, dim3(256), 0, s, a, groups);
+}
+
+template <int LPG>
+void launch_vec(const MropeArgs& a, hipStream_t s) {
+  const int64_t heads = a.H + (a.Kc ? 2 : 1) * a.Hkv;
+  // Four heads a group once that still gives every CU 512 threads (16 + 2 x 8 heads of 128: 1024 tokens take 8.2 us
+  // with one head a group and 9.0 with four, 2048 tokens 12.8 and 11.4), and the non-temporal hint once the heads
+  // read and written pass three quarters of the memory-side cache: 16384 tokens of 32 + 2 x 8 heads (400 MB) take
+  // 80 us with it and 92 without, 9999 tokens of 16 + 16 heads of 80 (102 MB) 31 and 22.
+  if (a.T * heads * LPG < int64_t(8) * 256 * 256) launch_vec<LPG, 1, false>(a, s);
+  else if (a.T * heads * a.D * 4 < int64_t(192) << 20) launch_vec<LPG, 4, false>(a, s);
+  else launch_vec<LPG, 4, true>(a, s);
+}
+
 int launch_mrope(const MropeArgs& a, hipStream_t s) {
+  if (vec_form(a)) {
+    if (a.D <= 64) launch_vec<4>(a, s);
+    else if (a.D <= 128) launch_vec<8>(a, s);
+    else if (a.D <= 256) launch_vec<16>(a, s);
+    else launch_vec<32>(a, s);
+    return launch_status("qk_norm_mrope");
+  }
   const int64_t blocks = (a.T * (a.H + a.Hkv) + 3) / 4;
   hipLaunchKernelGGL(qk_norm_mrope_kernel, dim3(unsigned(blocks < (1 << 20) ? blocks : 1 << 20)), dim3(256), 0, s, a);
   return launch_status("qk_norm_mrope");
