@@ -201,22 +201,45 @@ def check(t: torch.Tensor, name: str, shape: tuple, dtype: torch.dtype) -> None:
 
 
 def check_rows(t: torch.Tensor, name: str, shape: tuple, dtype: torch.dtype) -> int:
-    """``check`` for a tensor whose rows (all dims behind the first) are contiguous and may lie apart, as slices of
-    a packed projection do; returns the distance of the rows in elements."""
+    """``check`` for a [rows, heads, dim] tensor whose rows are contiguous and may lie apart, as slices of a packed
+    projection do; returns the distance of the rows in elements."""
+    _, heads, dim = shape
+    n = heads * dim
+    if t.shape == shape and t.dtype is dtype:
+        st = t.stride()
+        if st[2] == 1 and st[1] == dim and st[0] >= n:
+            return st[0]
     if tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.dtype != dtype:
         raise ValueError(f"{name}: expected dtype {dtype}, got {t.dtype}")
-    n = 1
-    for size_, stride_ in zip(reversed(shape[1:]), reversed(t.stride()[1:])):
-        if size_ != 1 and stride_ != n:
-            raise ValueError(f"{name}: the dims behind the first must be contiguous, got strides {t.stride()}")
-        n *= size_
+    st = t.stride()
+    if (dim > 1 and st[2] != 1) or (heads > 1 and st[1] != dim):
+        raise ValueError(f"{name}: the dims behind the first must be contiguous, got strides {st}")
     if shape[0] <= 1:
         return n
-    if t.stride(0) < n:
-        raise ValueError(f"{name}: rows must not overlap, got a row stride of {t.stride(0)} elements for {n}")
-    return t.stride(0)
+    if st[0] < n:
+        raise ValueError(f"{name}: rows must not overlap, got a row stride of {st[0]} elements for {n}")
+    return st[0]
+
+
+def check_all(specs: tuple, *tensors: torch.Tensor) -> None:
+    """``check`` of every tensor against its (name, shape, dtype) in one go."""
+    for (name, shape, dtype), t in zip(specs, tensors):
+        if not (t.shape == shape and t.dtype is dtype and t.is_contiguous()):
+            check(t, name, shape, dtype)
+
+
+def one_gpu(first: torch.Tensor, *tensors: torch.Tensor | None) -> torch.device:
+    """``require_gpu`` with one lookup per tensor."""
+    index = first.get_device()
+    if index >= 0:
+        for t in tensors:
+            if t is not None and t.get_device() != index:
+                break
+        else:
+            return first.device
+    return require_gpu(first, *tensors)
 
 
 class Workspace:

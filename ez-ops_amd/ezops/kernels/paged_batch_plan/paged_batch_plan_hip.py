@@ -12,34 +12,34 @@ from ..base_kernel import BaseKernel
 class PagedBatchPlanHipKernel(BaseKernel):
     def __init__(self, batch: int, num_tokens: int, page_size: int, max_pages: int, num_pages: int, num_free: int):
         self.B, self.T, self.P, self.M, self.NP, self.NF = batch, num_tokens, page_size, max_pages, num_pages, num_free
+        i32, i64 = torch.int32, torch.int64
+        self._in = (("q_lens", (batch,), i32), ("block_table", (batch, max_pages), i32), ("free_pages", (num_free,), i32))
+        self._past = (("past_lens", (batch,), i32),)
+        self._out = (("out.cu_seqlens", (batch + 1,), i32), ("out.kv_lens", (batch,), i32),
+                     ("out.positions", (num_tokens,), i32), ("out.slot_mapping", (num_tokens,), i64),
+                     ("out.free_span", (3,), i32))
 
     def __call__(self, q_lens, past_lens, block_table, free_pages, free_span, out=None):
-        from ...ops.paged_batch_plan import PagedBatchPlan
-
-        dev = _hip.require_gpu(q_lens, past_lens, block_table, free_pages, free_span)
-        i32, B, T = torch.int32, self.B, self.T
-        _hip.check(q_lens, "q_lens", (B,), i32)
-        if past_lens is not None:
-            _hip.check(past_lens, "past_lens", (B,), i32)
-        _hip.check(block_table, "block_table", (B, self.M), i32)
-        _hip.check(free_pages, "free_pages", (self.NF,), i32)
-        if free_span.dim() != 1 or free_span.numel() < 2:
-            raise ValueError(f"free_span: expected (head, tail), got shape {tuple(free_span.shape)}")
-        _hip.check(free_span, "free_span", tuple(free_span.shape), i32)
-        if out is None:
-            out = PagedBatchPlan(torch.empty(B + 1, dtype=i32, device=dev), torch.empty(B, dtype=i32, device=dev),
-                                 torch.empty(T, dtype=i32, device=dev), torch.empty(T, dtype=torch.int64, device=dev),
-                                 torch.empty(3, dtype=i32, device=dev))
+        given = out is not None
+        if given:
+            cu, kv, positions, slots, span = out
+            dev = _hip.one_gpu(q_lens, past_lens, block_table, free_pages, free_span, cu, kv, positions, slots, span)
+            _hip.check_all(self._out, cu, kv, positions, slots, span)
         else:
-            if _hip.require_gpu(*out) != dev:
-                raise RuntimeError(f"out is not on {dev}")
-            _hip.check(out.cu_seqlens, "out.cu_seqlens", (B + 1,), i32)
-            _hip.check(out.kv_lens, "out.kv_lens", (B,), i32)
-            _hip.check(out.positions, "out.positions", (T,), i32)
-            _hip.check(out.slot_mapping, "out.slot_mapping", (T,), torch.int64)
-            _hip.check(out.free_span, "out.free_span", (3,), i32)
-        _hip.call_on(dev, "ezops_paged_batch_plan", q_lens.data_ptr(), _hip.ptr(past_lens), block_table.data_ptr(),
-                     free_pages.data_ptr(), free_span.data_ptr(), out.cu_seqlens.data_ptr(), out.kv_lens.data_ptr(),
-                     out.positions.data_ptr(), out.slot_mapping.data_ptr(), out.free_span.data_ptr(), B, T, self.P,
-                     self.M, self.NP, self.NF)
+            dev = _hip.one_gpu(q_lens, past_lens, block_table, free_pages, free_span)
+        _hip.check_all(self._in, q_lens, block_table, free_pages)
+        if past_lens is not None:
+            _hip.check_all(self._past, past_lens)
+        if free_span.dtype is not torch.int32 or free_span.dim() != 1 or free_span.shape[0] < 2 or free_span.stride(0) != 1:
+            raise ValueError("free_span: expected a contiguous int32 tensor of two or more (head, tail), got shape "
+                             f"{tuple(free_span.shape)}, {free_span.dtype}")
+        if not given:
+            from ...ops.paged_batch_plan import PagedBatchPlan
+
+            cu, kv, positions, slots, span = out = PagedBatchPlan(
+                *(torch.empty(shape, dtype=dtype, device=dev) for _, shape, dtype in self._out))
+        _hip.call_on(dev, "ezops_paged_batch_plan", q_lens.data_ptr(), None if past_lens is None else past_lens.data_ptr(),
+                     block_table.data_ptr(), free_pages.data_ptr(), free_span.data_ptr(), cu.data_ptr(), kv.data_ptr(),
+                     positions.data_ptr(), slots.data_ptr(), span.data_ptr(), self.B, self.T, self.P, self.M, self.NP,
+                     self.NF)
         return out

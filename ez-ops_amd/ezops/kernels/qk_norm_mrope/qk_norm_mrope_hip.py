@@ -9,8 +9,6 @@ from ... import _hip
 from ...registry import register_kernel
 from ..base_kernel import BaseKernel
 
-_TABLES = (torch.bfloat16, torch.float32)
-
 
 @register_kernel("qk_norm_mrope", "hip", family="ragged")
 class QkNormMropeHipKernel(BaseKernel):
@@ -21,10 +19,17 @@ class QkNormMropeHipKernel(BaseKernel):
         self.A, self.interleaved, self.norm, self.eps = len(sections), int(interleaved), int(norm), eps
         self._sections = (ctypes.c_int64 * self.A)(*sections)
         self.P, self.NP = page_size, num_pages
+        T, H, Hkv, D, S, bf = num_tokens, num_heads, num_kv_heads, head_dim, max_position, torch.bfloat16
+        self._q, self._kv = (T, H, D), (T, Hkv, D)
+        self._positions = (("positions", (self.A, T), torch.int32),)
+        self._tables = {d: (("cos", (S, D), d), ("sin", (S, D), d)) for d in (bf, torch.float32)}
+        self._qw, self._kw = (("q_norm_w", (D,), bf),), (("k_norm_w", (D,), bf),)
+        pool = (num_pages, Hkv, page_size, D)
+        self._cache = (("K_cache", pool, bf), ("V_cache", pool, bf), ("slot_mapping", (T,), torch.int64))
+        self._q_out, self._k_out = (("q_out", (T, H, D), bf),), (("k_out", (T, Hkv, D), bf),)
 
     def __call__(self, q, k, v, q_norm_w, k_norm_w, cos, sin, positions, K_cache=None, V_cache=None, slot_mapping=None, *,
                  q_out=None, k_out=None):
-        T, H, Hkv, D, S = self.T, self.H, self.Hkv, self.D, self.S
         paged = self.P is not None
         if paged != (K_cache is not None) or paged != (V_cache is not None) or paged != (slot_mapping is not None):
             raise ValueError("K_cache, V_cache and slot_mapping are required with a paged cache and only then")
@@ -32,38 +37,36 @@ class QkNormMropeHipKernel(BaseKernel):
             raise ValueError("v is required with a cache")
         if not self.norm and (q_norm_w is not None or k_norm_w is not None):
             raise ValueError("norm weights given to an op without norm")
-        dev = _hip.require_gpu(q, k, v, q_norm_w, k_norm_w, cos, sin, positions, K_cache, V_cache, slot_mapping, q_out,
-                               k_out)
+        dev = _hip.one_gpu(q, k, v, q_norm_w, k_norm_w, cos, sin, positions, K_cache, V_cache, slot_mapping, q_out, k_out)
         bf = torch.bfloat16
-        q_rs = _hip.check_rows(q, "q", (T, H, D), bf)
-        k_rs = _hip.check_rows(k, "k", (T, Hkv, D), bf)
-        v_rs = _hip.check_rows(v, "v", (T, Hkv, D), bf) if paged else 0
+        q_rs = _hip.check_rows(q, "q", self._q, bf)
+        k_rs = _hip.check_rows(k, "k", self._kv, bf)
         if q_norm_w is not None:
-            _hip.check(q_norm_w, "q_norm_w", (D,), bf)
+            _hip.check_all(self._qw, q_norm_w)
         if k_norm_w is not None:
-            _hip.check(k_norm_w, "k_norm_w", (D,), bf)
-        table = cos.dtype
-        if table not in _TABLES:
-            raise ValueError(f"cos: expected bfloat16 or float32, got {table}")
-        _hip.check(cos, "cos", (S, D), table)
-        _hip.check(sin, "sin", (S, D), table)
-        _hip.check(positions, "positions", (self.A, T), torch.int32)
+            _hip.check_all(self._kw, k_norm_w)
+        tables = self._tables.get(cos.dtype)
+        if tables is None:
+            raise ValueError(f"cos: expected bfloat16 or float32, got {cos.dtype}")
+        _hip.check_all(tables, cos, sin)
+        _hip.check_all(self._positions, positions)
         if paged:
-            pool = (self.NP, Hkv, self.P, D)
-            _hip.check(K_cache, "K_cache", pool, bf)
-            _hip.check(V_cache, "V_cache", pool, bf)
-            _hip.check(slot_mapping, "slot_mapping", (T,), torch.int64)
-        if q_out is None:
-            q_out = torch.empty(T, H, D, dtype=bf, device=dev)
+            v_rs = _hip.check_rows(v, "v", self._kv, bf)
+            _hip.check_all(self._cache, K_cache, V_cache, slot_mapping)
+            cache = (slot_mapping.data_ptr(), K_cache.data_ptr(), V_cache.data_ptr(), self.NP, self.P)
+            v_ptr = v.data_ptr()
         else:
-            _hip.check(q_out, "q_out", (T, H, D), bf)
+            v_rs, v_ptr, cache = 0, None, (None, None, None, 0, 0)
+        if q_out is None:
+            q_out = torch.empty(self._q, dtype=bf, device=dev)
+        else:
+            _hip.check_all(self._q_out, q_out)
         if k_out is not None:
-            _hip.check(k_out, "k_out", (T, Hkv, D), bf)
+            _hip.check_all(self._k_out, k_out)
         elif not paged:
-            k_out = torch.empty(T, Hkv, D, dtype=bf, device=dev)
-        _hip.call_on(dev, "ezops_qk_norm_mrope_bf16", q.data_ptr(), q_rs, k.data_ptr(), k_rs,
-                     v.data_ptr() if paged else None, v_rs, _hip.ptr(q_norm_w), _hip.ptr(k_norm_w), self.norm,
-                     cos.data_ptr(), sin.data_ptr(), int(table is torch.float32), positions.data_ptr(), self.A,
-                     self._sections, self.interleaved, _hip.ptr(slot_mapping), _hip.ptr(K_cache), _hip.ptr(V_cache),
-                     self.NP or 0, self.P or 0, q_out.data_ptr(), _hip.ptr(k_out), T, H, Hkv, D, S, self.eps)
+            k_out = torch.empty(self._kv, dtype=bf, device=dev)
+        _hip.call_on(dev, "ezops_qk_norm_mrope_bf16", q.data_ptr(), q_rs, k.data_ptr(), k_rs, v_ptr, v_rs,
+                     _hip.ptr(q_norm_w), _hip.ptr(k_norm_w), self.norm, cos.data_ptr(), sin.data_ptr(),
+                     cos.dtype is torch.float32, positions.data_ptr(), self.A, self._sections, self.interleaved, *cache,
+                     q_out.data_ptr(), _hip.ptr(k_out), self.T, self.H, self.Hkv, self.D, self.S, self.eps)
         return q_out, k_out
