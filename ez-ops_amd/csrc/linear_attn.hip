@@ -34,6 +34,7 @@ struct LinAttnArgs {
   int64_t T, num_slots, max_q;
   int seg, seg_sh;            // prefill: tokens per segment (1 << seg_sh)
   int segments;               // prefill: segment numbers
+  int split;                  // prefill: blocks that share the query heads of a kv head
   float* ws;                  // prefill: [segments, Hkv, D, D] or NULL (one segment a sequence)
   int B, H, Hkv;
   float scale;
@@ -264,28 +265,37 @@ struct Segment {
 // Finds segment number `id`; false if there is none (every thread agrees).  Contains barriers.
 template <int THREADS>
 __device__ __forceinline__ bool find_segment(const LinAttnArgs& a, int id, Segment& g) {
-  __shared__ int s_row[2], s_slot, s_past;
+  __shared__ int s_seq[4];
   const int T = int(a.T);
+  // every thread looks at its sequences with all of their entries at once: one memory latency, not three
   int count = 0;  // sequences whose first segment number is at most id: the last of them is ours
+  int begin = 0, end = 0, slot = -1, past = 0;
   for (int c0 = 0; c0 < a.B; c0 += THREADS) {
     const int c = c0 + threadIdx.x;
     bool in = false;
-    if (c < a.B) in = (min(max(a.cu[c], 0), T) >> a.seg_sh) + c <= id;
+    if (c < a.B) {
+      const int r = min(max(a.cu[c], 0), T), e = min(a.cu[c + 1], T);
+      const int sl = a.state ? (a.state_slots ? a.state_slots[c] : c) : -1, p = a.past ? a.past[c] : 0;
+      in = (r >> a.seg_sh) + c <= id;
+      if (in) begin = r, end = e, slot = sl, past = p;
+    }
     count += __syncthreads_count(in);
   }
   const int b = __builtin_amdgcn_readfirstlane(count) - 1;
   if (b < 0) return false;
-  if (threadIdx.x == 0) {
-    s_row[0] = min(max(a.cu[b], 0), T);
-    s_row[1] = min(a.cu[b + 1], T);
-    s_slot = a.state ? (a.state_slots ? a.state_slots[b] : b) : -1;
-    s_past = a.past ? a.past[b] : 0;
+  if (int(threadIdx.x) == b % THREADS) {
+    // offsets that do not decrease: this thread's last sequence with a number at most id is b
+    s_seq[0] = begin;
+    s_seq[1] = end;
+    s_seq[2] = slot;
+    s_seq[3] = past;
   }
   __syncthreads();
   // out of LDS into scalar registers: every thread has the same
-  const int r0 = __builtin_amdgcn_readfirstlane(s_row[0]);
-  const int n = min(__builtin_amdgcn_readfirstlane(s_row[1]) - r0, int(a.max_q));
-  const int slot = __builtin_amdgcn_readfirstlane(s_slot);
+  const int r0 = __builtin_amdgcn_readfirstlane(s_seq[0]);
+  const int n = min(__builtin_amdgcn_readfirstlane(s_seq[1]) - r0, int(a.max_q));
+  slot = __builtin_amdgcn_readfirstlane(s_seq[2]);
+  past = __builtin_amdgcn_readfirstlane(s_seq[3]);
   if (a.state) {
     int dup = slot < 0 || slot >= a.num_slots;
     if (a.state_slots)
@@ -300,7 +310,7 @@ __device__ __forceinline__ bool find_segment(const LinAttnArgs& a, int id, Segme
   g.s = s;
   g.count = cnt;
   g.slot = slot;
-  g.cont = a.state && __builtin_amdgcn_readfirstlane(s_past) > 0;
+  g.cont = a.state && past > 0;
   g.row = r0 + (s ? first + ((s - 1) << a.seg_sh) : 0);
   g.len = s ? a.seg : first;
   return true;
@@ -313,13 +323,13 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
   EZ_PROF_WAVE(OUT ? kProfLinAttnPrefill : kProfLinAttnState);
   constexpr int THREADS = 2 * D, NT = D / 32, NK = D / 16, P = 2 * D;  // P: bytes of an LDS row
   constexpr int TILE = kC * P, LPT = TILE / 16 / THREADS;
-  // K in two buffers (read up to the end of its chunk), V and Q in one each: they are in
-  // registers before the next ones are asked for.  76 KiB at D = 128: two blocks a CU.
+  // K in two buffers (read up to the end of its chunk; the next one is asked for at the chunk's start), V and Q
+  // in one each: asked for once the ones before are in registers.  76 KiB at D = 128: two blocks a CU.
   __shared__ __align__(1024) uint16_t Ks[2][kC * D], Vs[OUT ? 1 : 2][kC * D], Qs[OUT ? kC * D : 8];
   __shared__ __align__(1024) uint16_t Ps[OUT ? 3 * 4 * 512 : 8];  // block of P x (16-key step, part) x lane x 8
   __shared__ float pw[96];
-  const int id = blockIdx.x / a.Hkv;
-  const int kvh = blockIdx.x % a.Hkv;
+  const int split = OUT ? a.split : 1, part = blockIdx.x % split;
+  const int kvh = blockIdx.x / split % a.Hkv, id = blockIdx.x / split / a.Hkv;
   Segment sg;
   if (!find_segment<THREADS>(a, id, sg)) return;
   if (!OUT && sg.s == sg.count - 1) return;
@@ -339,7 +349,7 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
   float* pool = sg.slot >= 0 ? a.state + (int64_t(sg.slot) * a.Hkv + kvh) * D * D : nullptr;
   float* ws = a.ws + (int64_t(id) * a.Hkv + kvh) * D * D;
   if (OUT && (sg.s > 0 || sg.cont)) {
-    const float* src = sg.count > 1 ? ws : pool;
+    const float* src = a.ws ? ws : pool;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -371,10 +381,8 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
           res, (__attribute__((address_space(3))) void*)(to + (i * THREADS + w * kWave) * 8), 16,
           off + uint32_t(i * RPL - back) * pitch, 0, 0, 0);
   };
-  auto load_kv = [&](int c) {
-    load_tile(a.k, a.k_rs, kvh, c, Ks[c & 1]);
-    load_tile(a.v, a.v_rs, kvh, c, Vs[OUT ? 0 : c & 1]);
-  };
+  auto load_k = [&](int c) { load_tile(a.k, a.k_rs, kvh, c, Ks[c & 1]); };
+  auto load_v = [&](int c) { load_tile(a.v, a.v_rs, kvh, c, Vs[OUT ? 0 : c & 1]); };
 
   // LDS read addresses in buffer 0
   const uint32_t kbase = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint16_t*)(&Ks[0][0])));
@@ -400,8 +408,8 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
   const uint32_t owr = obase + uint32_t(j * 64 + ((h ^ ((j >> 2) & 3)) << 4));
   const uint32_t ord = obase + uint32_t((lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 4) & 3)) << 4));
 
-  const int G = a.H / a.Hkv;
-  float* dst = OUT ? (sg.s == sg.count - 1 ? pool : nullptr) : id + 1 < a.segments ? ws + int64_t(a.Hkv) * D * D : nullptr;
+  const int G = a.H / a.Hkv / split, h0 = kvh * (a.H / a.Hkv) + part * G;  // this block's query heads
+  float* dst = OUT ? (sg.s == sg.count - 1 && part == 0 ? pool : nullptr) : id + 1 < a.segments ? ws + int64_t(a.Hkv) * D * D : nullptr;
   const Keep keep_first = uniform(keep_over(g, float(kC - pad))), keep_full = uniform(keep_over(g, float(kC)));
   // One 32 x 32 block of P (0: first keys and queries, 1: first keys, second queries, 2: second keys and
   // queries), weighted, in two parts: the operand of the product with V, four fragments.
@@ -434,24 +442,31 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
     }
     lds_write_frags4(pfr + 4096 * blk, pf);
   };
-  load_kv(0);
-  if constexpr (OUT) load_tile(a.q, a.q_rs, kvh * G, 0, Qs);
+  load_k(0);
+  load_v(0);
+  if constexpr (OUT) load_tile(a.q, a.q_rs, h0, 0, Qs);
   wait_vm<0>();
   __syncthreads();
   for (int c = 0; c < chunks; ++c) {
     const uint32_t buf = uint32_t(c & 1) * TILE;
     const int r0 = c * kC - pad;
     const bool more = c + 1 < chunks;
-    if (!OUT && more) load_kv(c + 1);
+    if (more) {
+      load_k(c + 1);
+      if (!OUT) load_v(c + 1);
+    }
     i32x2_t vf[8];
-    lds_tr_steps<P>(lds_at(vtr, OUT ? 0 : buf), vf);
+    if (!OUT) lds_tr_steps<P>(lds_at(vtr, buf), vf);
     if constexpr (OUT) {
       for (int hg = 0; hg < G; ++hg) {
-        const int hq = kvh * G + hg;
+        const int hq = h0 + hg;
         // blocks of P: wave w makes block w (0: first keys and queries, 1: first keys, second queries,
         // 2: second keys and queries); of two waves the first makes block 2 too
-        if (w < 3) make_p(w, buf);
-        if (D == 64 && w == 0) make_p(2, buf);
+        // three blocks of P for the waves: the one that goes without (or, of two waves, the one that makes two)
+        // is not on the same SIMD in the two blocks of a CU, which are 256 apart
+        const int odd = (blockIdx.x >> 8) & 1, blk = D == 64 ? w : (w + 2 * odd) & 3;
+        if (blk < 3) make_p(blk, buf);
+        if (D == 64 && w == odd) make_p(2, buf);
         __builtin_amdgcn_sched_barrier(0);
         bf16x8_t q[2][NK];
         lds_row<0>(lds_at(qrd, 0), q[0]);
@@ -490,10 +505,14 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
           for (int r = 0; r < 16; ++r) o[t][r] *= f;
         }
         __builtin_amdgcn_sched_barrier(0);
-        block_barrier();  // P is there; V and Q have been read
+        if (hg == 0 && c > 0) {  // V has landed; the next K need not have
+          if (more) wait_vm<LPT>();
+          else wait_vm<0>();
+        }
+        block_barrier();  // P and V are there, Q has been read
         if (hg + 1 < G) load_tile(a.q, a.q_rs, hq + 1, c, Qs);
-        else if (more) load_tile(a.q, a.q_rs, kvh * G, c + 1, Qs);
-        if (hg == 0 && more) load_kv(c + 1);
+        else if (more) load_tile(a.q, a.q_rs, h0, c + 1, Qs);
+        if (hg == 0) lds_tr_steps<P>(lds_at(vtr, 0), vf);
         // what the chunk's own tokens give: block 0 to the first queries, blocks 1 and 2 to the second
         bf16x8_t pa[12];
         lds_frags12(pfr, pa);
@@ -504,7 +523,8 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
           o[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v0, pa[i], o[0], 0, 0, 0);
           o[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v1, pa[8 + i], o[1], 0, 0, 0);
         }
-        block_barrier();  // P has been read: its place serves the outputs
+        block_barrier();  // P has been read: its place serves the outputs; V is in registers
+        if (hg == 0 && more) load_v(c + 1);
         // o[t][4e + x] = O^T[column 8e + 4h + x][query j]: the lane halves swap groups, so that each holds
         // 16 bytes of a row, columns 16p + 8h..+7; through LDS to four lanes a row (stores of 64 lanes on
         // 64 lines cost the address unit four times as much)
@@ -527,11 +547,11 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
             if (row >= 0) *reinterpret_cast<u32x4_t*>(a.out + ((sg.row + row) * a.H + hq) * D + 32 * w + 8 * (lane & 3)) = y[i];
           }
         }
+        // The next Q has landed: behind it in the counter are this head's four stores (all there unless the
+        // chunk is short) and, once a chunk, the next V.
         if (hg + 1 < G) {
-          // the next head's Q has landed: in front of it in the counter are this head's four stores (all
-          // there unless the chunk is short) and, once a chunk, the next K and V
           if (r0 < 0) wait_vm<0>();
-          else if (hg == 0 && more) wait_vm<4 + 2 * LPT>();
+          else if (hg == 0 && more) wait_vm<4 + LPT>();
           else wait_vm<4>();
           block_barrier();
         }
@@ -591,7 +611,9 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
     add_step(std::integral_constant<int, 1>{});
     add_step(std::integral_constant<int, 2>{});
     add_step(std::integral_constant<int, 3>{});
-    wait_vm<0>();  // the next chunk has landed
+    if (!OUT) wait_vm<0>();  // the next chunk has landed
+    else if (G > 1) r0 < 0 ? wait_vm<0>() : wait_vm<4>();  // the next K and Q have: behind them are four stores
+    else r0 < 0 ? wait_vm<LPT>() : wait_vm<4 + LPT>();      // ... and the next V
     block_barrier();
   }
   if (dst) {
@@ -604,7 +626,7 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
 
 // The workspace's slot of segment s > 0 holds the sum of segment s - 1; becomes the state
 // before segment s.  Slot 0 gets the stored state where the sequence continues (the output
-// kernel's last segment overwrites the pool while its first may still have to start).
+// kernel overwrites the pool while blocks that start from there may still have to read it).
 // Block = (sequence, kv head, 256 elements), one element a thread: the chain over the segments is
 // short of work per step, so the chip is filled with threads, each eight loads ahead of its sums.
 template <int D>
@@ -613,7 +635,9 @@ __global__ __launch_bounds__(256) void linear_attn_scan_kernel(LinAttnArgs a) {
   constexpr int PARTS = D * D / 256, AHEAD = 8;
   const int part = blockIdx.x % PARTS, kvh = blockIdx.x / PARTS % a.Hkv, b = blockIdx.x / PARTS / a.Hkv;
   const int T = int(a.T), r0 = min(max(a.cu[b], 0), T), n = min(min(a.cu[b + 1], T) - r0, int(a.max_q));
-  if (n <= a.seg) return;
+  if (n <= 0) return;
+  const bool cont = a.state && a.past && a.past[b] > 0;
+  if (n <= a.seg && !cont) return;
   int slot = -1;
   if (a.state) {
     slot = slot_of<256>(a, b);
@@ -621,7 +645,6 @@ __global__ __launch_bounds__(256) void linear_attn_scan_kernel(LinAttnArgs a) {
   }
   const int cnt = (n + a.seg - 1) >> a.seg_sh, id = (r0 >> a.seg_sh) + b;
   const int last = min(cnt, a.segments - id);  // decreasing offsets must not lead past the workspace
-  if (last < 2) return;
   const int at = part * 256 + int(threadIdx.x);
   const int64_t step = int64_t(a.Hkv) * D * D;
   float* ws = a.ws + (int64_t(id) * a.Hkv + kvh) * D * D + at;
@@ -630,16 +653,16 @@ __global__ __launch_bounds__(256) void linear_attn_scan_kernel(LinAttnArgs a) {
     for (int i = 0; i < AHEAD; ++i) x[i] = ws[min(s0 + i, last - 1) * step];
   };
   float x[AHEAD], next[AHEAD];
-  load(x, 1);
+  if (last > 1) load(x, 1);
   float S = 0.f;
-  if (slot >= 0 && a.past && a.past[b] > 0) {
+  if (cont) {
     S = a.state[(int64_t(slot) * a.Hkv + kvh) * D * D + at];
     ws[0] = S;
   }
   const float g = a.log_decay[kvh];
   const Keep first = keep_over(g, float(n - ((cnt - 1) << a.seg_sh))), rest = keep_over(g, float(a.seg));
   for (int s0 = 1; s0 < last; s0 += AHEAD) {
-    load(next, s0 + AHEAD);
+    if (s0 + AHEAD < last) load(next, s0 + AHEAD);
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
       if (s0 + i < last) {
@@ -652,11 +675,22 @@ __global__ __launch_bounds__(256) void linear_attn_scan_kernel(LinAttnArgs a) {
 }
 
 // log2 of the tokens per segment: the longest segments that still give about 512 blocks over the whole
-// batch, at least a chunk.
-int segment_shift(int64_t T, int64_t Hkv) {
+// batch, two a CU (32 / 8 heads, all three kernels: 16384 tokens 125 us, with 256 blocks 136); two chunks
+// as soon as that gives one block a CU (4096 tokens: 54 us, with 512 blocks of a chunk 57: each segment costs
+// 256 KiB of state traffic a kv head); at least a chunk.  Two chunks of one or two query heads a kv head are not
+// cut at all (128 tokens of 8 / 8 heads 13.9 us, cut 18.4).
+int segment_shift(int64_t T, int64_t G, int64_t Hkv, int64_t max_q) {
   int sh = 6;
-  while ((T * Hkv) >> (sh + 1) >= 512) ++sh;
-  return sh;
+  while ((T * Hkv) >> (sh + 1) >= (sh < 7 ? 256 : 512)) ++sh;
+  return G <= 2 && max_q <= 2 * kC && sh < 7 ? 7 : sh;
+}
+// Blocks a kv head's query heads are shared out to where the segments alone leave CUs without work (up to
+// about two a CU); each of them updates the state for itself, and the first leaves it.  64 tokens of
+// 32 / 8 heads: 9.6 us, in one block a kv head 16.4; 1024 tokens of 32 / 8: outputs 17.7, with 272 blocks 16.2.
+int head_split(int64_t blocks, int64_t G) {
+  int64_t n = 1;
+  while (2 * n <= G && blocks * 2 * n <= 576) n *= 2;
+  return int(n);
 }
 int64_t segment_count(int64_t B, int64_t T, int sh) { return (T >> sh) + B; }
 
@@ -737,8 +771,9 @@ int check_common(const LinAttnArgs& a, int64_t H, int64_t Hkv, int64_t D, const 
 extern "C" size_t ezops_linear_attn_prefill_workspace_size(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t D,
                                                            int64_t max_q_len) {
   if (B < 1 || T < 1 || Hkv < 1 || D < 1) return 0;
-  const int sh = ez::segment_shift(T, Hkv);
-  if ((max_q_len > 0 && max_q_len < T ? max_q_len : T) <= int64_t(1) << sh) return 0;
+  const int64_t max_q = max_q_len > 0 && max_q_len < T ? max_q_len : T;
+  const int sh = ez::segment_shift(T, H / Hkv, Hkv, max_q);
+  if (max_q <= int64_t(1) << sh) return 0;
   return size_t(ez::segment_count(B, T, sh)) * Hkv * D * D * sizeof(float);
 }
 
@@ -770,29 +805,31 @@ extern "C" int ezops_linear_attn_prefill_bf16(const void* q, int64_t q_stride, c
   a.scale = scale > 0.f ? scale : 1.f / sqrtf(float(D));
   EZ_REQUIRE(q_stride < (1 << 23) && k_stride < (1 << 23) && v_stride < (1 << 23),
              "linear_attn_prefill: token strides must be below 2^23");
-  a.seg_sh = ez::segment_shift(T, Hkv);
+  a.seg_sh = ez::segment_shift(T, H / Hkv, Hkv, a.max_q);
   a.seg = 1 << a.seg_sh;
   const int64_t segments = ez::segment_count(B, T, a.seg_sh);
   const size_t need = ezops_linear_attn_prefill_workspace_size(B, T, H, Hkv, D, max_q_len);
   EZ_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ez::aligned16(workspace)),
              "linear_attn_prefill: needs a 16-byte aligned workspace of %zu bytes", need);
-  EZ_REQUIRE(segments * Hkv < (int64_t(1) << 31) && B * Hkv < (int64_t(1) << 25),
+  EZ_REQUIRE(segments * Hkv < (int64_t(1) << 27) && B * Hkv < (int64_t(1) << 25),
              "linear_attn_prefill: too many sequences and heads for one launch");
   a.segments = int(segments);
-  a.ws = static_cast<float*>(workspace);
-  const dim3 grid(unsigned(segments * Hkv)), parts(unsigned(B * Hkv * (D * D / 256)));
+  a.ws = need ? static_cast<float*>(workspace) : nullptr;
+  // without a workspace the first block's last state would meet the others' reads of the stored one
+  a.split = need || !state || !past_lens ? ez::head_split(segments * Hkv, H / Hkv) : 1;
+  const dim3 grid(unsigned(segments * Hkv)), outs(unsigned(segments * Hkv * a.split)), parts(unsigned(B * Hkv * (D * D / 256)));
   if (D == 64) {
     if (need) {
       hipLaunchKernelGGL((ez::linear_attn_chunk_kernel<64, false>), grid, dim3(128), 0, stream, a);
       hipLaunchKernelGGL(ez::linear_attn_scan_kernel<64>, parts, dim3(256), 0, stream, a);
     }
-    hipLaunchKernelGGL((ez::linear_attn_chunk_kernel<64, true>), grid, dim3(128), 0, stream, a);
+    hipLaunchKernelGGL((ez::linear_attn_chunk_kernel<64, true>), outs, dim3(128), 0, stream, a);
   } else {
     if (need) {
       hipLaunchKernelGGL((ez::linear_attn_chunk_kernel<128, false>), grid, dim3(256), 0, stream, a);
       hipLaunchKernelGGL(ez::linear_attn_scan_kernel<128>, parts, dim3(256), 0, stream, a);
     }
-    hipLaunchKernelGGL((ez::linear_attn_chunk_kernel<128, true>), grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((ez::linear_attn_chunk_kernel<128, true>), outs, dim3(256), 0, stream, a);
   }
   return ez::launch_status("linear_attn_prefill");
 }
