@@ -173,6 +173,24 @@ def test_long_sequences(H, Hkv, D, lens):
     _prefill(lens, past, H, Hkv, D, seed=5, max_q_len=0)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_more_sequences_than_threads(D):
+    """Sequences are found by a block of 128 or 256 threads: 300 short ones, some empty, some continued, a slot twice."""
+    r = np.random.RandomState(3)
+    lens = r.choice([0, 1, 2, 5, 70], 300, p=[0.2, 0.4, 0.2, 0.18, 0.02]).tolist()
+    slots = r.permutation(303)[:300].tolist()
+    slots[290] = slots[4]
+    _prefill(lens, r.choice([0, 3], 300).tolist(), 2, 1, D, slots=slots, pool=303, seed=9, pad=11)
+
+
+@pytest.mark.parametrize("H,lens,past", [(8, [64], [3]), (16, [100, 300], [7, 0]), (4, [130, 0, 64, 5], [1, 1, 1, 1])])
+def test_shared_query_heads_of_few_blocks(H, lens, past):
+    """The query heads of a kv head in several blocks, all of which start from the stored state that one replaces."""
+    for known in (None, 0):
+        _prefill(lens, past, H, 1, 128, seed=21, max_q_len=known)
+        _prefill(lens, [0] * len(lens), H, 1, 64, seed=22, max_q_len=known)
+
+
 def test_chunks_equal_the_whole():
     """A prompt in two calls through the state gives what one call gives (within the sum of both tolerances)."""
     H, Hkv, D, T = 4, 2, 128, 300
