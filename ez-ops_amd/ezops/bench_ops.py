@@ -212,6 +212,15 @@ def _qk_rope_f1(B):
 
 _F1_POS: dict = {}
 
+
+# ---- QK norm + rotary positions with several axes (no reference counterpart).  The other ragged-batch ops are not
+# here: their references read lengths on the host, which no graph takes.
+def _mrope(T, H, Hkv, D, sections, label, **kw):
+    from .ops.qk_norm_mrope import QkNormMropeOp
+
+    return Workload(label, f"{T} tokens  heads {H}q/{Hkv}kv x {D}  sections {sections}",
+                    lambda b: QkNormMropeOp(T, H, Hkv, D, 4096, sections, backend=b, **kw), _same)
+
 _OPF_SHAPES = {
     "qwen3-0.6b": dict(hidden_size=1024, intermediate_size=3072, num_heads=16, head_dim=128),
     "qwen3-vl-2b": dict(hidden_size=2048, intermediate_size=6144, num_heads=16, head_dim=128),
@@ -280,6 +289,10 @@ def registry() -> dict[str, OpBench]:
         "fused_qk_norm_rope": OpBench("fused_qk_norm_rope", "FusedQkNormRope", [
             _qk_rope(1, 128, "qwen3-s128"), _qk_rope(1, 1024, "qwen3-s1k"), _qk_rope(1, 4096, "qwen3-s4k"),
             _qk_rope(1, 8192, "qwen3-s8k"), _qk_rope(1, 32768, "qwen3-s32k"), _qk_rope_f1(1), _qk_rope_f1(16)]),
+        "qk_norm_mrope": OpBench("qk_norm_mrope", "QkNormMrope", [
+            _mrope(64, 16, 8, 128, (24, 20, 20), "qwen3-vl-2b-t64", interleaved=True),
+            _mrope(4096, 16, 8, 128, (24, 20, 20), "qwen3-vl-2b-t4k", interleaved=True),
+            _mrope(16384, 32, 8, 128, (16, 24, 24), "qwen3-8b-t16k")]),
         "fused_o_proj_ffn": OpBench("fused_o_proj_ffn", "FusedOProjFfn", [
             _oproj_ffn(1, "qwen3-0.6b", "qwen3-0.6b-b1"), _oproj_ffn(1, "qwen3-vl-2b", "qwen3-vl-2b-b1"),
             _oproj_ffn(1, "qwen3-8b", "config-F2-b1", cfg=True), _oproj_ffn(16, "qwen3-8b", "config-F2-b16", cfg=True)]),

@@ -152,13 +152,12 @@ class QkNormMropeOp(Op):
             return rope_half_f32(xf, c, s)
 
         qr, kr = turned(q, q_norm_w), turned(k, k_norm_w)
-        if q_out is None:
-            q_out = torch.empty_like(qr)
-        q_out[live] = qr[live]
-        if k_out is None and K_cache is None:
-            k_out = torch.empty_like(kr)
+        on = live[:, None, None]
+        q_out = qr if q_out is None else q_out.copy_(torch.where(on, qr, q_out))
         if k_out is not None:
-            k_out[live] = kr[live]
+            k_out.copy_(torch.where(on, kr, k_out))
+        elif K_cache is None:
+            k_out = kr
         if K_cache is not None:
             ok = live & (slot_mapping >= 0) & (slot_mapping < self.num_pages * self.page_size)
             slot = slot_mapping[ok]
