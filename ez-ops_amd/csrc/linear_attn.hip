@@ -211,17 +211,6 @@ __device__ __forceinline__ void lds_weights(uint32_t a, float (&r)[16]) {
         "=&v"(r[8]), "=&v"(r[9]), "=&v"(r[10]), "=&v"(r[11]), "=&v"(r[12]), "=&v"(r[13]), "=&v"(r[14]), "=&v"(r[15])
       : "v"(a));
 }
-// A wave's own 32 rows of 64 bytes, written 16 bytes a lane at `wr` and `wr ^ 32` and read back at
-// `rd` and 1 KiB further on.
-__device__ __forceinline__ void lds_turn(uint32_t wr, uint32_t rd, const uint4& x, const uint4& y, u32x4_t (&r)[2]) {
-  const u32x4_t a = {x.x, x.y, x.z, x.w}, b = {y.x, y.y, y.z, y.w};
-  asm volatile(
-      "ds_write_b128 %2, %4\n\tds_write_b128 %3, %5\n\ts_waitcnt lgkmcnt(0)\n\t"
-      "ds_read_b128 %0, %6\n\tds_read_b128 %1, %6 offset:1024\n\ts_waitcnt lgkmcnt(0)"
-      : "=&v"(r[0]), "=&v"(r[1])
-      : "v"(wr), "v"(wr ^ 32), "v"(a), "v"(b), "v"(rd)
-      : "memory");
-}
 __device__ __forceinline__ bf16x8_t join(const i32x2_t& x, const i32x2_t& y) {
   return as_bf16x8(make_uint4(uint32_t(x[0]), uint32_t(x[1]), uint32_t(y[0]), uint32_t(y[1])));
 }
@@ -402,12 +391,6 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
   // register r wants n = j - 8 (r / 4) - 4 h - r % 4
   const uint32_t pwrd = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const float*)(&pw[0]))) +
                         uint32_t(4 * (31 + j - 4 * h - 27));
-  // the outputs on their way: row j of the wave's 2 KiB, 16-byte chunk c at c ^ (row / 4 % 4)
-  const uint32_t obase = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint16_t*)(&Ps[0]))) +
-                         uint32_t(w * 2048);
-  const uint32_t owr = obase + uint32_t(j * 64 + ((h ^ ((j >> 2) & 3)) << 4));
-  const uint32_t ord = obase + uint32_t((lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 4) & 3)) << 4));
-
   const int G = a.H / a.Hkv / split, h0 = kvh * (a.H / a.Hkv) + part * G;  // this block's query heads
   float* dst = OUT ? (sg.s == sg.count - 1 && part == 0 ? pool : nullptr) : id + 1 < a.segments ? ws + int64_t(a.Hkv) * D * D : nullptr;
   const Keep keep_first = uniform(keep_over(g, float(kC - pad))), keep_full = uniform(keep_over(g, float(kC)));
@@ -451,6 +434,7 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
     const uint32_t buf = uint32_t(c & 1) * TILE;
     const int r0 = c * kC - pad;
     const bool more = c + 1 < chunks;
+    if (OUT && G == 1 && c > 0) load_v(c);  // with more heads it is asked for behind the first one
     if (more) {
       load_k(c + 1);
       if (!OUT) load_v(c + 1);
@@ -523,37 +507,28 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
           o[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v0, pa[i], o[0], 0, 0, 0);
           o[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v1, pa[8 + i], o[1], 0, 0, 0);
         }
-        block_barrier();  // P has been read: its place serves the outputs; V is in registers
-        if (hg == 0 && more) load_v(c + 1);
-        // o[t][4e + x] = O^T[column 8e + 4h + x][query j]: the lane halves swap groups, so that each holds
-        // 16 bytes of a row, columns 16p + 8h..+7; through LDS to four lanes a row (stores of 64 lanes on
-        // 64 lines cost the address unit four times as much)
+        // o[t][4e + x] = O^T[column 8e + 4h + x][query j]: the lane halves swap groups, so that each stores 16 bytes
+        // of a row, columns 16p + 8h..+7.  (Through LDS to four lanes a row: 1-5% slower for its barrier.)
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          uint4 x[2];
+          const int row = r0 + 32 * t + j;
+          uint16_t* op = a.out + (int64_t(sg.row + max(row, 0)) * a.H + hq) * D + 32 * w + 8 * h;
 #pragma unroll
           for (int p = 0; p < 2; ++p) {
             const auto u = __builtin_amdgcn_permlane32_swap(cvt_bf2(o[t][8 * p], o[t][8 * p + 1]),
                                                             cvt_bf2(o[t][8 * p + 4], o[t][8 * p + 5]), false, false);
             const auto v = __builtin_amdgcn_permlane32_swap(cvt_bf2(o[t][8 * p + 2], o[t][8 * p + 3]),
                                                             cvt_bf2(o[t][8 * p + 6], o[t][8 * p + 7]), false, false);
-            x[p] = make_uint4(u[0], v[0], u[1], v[1]);
-          }
-          u32x4_t y[2];
-          lds_turn(owr, ord, x[0], x[1], y);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int row = r0 + 32 * t + 16 * i + (lane >> 2);
-            if (row >= 0) *reinterpret_cast<u32x4_t*>(a.out + ((sg.row + row) * a.H + hq) * D + 32 * w + 8 * (lane & 3)) = y[i];
+            if (row >= 0) *reinterpret_cast<uint4*>(op + 16 * p) = make_uint4(u[0], v[0], u[1], v[1]);
           }
         }
         // The next Q has landed: behind it in the counter are this head's four stores (all there unless the
-        // chunk is short) and, once a chunk, the next V.
+        // chunk is short).  V is in registers, P has been read.
         if (hg + 1 < G) {
           if (r0 < 0) wait_vm<0>();
-          else if (hg == 0 && more) wait_vm<4 + LPT>();
           else wait_vm<4>();
           block_barrier();
+          if (hg == 0 && more) load_v(c + 1);
         }
       }
     }
@@ -612,8 +587,7 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
     add_step(std::integral_constant<int, 2>{});
     add_step(std::integral_constant<int, 3>{});
     if (!OUT) wait_vm<0>();  // the next chunk has landed
-    else if (G > 1) r0 < 0 ? wait_vm<0>() : wait_vm<4>();  // the next K and Q have: behind them are four stores
-    else r0 < 0 ? wait_vm<LPT>() : wait_vm<4 + LPT>();      // ... and the next V
+    else r0 < 0 ? wait_vm<0>() : wait_vm<4>();  // the next K and Q have: behind them are four stores
     block_barrier();
   }
   if (dst) {
