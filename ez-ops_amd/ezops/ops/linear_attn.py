@@ -13,7 +13,9 @@ a pool ``state [num_slots, Hkv, D, D]``; sequence ``b`` owns slot
 ``state_slots[b]`` (None: slot ``b``), updated in place.  A sequence whose slot is
 outside the pool (-1: a padded row of the batch), or that an earlier sequence of
 the batch holds already, is left out whole: its rows of ``out`` and every state
-stay as they were.
+stay as they were.  In a prompt a token whose k or v is not finite leaves its own
+sequence's outputs undefined from the first token of its 64-token chunk on; other
+sequences are not touched.
 """
 
 import torch
