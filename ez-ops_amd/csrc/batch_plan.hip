@@ -166,6 +166,14 @@ extern "C" int ezops_paged_batch_plan(const int32_t* q_lens, const int32_t* past
              "paged_batch_plan: max_pages * page_size must be in [page_size, 2^30]");
   EZ_REQUIRE(num_pages >= 1 && num_pages < (int64_t(1) << 31) && num_free >= 0 && num_free < (int64_t(1) << 30),
              "paged_batch_plan: num_pages must be in [1, 2^31) and num_free in [0, 2^30)");
+  // every block reads the inputs for itself, the first while others still have to: no output may be one of them
+  const struct { const void* p; int64_t n; } in[] = {{q_lens, 4 * B}, {past_lens, 4 * B}, {free_pages, 4 * num_free}, {free_span, 8}},
+      out[] = {{cu_seqlens, 4 * (B + 1)}, {kv_lens, 4 * B}, {positions, 4 * T}, {slot_mapping, 8 * T}, {free_span_out, 12},
+               {block_table, 4 * B * max_pages}};
+  for (const auto& x : in)
+    for (const auto& y : out)
+      EZ_REQUIRE(!ez::overlap(x.p, x.n, y.p, y.n), "paged_batch_plan: an output overlaps an input (copy the lengths or the "
+                 "span of the plan before that is written again)");
   ez::PlanArgs a{};
   a.q_lens = q_lens; a.past_lens = past_lens;
   a.table = block_table;

@@ -8,6 +8,12 @@
 
 namespace ez {
 
+// Whether two byte ranges share memory (a null pointer's none).
+inline bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a && b && x < y + uintptr_t(nb) && y < x + uintptr_t(na);
+}
+
 // "MFMA-packed" activation layout for the skinny GEMM (M > 4): batch rows
 // in blocks of 16, each 32-wide k-step of a block stored as the 1 KiB B
 // operand of v_mfma_f32_16x16x32_bf16 (lane 16 g + i holds row i, k-slots

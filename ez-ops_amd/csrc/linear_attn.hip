@@ -183,6 +183,12 @@ __device__ __forceinline__ void lds_tr_tiles(uint32_t a, i32x2_t (&r)[4]) {
 // A barrier without a wait: __syncthreads() waits for outstanding LDS DMA as well, which here is the next
 // chunk's.  LDS reads and writes in front of it have ended with waits of their own.
 __device__ __forceinline__ void block_barrier() { asm volatile("s_barrier" ::: "memory"); }
+// The same with at most N of this wave's memory operations still out.  One block, so that no store moves between the
+// wait that counts it and the barrier.
+template <int N>
+__device__ __forceinline__ void wait_vm_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"(N) : "memory");
+}
 
 // Twelve 1 KiB fragments in a row (16 bytes a lane).
 __device__ __forceinline__ void lds_frags12(uint32_t a, bf16x8_t (&r)[12]) {
@@ -495,11 +501,10 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
           for (int r = 0; r < 16; ++r) o[t][r] *= f;
         }
         __builtin_amdgcn_sched_barrier(0);
-        if (hg == 0 && c > 0) {  // V has landed; the next K need not have
-          if (more) wait_vm<LPT>();
-          else wait_vm<0>();
-        }
-        block_barrier();  // P and V are there, Q has been read
+        // P is there, Q has been read; for the first head V has landed (behind it is the next K)
+        if (hg > 0 || c == 0) block_barrier();
+        else if (more) wait_vm_barrier<LPT>();
+        else wait_vm_barrier<0>();
         if (hg + 1 < G) load_tile(a.q, a.q_rs, hq + 1, c, Qs);
         else if (more) load_tile(a.q, a.q_rs, h0, c + 1, Qs);
         if (hg == 0) lds_tr_steps<P>(lds_at(vtr, 0), vf);
@@ -531,9 +536,8 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
         // The next Q has landed: behind it in the counter are this head's four stores (all there unless the
         // chunk is short).  V is in registers, P has been read.
         if (hg + 1 < G) {
-          if (r0 < 0) wait_vm<0>();
-          else wait_vm<4>();
-          block_barrier();
+          if (r0 < 0) wait_vm_barrier<0>();
+          else wait_vm_barrier<4>();
           if (hg == 0 && more) load_v(c + 1);
         }
       }
@@ -592,9 +596,9 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
     add_step(std::integral_constant<int, 1>{});
     add_step(std::integral_constant<int, 2>{});
     add_step(std::integral_constant<int, 3>{});
-    if (!OUT) wait_vm<0>();  // the next chunk has landed
-    else r0 < 0 ? wait_vm<0>() : wait_vm<4>();  // the next K and Q have: behind them are four stores
-    block_barrier();
+    // the next chunk (OUT: the next K and Q) has landed: behind it are at most the four stores
+    if (!OUT || r0 < 0) wait_vm_barrier<0>();
+    else wait_vm_barrier<4>();
   }
   if (dst) {
 #pragma unroll
@@ -731,6 +735,16 @@ __global__ __launch_bounds__(256) void linear_attn_decode_kernel(LinAttnArgs a) 
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// out [rows, H, D] must not share memory with q, k or v: other blocks may still have to read them.
+int check_out(const LinAttnArgs& a, int64_t rows, int64_t D, const char* what) {
+  auto meets = [&](const uint16_t* x, int64_t rs, int64_t heads) {
+    return overlap(x, ((rows - 1) * rs + heads * D) * 2, a.out, rows * a.H * D * 2);
+  };
+  EZ_REQUIRE(!meets(a.q, a.q_rs, a.H) && !meets(a.k, a.k_rs, a.Hkv) && !meets(a.v, a.v_rs, a.Hkv),
+             "%s: out must not overlap q, k or v", what);
+  return EZ_OK;
+}
+
 int check_common(const LinAttnArgs& a, int64_t H, int64_t Hkv, int64_t D, const char* what) {
   EZ_REQUIRE(a.q && a.k && a.v && a.log_decay && a.out, "%s: null pointer", what);
   EZ_REQUIRE(Hkv >= 1 && H >= 1 && H <= 4096 && H % Hkv == 0, "%s: num_heads must be divisible by num_kv_heads", what);
@@ -793,6 +807,8 @@ extern "C" int ezops_linear_attn_prefill_bf16(const void* q, int64_t q_stride, c
              "linear_attn_prefill: needs a 16-byte aligned workspace of %zu bytes", need);
   EZ_REQUIRE(segments * Hkv < (int64_t(1) << 27) && B * Hkv < (int64_t(1) << 25),
              "linear_attn_prefill: too many sequences and heads for one launch");
+  const int out_rc = ez::check_out(a, T, D, "linear_attn_prefill");
+  if (out_rc != EZ_OK) return out_rc;
   a.segments = int(segments);
   a.ws = need ? static_cast<float*>(workspace) : nullptr;
   // without a workspace the first block's last state would meet the others' reads of the stored one
@@ -833,6 +849,8 @@ extern "C" int ezops_linear_attn_decode_bf16(const void* q, int64_t q_stride, co
   EZ_REQUIRE(num_slots >= 1 && num_slots < (int64_t(1) << 31), "linear_attn_decode: num_slots must be in [1, 2^31)");
   a.B = int(B); a.H = int(H); a.Hkv = int(Hkv);
   a.scale = scale > 0.f ? scale : 1.f / sqrtf(float(D));
+  const int out_rc = ez::check_out(a, B, D, "linear_attn_decode");
+  if (out_rc != EZ_OK) return out_rc;
   const dim3 grid(unsigned(B * Hkv));
   if (D == 64) hipLaunchKernelGGL((ez::linear_attn_decode_kernel<64, 64>), grid, dim3(256), 0, stream, a);
   else hipLaunchKernelGGL((ez::linear_attn_decode_kernel<128, 128>), grid, dim3(256), 0, stream, a);

@@ -378,5 +378,16 @@ extern "C" int ezops_qk_norm_mrope_bf16(const void* q, int64_t q_stride, const v
     a.page_sh = __builtin_ctzll(static_cast<unsigned long long>(page_size));
     a.num_slots = num_pages * page_size;
   }
+  // q_out in q's place and k_out in k's are fine (every lane reads what it writes first), other overlaps a race
+  auto span = [&](int64_t rs, int64_t heads) { return ((T - 1) * rs + heads * D) * 2; };
+  const int64_t nq = T * H * D * 2, nk = T * Hkv * D * 2;
+  EZ_REQUIRE((q_out == q && q_stride == H * D) || !ez::overlap(q_out, nq, q, span(q_stride, H)),
+             "qk_norm_mrope: q_out must be q (tokens next to each other) or not overlap it");
+  EZ_REQUIRE((k_out == k && k_stride == Hkv * D) || !ez::overlap(k_out, nk, k, span(k_stride, Hkv)),
+             "qk_norm_mrope: k_out must be k (tokens next to each other) or not overlap it");
+  EZ_REQUIRE(!ez::overlap(q_out, nq, k, span(k_stride, Hkv)) && !ez::overlap(q_out, nq, k_out, nk) &&
+                 !ez::overlap(k_out, nk, q, span(q_stride, H)) &&
+                 !(K_cache && (ez::overlap(q_out, nq, v, span(v_stride, Hkv)) || ez::overlap(k_out, nk, v, span(v_stride, Hkv)))),
+             "qk_norm_mrope: an output overlaps another tensor");
   return ez::launch_mrope(a, stream);
 }

@@ -208,7 +208,7 @@ def check_rows(t: torch.Tensor, name: str, shape: tuple, dtype: torch.dtype) -> 
     if t.shape == shape and t.dtype is dtype:
         st = t.stride()
         if st[2] == 1 and st[1] == dim and st[0] >= n:
-            return st[0]
+            return st[0] if shape[0] > 1 else n
     if tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.dtype != dtype:

@@ -61,6 +61,8 @@ class LinearAttnPrefillHipKernel(BaseKernel):
         n = self._ws_bytes.get(max_q_len)
         if n is None:
             n = _hip.size("ezops_linear_attn_prefill_workspace_size", self.B, self.T, self.H, self.Hkv, self.D, max_q_len)
+            if len(self._ws_bytes) >= 1024:
+                self._ws_bytes.clear()
             self._ws_bytes[max_q_len] = n
         # from torch's allocator at every call: stream-ordered, and a captured graph keeps its own
         ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None

@@ -221,6 +221,37 @@ def test_bad_offsets_stay_in_bounds():
             _close(n(out[r]), o, to, b)
 
 
+def test_first_sequence_behind_the_first_row():
+    """Rows in front of the first sequence are of no sequence; one long enough to be cut into segments."""
+    H, Hkv, D, T = 4, 2, 128, 900
+    q, k, v = _inputs(T, H, Hkv, D, 14)
+    for x in (q, k, v):
+        x[:130] = float("nan")
+    S = torch.full((2, Hkv, D, D), float("nan"), device=DEV)
+    out = torch.full((T, H, D), 7.0, dtype=torch.bfloat16, device=DEV)
+    cu = torch.tensor([130, 170, 880], dtype=torch.int32, device=DEV)
+    LinearAttnPrefillOp(2, T, H, Hkv, D, backend="hip", num_slots=2)(q, k, v, _decay(Hkv), cu, S, out=out)
+    assert bool((out[:130] == 7).all()) and bool((out[880:] == 7).all())
+    for b, r in ((0, slice(130, 170)), (1, slice(170, 880))):
+        o, S1, to, ts = _expect(q[r], k[r], v[r], _decay(Hkv), np.zeros((Hkv, D, D)), D ** -0.5)
+        _close(n(out[r]), o, to, b)
+        _close(n(S[b]), S1, ts, b)
+
+
+def test_rows_of_one_token_with_any_stride():
+    """A single row's stride does not matter."""
+    H, Hkv, D = 4, 2, 64
+    x = torch.randn(3, (H + 2 * Hkv) * D + 3, device=DEV).bfloat16()
+    row = x[:1, :(H + 2 * Hkv) * D].unflatten(1, (H + 2 * Hkv, D))
+    q, k, v = row[:, :H], row[:, H:H + Hkv], row[:, H + Hkv:]
+    S = torch.randn(1, Hkv, D, D, device=DEV)
+    want = S.clone()
+    op = LinearAttnDecodeOp(1, H, Hkv, D, 1, backend="hip")
+    a = op(q, k, v, _decay(Hkv), S)
+    b = op(q.contiguous(), k.contiguous(), v.contiguous(), _decay(Hkv), want)
+    assert torch.equal(a, b) and torch.equal(S, want)
+
+
 def test_prefill_on_another_stream_and_in_two_graphs():
     H, Hkv, D, T = 8, 2, 128, 1100
     q, k, v = _inputs(T, H, Hkv, D, 13)

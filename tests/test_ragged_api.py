@@ -118,6 +118,40 @@ def test_prefill_workspace_is_checked_before_any_launch():
         assert b"workspace" in lib.ezops_hip_last_error()
 
 
+def test_c_entries_reject_overlaps():
+    """An output in an input's place, wholly or by an element, where another block may still read it."""
+    lib, err = _hip.lib(), _hip.lib().ezops_hip_last_error
+    at = lambda i: (i + 1) << 24  # noqa: E731  addresses far apart, never touched
+    B, T = 2, 8
+    good = [at(i) for i in range(10)]  # q_lens past table free span | cu kv positions slots span_out
+
+    def plan(p):
+        return lib.ezops_paged_batch_plan(*p, B, T, 64, 4, 16, 16, None)
+
+    for i, j, off in [(6, 1, 0), (6, 0, 4), (5, 0, 4), (9, 4, 0), (9, 4, 4), (7, 3, 60), (2, 0, 4), (8, 1, -60)]:
+        p = list(good)
+        p[i] = p[j] + off
+        assert plan(p) == _hip.EINVAL and (b"overlaps" in err() or b"free_span_out" in err()), (i, j, off, err())
+
+    sec = (ctypes.c_int64 * 1)(32)
+
+    def mrope(q=at(0), qs=256, k=at(1), ks=128, v=at(2), q_out=at(3), k_out=None):
+        return lib.ezops_qk_norm_mrope_bf16(q, qs, k, ks, v, 128, None, None, 1, at(5), at(5), 0, at(6), 1, sec, 0, at(7),
+                                            at(8), at(9), 4, 64, q_out, k_out, 4, 4, 2, 64, 16, 1e-6, None)
+
+    for kw in (dict(q_out=at(0) + 16), dict(q_out=at(0), qs=512), dict(q_out=at(1)), dict(q_out=at(2) + 64),
+               dict(k_out=at(0)), dict(k_out=at(1) - 16), dict(k_out=at(2)), dict(k_out=at(3) + 256),
+               dict(k_out=at(1), ks=256)):
+        assert mrope(**kw) == _hip.EINVAL and b"overlap" in err(), (kw, err())
+    for out in (at(0), at(1) + 128, at(2) - 16):
+        rc = lib.ezops_linear_attn_prefill_bf16(at(0), 256, at(1), 128, at(2), 128, at(3), at(4), None, None, None, 0, out, 1,
+                                                8, 4, 2, 64, 0, 0.0, None, 0, None)
+        assert rc == _hip.EINVAL and b"overlap" in err(), err()
+        rc = lib.ezops_linear_attn_decode_bf16(at(0), 256, at(1), 128, at(2), 128, at(3), at(5), None, 8, out, 2, 4, 2, 64,
+                                               0.0, None)
+        assert rc == _hip.EINVAL and b"overlap" in err(), err()
+
+
 def _np(t):
     return t.detach().double().numpy()
 
