@@ -147,11 +147,17 @@ _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.curre
 
 def call_on(device: torch.device, name: str, *args) -> None:
     """``call`` with the tensors' device as the current one and its stream as the last argument."""
-    if device.index == _current_device():
-        call(name, *args, stream(device))
-    else:
+    index = device.index
+    if index != _current_device():
         with torch.cuda.device(device):
             call(name, *args, stream(device))
+        return
+    of, fns = _entries
+    fn = fns.get(name) if of is not None and of is _lib else None
+    rc = (fn or _fn(name))(*args, _raw_stream(index) if _raw_stream is not None else stream(device))
+    if rc != 0:
+        msg = lib().ezops_hip_last_error().decode(errors="replace")
+        raise RuntimeError(f"{name} failed ({rc}): {msg}")
 
 
 def size(name: str, *args) -> int:
