@@ -10,7 +10,7 @@
 // Over prompts the work is matrix products (a chunk of 64 tokens: 2 x 64 x 128 x (64 + 128) flops a query
 // head and 2 x 64 x 128 x 128 a kv head, in two or three bf16 parts), bound by the matrix cores and the
 // conversions beside them at two waves a SIMD; for single tokens it is the state's traffic.  Measured: 4096 tokens
-// of 32 / 8 heads of 128 50 us (84 MB: 1.7 TB/s), two prompts of 16384 x 32 / 32 411 us (1.08 GB: 2.6 TB/s; read
+// of 32 / 8 heads of 128 50 us (84 MB: 1.7 TB/s), two prompts of 16384 x 32 / 32 408 us (1.08 GB: 2.6 TB/s; read
 // and written once at a copy's rate 219), 200 single tokens x 32 states 168 us (845 MB: 5.0 TB/s).
 //
 // A sequence's state lives in a pool of slots.  A sequence whose slot lies
@@ -190,24 +190,25 @@ __device__ __forceinline__ void wait_vm_barrier() {
   asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"(N) : "memory");
 }
 
-// Twelve 1 KiB fragments in a row (16 bytes a lane).
+// Fragments of 1 KiB in a row (16 bytes a lane): twelve read, four written.
 __device__ __forceinline__ void lds_frags12(uint32_t a, bf16x8_t (&r)[12]) {
   asm volatile(
-      "ds_read_b128 %0, %12\n\tds_read_b128 %1, %12 offset:1024\n\tds_read_b128 %2, %12 offset:2048\n\t"
-      "ds_read_b128 %3, %12 offset:3072\n\tds_read_b128 %4, %12 offset:4096\n\tds_read_b128 %5, %12 offset:5120\n\t"
-      "ds_read_b128 %6, %12 offset:6144\n\tds_read_b128 %7, %12 offset:7168\n\tds_read_b128 %8, %12 offset:8192\n\t"
-      "ds_read_b128 %9, %12 offset:9216\n\tds_read_b128 %10, %12 offset:10240\n\t"
-      "ds_read_b128 %11, %12 offset:11264\n\ts_waitcnt lgkmcnt(0)"
+      "ds_read_b128 %0, %12\n\tds_read_b128 %1, %12 offset:%13\n\tds_read_b128 %2, %12 offset:%14\n\t"
+      "ds_read_b128 %3, %12 offset:%15\n\tds_read_b128 %4, %12 offset:%16\n\tds_read_b128 %5, %12 offset:%17\n\t"
+      "ds_read_b128 %6, %12 offset:%18\n\tds_read_b128 %7, %12 offset:%19\n\tds_read_b128 %8, %12 offset:%20\n\t"
+      "ds_read_b128 %9, %12 offset:%21\n\tds_read_b128 %10, %12 offset:%22\n\tds_read_b128 %11, %12 offset:%23\n\t"
+      "s_waitcnt lgkmcnt(0)"
       : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7]),
         "=&v"(r[8]), "=&v"(r[9]), "=&v"(r[10]), "=&v"(r[11])
-      : "v"(a));
+      : "v"(a), "i"(1 << 10), "i"(2 << 10), "i"(3 << 10), "i"(4 << 10), "i"(5 << 10), "i"(6 << 10), "i"(7 << 10),
+        "i"(8 << 10), "i"(9 << 10), "i"(10 << 10), "i"(11 << 10));
 }
 __device__ __forceinline__ void lds_write_frags4(uint32_t a, const bf16x8_t (&r)[4]) {
   asm volatile(
-      "ds_write_b128 %0, %1\n\tds_write_b128 %0, %2 offset:1024\n\tds_write_b128 %0, %3 offset:2048\n\t"
-      "ds_write_b128 %0, %4 offset:3072\n\ts_waitcnt lgkmcnt(0)"
+      "ds_write_b128 %0, %1\n\tds_write_b128 %0, %2 offset:%5\n\tds_write_b128 %0, %3 offset:%6\n\t"
+      "ds_write_b128 %0, %4 offset:%7\n\ts_waitcnt lgkmcnt(0)"
       :
-      : "v"(a), "v"(r[0]), "v"(r[1]), "v"(r[2]), "v"(r[3])
+      : "v"(a), "v"(r[0]), "v"(r[1]), "v"(r[2]), "v"(r[3]), "i"(1 << 10), "i"(2 << 10), "i"(3 << 10)
       : "memory");
 }
 // Register r: 8 (r / 4) + r % 4 floats below the address + 108.

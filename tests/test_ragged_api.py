@@ -152,6 +152,35 @@ def test_c_entries_reject_overlaps():
         assert rc == _hip.EINVAL and b"overlap" in err(), err()
 
 
+def test_calls_make_the_tensors_device_current(monkeypatch):
+    """``call_on`` with another device current: the call runs inside a switch to the tensors' device, on its stream."""
+    seen, current = [], [1]
+
+    class Switch:
+        def __init__(self, device):
+            self.to = device.index
+
+        def __enter__(self):
+            current[0], self.back = self.to, current[0]
+
+        def __exit__(self, *exc):
+            current[0] = self.back
+
+    monkeypatch.setattr(torch.cuda, "device", Switch)
+    monkeypatch.setattr(_hip, "_current_device", lambda: current[0])
+    monkeypatch.setattr(_hip, "_raw_stream", lambda index: 100 + index)
+    monkeypatch.setattr(_hip, "_entries", (None, {}))
+    monkeypatch.setattr(_hip, "_fn", lambda name: lambda *a: seen.append((name, a, current[0])) or 0)
+    _hip.call_on(torch.device("cuda", 0), "f", 7)
+    _hip.call_on(torch.device("cuda", 1), "g")
+    assert seen == [("f", (7, 100), 0), ("g", (101,), 1)] and current == [1]
+    monkeypatch.setattr(_hip, "_fn", lambda name: lambda *a: -22)
+    for index in (0, 1):
+        with pytest.raises(RuntimeError, match="h failed"):
+            _hip.call_on(torch.device("cuda", index), "h")
+    assert current == [1]
+
+
 def _np(t):
     return t.detach().double().numpy()
 
