@@ -174,6 +174,9 @@ extern "C" int ezops_paged_batch_plan(const int32_t* q_lens, const int32_t* past
     for (const auto& y : out)
       EZ_REQUIRE(!ez::overlap(x.p, x.n, y.p, y.n), "paged_batch_plan: an output overlaps an input (copy the lengths or the "
                  "span of the plan before that is written again)");
+  for (const auto& x : out)
+    for (const auto& y : out)
+      EZ_REQUIRE(&x == &y || !ez::overlap(x.p, x.n, y.p, y.n), "paged_batch_plan: two outputs overlap");
   ez::PlanArgs a{};
   a.q_lens = q_lens; a.past_lens = past_lens;
   a.table = block_table;

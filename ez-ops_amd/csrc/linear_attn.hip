@@ -618,7 +618,7 @@ template <int D>
 __global__ __launch_bounds__(256) void linear_attn_scan_kernel(LinAttnArgs a) {
   EZ_PROF_WAVE(kProfLinAttnState);
   constexpr int PARTS = D * D / 256, AHEAD = 8;
-  const int part = blockIdx.x % PARTS, kvh = blockIdx.x / PARTS % a.Hkv, b = blockIdx.x / PARTS / a.Hkv;
+  const int part = blockIdx.x % PARTS, kvh = blockIdx.x / PARTS, b = blockIdx.y;
   const int T = int(a.T), r0 = min(max(a.cu[b], 0), T), n = min(min(a.cu[b + 1], T) - r0, int(a.max_q));
   if (n <= 0) return;
   const bool cont = a.state && a.past && a.past[b] > 0;
@@ -736,13 +736,19 @@ __global__ __launch_bounds__(256) void linear_attn_decode_kernel(LinAttnArgs a) 
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// out [rows, H, D] must not share memory with q, k or v: other blocks may still have to read them.
+// out [rows, H, D] and the states must not share memory with q, k, v or each other: other blocks may still have to
+// read them.
 int check_out(const LinAttnArgs& a, int64_t rows, int64_t D, const char* what) {
+  const int64_t states = a.num_slots * a.Hkv * D * D * 4;
+  bool states_meet = overlap(a.out, rows * a.H * D * 2, a.state, states);
   auto meets = [&](const uint16_t* x, int64_t rs, int64_t heads) {
-    return overlap(x, ((rows - 1) * rs + heads * D) * 2, a.out, rows * a.H * D * 2);
+    const int64_t n = ((rows - 1) * rs + heads * D) * 2;
+    states_meet |= overlap(x, n, a.state, states);
+    return overlap(x, n, a.out, rows * a.H * D * 2);
   };
   EZ_REQUIRE(!meets(a.q, a.q_rs, a.H) && !meets(a.k, a.k_rs, a.Hkv) && !meets(a.v, a.v_rs, a.Hkv),
              "%s: out must not overlap q, k or v", what);
+  EZ_REQUIRE(!states_meet, "%s: state must not overlap q, k, v or out", what);
   return EZ_OK;
 }
 
@@ -806,7 +812,8 @@ extern "C" int ezops_linear_attn_prefill_bf16(const void* q, int64_t q_stride, c
   const size_t need = ezops_linear_attn_prefill_workspace_size(B, T, H, Hkv, D, max_q_len);
   EZ_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ez::aligned16(workspace)),
              "linear_attn_prefill: needs a 16-byte aligned workspace of %zu bytes", need);
-  EZ_REQUIRE(segments * Hkv < (int64_t(1) << 27) && B * Hkv < (int64_t(1) << 25),
+  // a launch takes fewer than 2^32 threads along an axis; T / seg * Hkv is below 1024 by the rule above
+  EZ_REQUIRE(segments * Hkv < (int64_t(1) << 24),
              "linear_attn_prefill: too many sequences and heads for one launch");
   const int out_rc = ez::check_out(a, T, D, "linear_attn_prefill");
   if (out_rc != EZ_OK) return out_rc;
@@ -814,7 +821,7 @@ extern "C" int ezops_linear_attn_prefill_bf16(const void* q, int64_t q_stride, c
   a.ws = need ? static_cast<float*>(workspace) : nullptr;
   // without a workspace the first block's last state would meet the others' reads of the stored one
   a.split = need || !state || !past_lens ? ez::head_split(segments * Hkv, H / Hkv) : 1;
-  const dim3 grid(unsigned(segments * Hkv)), outs(unsigned(segments * Hkv * a.split)), parts(unsigned(B * Hkv * (D * D / 256)));
+  const dim3 grid(unsigned(segments * Hkv)), outs(unsigned(segments * Hkv * a.split)), parts(unsigned(Hkv * (D * D / 256)), unsigned(B));
   if (D == 64) {
     if (need) {
       hipLaunchKernelGGL((ez::linear_attn_chunk_kernel<64, false>), grid, dim3(128), 0, stream, a);
@@ -848,6 +855,8 @@ extern "C" int ezops_linear_attn_decode_bf16(const void* q, int64_t q_stride, co
   EZ_REQUIRE(state, "linear_attn_decode: null pointer");
   EZ_REQUIRE(B >= 1 && B <= 65536, "linear_attn_decode: batch must be in [1, 65536]");
   EZ_REQUIRE(num_slots >= 1 && num_slots < (int64_t(1) << 31), "linear_attn_decode: num_slots must be in [1, 2^31)");
+  EZ_REQUIRE(B * Hkv < (int64_t(1) << 24),  // a launch takes fewer than 2^32 threads along an axis
+             "linear_attn_decode: too many sequences and heads for one launch");
   a.B = int(B); a.H = int(H); a.Hkv = int(Hkv);
   a.scale = scale > 0.f ? scale : 1.f / sqrtf(float(D));
   const int out_rc = ez::check_out(a, B, D, "linear_attn_decode");

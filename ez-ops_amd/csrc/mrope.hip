@@ -389,5 +389,12 @@ extern "C" int ezops_qk_norm_mrope_bf16(const void* q, int64_t q_stride, const v
                  !ez::overlap(k_out, nk, q, span(q_stride, H)) &&
                  !(K_cache && (ez::overlap(q_out, nq, v, span(v_stride, Hkv)) || ez::overlap(k_out, nk, v, span(v_stride, Hkv)))),
              "qk_norm_mrope: an output overlaps another tensor");
+  const int64_t pool = a.num_slots * Hkv * D * 2;  // 0 without a cache
+  for (const void* c : {K_cache, V_cache})
+    EZ_REQUIRE(!ez::overlap(c, pool, q, span(q_stride, H)) && !ez::overlap(c, pool, k, span(k_stride, Hkv)) &&
+                   !ez::overlap(c, pool, v, span(v_stride, Hkv)) && !ez::overlap(c, pool, q_out, nq) &&
+                   !ez::overlap(c, pool, k_out, nk),
+               "qk_norm_mrope: a cache overlaps another tensor");
+  EZ_REQUIRE(!ez::overlap(K_cache, pool, V_cache, pool), "qk_norm_mrope: K_cache and V_cache overlap");
   return ez::launch_mrope(a, stream);
 }

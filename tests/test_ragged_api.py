@@ -152,6 +152,48 @@ def test_c_entries_reject_overlaps():
         assert rc == _hip.EINVAL and b"overlap" in err(), err()
 
 
+def test_c_entries_reject_overlaps_of_caches_states_and_outputs():
+    lib, err = _hip.lib(), _hip.lib().ezops_hip_last_error
+    at = lambda i: (i + 1) << 24  # noqa: E731  addresses far apart, never touched
+    good = [at(i) for i in range(10)]  # q_lens past table free span | cu kv positions slots span_out
+    for i, j, off in [(5, 6, 0), (6, 5, 8), (7, 8, 60), (9, 5, 8), (2, 7, -124), (8, 2, 124)]:
+        p = list(good)
+        p[i] = p[j] + off
+        rc = lib.ezops_paged_batch_plan(*p, 2, 8, 64, 16, 16, 16, None)
+        assert rc == _hip.EINVAL and b"two outputs overlap" in err(), (i, j, off, err())
+
+    sec = (ctypes.c_int64 * 1)(32)
+    pool = 4 * 2 * 64 * 64 * 2
+    for kc, vc in [(at(0), at(9)), (at(1) - pool + 2, at(9)), (at(8), at(2) + 16), (at(8), at(3)), (at(4) + 64, at(9)),
+                   (at(8), at(8)), (at(8), at(8) + pool - 16)]:
+        rc = lib.ezops_qk_norm_mrope_bf16(at(0), 256, at(1), 128, at(2), 128, None, None, 1, at(5), at(5), 0, at(6), 1, sec,
+                                          0, at(7), kc, vc, 4, 64, at(3), at(4), 4, 4, 2, 64, 16, 1e-6, None)
+        assert rc == _hip.EINVAL and b"overlap" in err(), (kc, vc, err())
+
+    states = 8 * 2 * 64 * 64 * 4
+    for state in (at(0), at(1) + 1024, at(2) - states + 16, at(6)):
+        rc = lib.ezops_linear_attn_prefill_bf16(at(0), 256, at(1), 128, at(2), 128, at(3), at(4), None, state, None, 8, at(6),
+                                                1, 8, 4, 2, 64, 0, 0.0, None, 0, None)
+        assert rc == _hip.EINVAL and b"state must not overlap" in err(), err()
+        rc = lib.ezops_linear_attn_decode_bf16(at(0), 256, at(1), 128, at(2), 128, at(3), state, None, 8, at(6), 8, 4, 2, 64,
+                                               0.0, None)
+        assert rc == _hip.EINVAL and b"state must not overlap" in err(), err()
+
+
+def test_c_entries_reject_launches_past_the_grid():
+    """65536 sequences of 256 heads would take 2^32 threads along one axis."""
+    lib, err = _hip.lib(), _hip.lib().ezops_hip_last_error
+    at = lambda i: (i + 1) << 40  # noqa: E731  addresses far apart, never touched
+    rs = 256 * 64
+    rc = lib.ezops_linear_attn_decode_bf16(at(0), rs, at(1), rs, at(2), rs, at(3), at(5), None, 8, at(6), 65536, 256, 256, 64,
+                                           0.0, None)
+    assert rc == _hip.EINVAL and b"one launch" in err(), err()
+    need = lib.ezops_linear_attn_prefill_workspace_size(65536, 65536, 256, 256, 64, 64)
+    rc = lib.ezops_linear_attn_prefill_bf16(at(0), rs, at(1), rs, at(2), rs, at(3), at(4), None, None, None, 0, at(6), 65536,
+                                            65536, 256, 256, 64, 64, 0.0, at(7), need, None)
+    assert rc == _hip.EINVAL and b"one launch" in err(), err()
+
+
 def test_calls_make_the_tensors_device_current(monkeypatch):
     """``call_on`` with another device current: the call runs inside a switch to the tensors' device, on its stream."""
     seen, current = [], [1]
