@@ -14,7 +14,7 @@
 // The work is memory traffic: q and k in and out, v into the cache, 2 D bytes a
 // head each; the table rows are shared by the heads of a token.  Measured: 16384
 // tokens of 32 + 2 x 8 heads of 128 80 us, 5.1 TB/s (a large copy reaches 4.9); 4097
-// tokens of 16 + 2 x 8 17 us; 16 tokens 5.3 us, a launch and three dependent loads.
+// tokens of 16 + 2 x 8 14.3 us; 16 tokens 5.3 us, a launch and three dependent loads.
 #include "common.h"
 #include "internal.h"
 #include "prof.h"
@@ -178,8 +178,8 @@ __device__ __forceinline__ void store16(uint16_t* p, const uint4& v) {
 // D a multiple of 16 with everything on 16 bytes: a group of LPG lanes (the power of two from D / 16 on)
 // per token and HPT heads (q, then k, then with a cache v, which is only copied), lane l holding pairs
 // 8l..8l+7, so that rotation needs no exchange, the norm one sum over the group, and the table entries
-// (chosen by axis) are read once for all HPT heads.
-template <int LPG, int HPT, bool NT, class TAB>
+// (chosen by axis) are read once for all HPT heads.  LD, ST: heads read, written with the non-temporal hint.
+template <int LPG, int HPT, bool LD, bool ST, class TAB>
 __global__ __launch_bounds__(256) void qk_norm_mrope_vec_kernel(MropeArgs a, uint32_t groups) {
   EZ_PROF_WAVE(kProfQkMrope);
   const int l = threadIdx.x % LPG;
@@ -198,8 +198,8 @@ __global__ __launch_bounds__(256) void qk_norm_mrope_vec_kernel(MropeArgs a, uin
     const uint16_t* src = at + (u < a.H     ? a.q + t * a.q_rs + int64_t(u) * a.D
                                 : u < heads ? a.k + t * a.k_rs + int64_t(u - a.H) * a.D
                                             : a.v + t * a.v_rs + int64_t(u - heads) * a.D);
-    x1[i] = load16<NT>(src);
-    x2[i] = load16<NT>(src + half);
+    x1[i] = load16<LD>(src);
+    x2[i] = load16<LD>(src + half);
   }
   int pos[kMaxAxes];
   bool ok = true;
@@ -275,13 +275,13 @@ __global__ __launch_bounds__(256) void qk_norm_mrope_vec_kernel(MropeArgs a, uin
     if (lane_on && u < units) {
       uint16_t* dst = is_q ? a.q_out + (t * a.H + u) * a.D : a.k_out && u < heads ? a.k_out + (t * a.Hkv + u - a.H) * a.D : nullptr;
       if (dst) {
-        store16<NT>(dst + at, p1);
-        store16<NT>(dst + at + half, p2);
+        store16<ST>(dst + at, p1);
+        store16<ST>(dst + at + half, p2);
       }
       if (!is_q && cached) {
         uint16_t* pool = u < heads ? a.Kc + slot_offset(a, slot, u - a.H) : a.Vc + slot_offset(a, slot, u - heads);
-        store16<NT>(pool + at, p1);
-        store16<NT>(pool + at + half, p2);
+        store16<ST>(pool + at, p1);
+        store16<ST>(pool + at + half, p2);
       }
     }
   }
@@ -295,24 +295,40 @@ bool vec_form(const MropeArgs& a) {
          aligned16(a.Vc) && aligned16(a.q_out) && aligned16(a.k_out) && a.T * (a.H + 2 * a.Hkv) < (int64_t(1) << 31);
 }
 
-template <int LPG, int HPT, bool NT>
+template <int LPG, int HPT, bool LD, bool ST>
 void launch_vec(const MropeArgs& a, hipStream_t s) {
   const uint32_t groups = uint32_t((a.H + (a.Kc ? 2 : 1) * a.Hkv + HPT - 1) / HPT);
   const dim3 grid(unsigned((a.T * groups + 256 / LPG - 1) / (256 / LPG)));
-  if (a.table_f32) hipLaunchKernelGGL((qk_norm_mrope_vec_kernel<LPG, HPT, NT, float>), grid, dim3(256), 0, s, a, groups);
-  else hipLaunchKernelGGL((qk_norm_mrope_vec_kernel<LPG, HPT, NT, uint16_t>), grid, dim3(256), 0, s, a, groups);
+  if (a.table_f32) hipLaunchKernelGGL((qk_norm_mrope_vec_kernel<LPG, HPT, LD, ST, float>), grid, dim3(256), 0, s, a, groups);
+  else hipLaunchKernelGGL((qk_norm_mrope_vec_kernel<LPG, HPT, LD, ST, uint16_t>), grid, dim3(256), 0, s, a, groups);
+}
+
+// The non-temporal hint, by the bytes of the heads read and written.  From 8 MB on where half a head is whole lines
+// of 128 bytes (1024 / 4097 / 16384 tokens of 16 + 2 x 8, 16 + 2 x 8 and 32 + 2 x 8 heads of 128: 9.1 / 21.6 / 92 us
+// without, 7.3 / 16.4 / 80 with it; a copy that reads q_out afterwards included, 11.7 / 27.7 and 11.4 / 25.8; 256
+// tokens with that copy 7.7 and 7.5, 128 tokens 6.9 and 7.4).  Where the halves of a head share lines, never on the
+// loads, which would fetch them twice (20000 tokens of 16 + 16 heads of 80: 61 us without, 70 with it), and on the
+// stores up to the size of the L2s, twice that where the heads are whole lines (3000 tokens 15.1 and 12.8 us, with the
+// copy 19.0 and 17.9, but for 6000 tokens 30.7 and 33.4; 4097 tokens of 32 + 2 x 8 heads of 64 18.2 and 14.6, with it
+// 24.8 and 23.6, for 8192 44.1 and 44.3).
+template <int LPG, int HPT>
+void launch_vec(const MropeArgs& a, int64_t heads, hipStream_t s) {
+  const int64_t bytes = a.T * heads * a.D * 4;
+  if (bytes >= int64_t(8) << 20) {
+    if constexpr (LPG >= 8)  // heads of at least 128
+      if (a.D % 128 == 0) return launch_vec<LPG, HPT, true, true>(a, s);
+    if (a.D % 128 != 0 && bytes < int64_t(a.D % 64 == 0 ? 64 : 32) << 20) return launch_vec<LPG, HPT, false, true>(a, s);
+  }
+  launch_vec<LPG, HPT, false, false>(a, s);
 }
 
 template <int LPG>
 void launch_vec(const MropeArgs& a, hipStream_t s) {
   const int64_t heads = a.H + (a.Kc ? 2 : 1) * a.Hkv;
-  // Four heads a group once that still gives every CU 512 threads (16 + 2 x 8 heads of 128: 1024 tokens take 8.2 us
-  // with one head a group and 9.0 with four, 2048 tokens 12.8 and 11.4), and the non-temporal hint once the heads
-  // read and written pass three quarters of the memory-side cache: 16384 tokens of 32 + 2 x 8 heads (400 MB) take
-  // 80 us with it and 92 without, 9999 tokens of 16 + 16 heads of 80 (102 MB) 31 and 22.
-  if (a.T * heads * LPG < int64_t(8) * 256 * 256) launch_vec<LPG, 1, false>(a, s);
-  else if (a.T * heads * a.D * 4 < int64_t(192) << 20) launch_vec<LPG, 4, false>(a, s);
-  else launch_vec<LPG, 4, true>(a, s);
+  // Four heads a group once that still gives every CU 512 threads (16 + 2 x 8 heads of 128: 1400 tokens take 8.8 us
+  // with one head a group and 10.0 with four, 3000 tokens 15.3 and 13.4).
+  if (a.T * heads * LPG < int64_t(8) * 256 * 256) launch_vec<LPG, 1>(a, heads, s);
+  else launch_vec<LPG, 4>(a, heads, s);
 }
 
 int launch_mrope(const MropeArgs& a, hipStream_t s) {

@@ -111,6 +111,33 @@ def test_against_64_bits(T, H, Hkv, D, sec, inter, norm, page, table, packed):
     assert torch.equal(a[0][live], b[0][live])
 
 
+@pytest.mark.parametrize("T,H,Hkv,D,sec,page,table", [
+    # bytes of the heads read and written: 8, 32 and 64 MB change how they are accessed, T * heads the heads a group
+    (511, 16, 8, 128, (24, 20, 20), 64, torch.bfloat16),    # 7.98 MB
+    (513, 16, 8, 128, (24, 20, 20), 64, torch.bfloat16),    # 8.02 MB
+    (2047, 16, 8, 128, (24, 20, 20), 32, torch.bfloat16),   # one head a group, then four
+    (2051, 15, 5, 128, (64,), None, torch.float32),
+    (1025, 8, 4, 256, (64, 32, 32), 64, torch.bfloat16),
+    (819, 16, 16, 80, (20, 20), None, torch.float32),       # 7.998 MB
+    (821, 16, 16, 80, (20, 20), None, torch.float32),
+    (2049, 16, 16, 80, (20, 20), None, torch.bfloat16),
+    (3277, 16, 16, 80, (20, 20), None, torch.float32),      # 32.002 MB
+    (3001, 32, 8, 64, (16, 8, 8), 64, torch.bfloat16),
+    (5500, 32, 8, 64, (32,), 64, torch.bfloat16),           # 64.5 MB
+    (2741, 16, 16, 48, (8, 8, 8), 32, torch.bfloat16),
+    (901, 16, 4, 144, (24, 24, 24), 32, torch.bfloat16),
+    (1301, 8, 4, 272, (136,), 32, torch.bfloat16),
+])
+def test_large_against_64_bits(T, H, Hkv, D, sec, page, table):
+    pages = -(-T // page) + 1 if page else None
+    op = QkNormMropeOp(T, H, Hkv, D, 211, sec, backend="hip", interleaved=len(sec) > 1, page_size=page, num_pages=pages)
+    d = _data(op, T, True, table)
+    d[7][0, T // 2], d[7][-1, T - 2] = -1, 211
+    q_out = torch.full((T, H, D), 7.0, dtype=torch.bfloat16, device=DEV)
+    k_out = torch.full((T, Hkv, D), 5.0, dtype=torch.bfloat16, device=DEV)
+    _run(op, d, q_out, k_out)
+
+
 def test_unit_weights_and_extremes():
     """No weights = unit; zeros, the largest and the smallest values, infinities and NaN stay in their own head."""
     T, H, Hkv, D = 6, 4, 2, 128
