@@ -11,7 +11,7 @@
 // head and 2 x 64 x 128 x 128 a kv head, in two or three bf16 parts), bound by the matrix cores and the
 // conversions beside them at two waves a SIMD; for single tokens it is the state's traffic.  Measured: 4096 tokens
 // of 32 / 8 heads of 128 50 us (84 MB: 1.7 TB/s), two prompts of 16384 x 32 / 32 406 us (1.08 GB: 2.7 TB/s; read
-// and written once at a copy's rate 219), 200 single tokens x 32 states 168 us (845 MB: 5.0 TB/s).
+// and written once at a copy's rate 219), 200 single tokens x 32 states 153 us (845 MB: 5.5 TB/s).
 //
 // A sequence's state lives in a pool of slots.  A sequence whose slot lies
 // outside the pool, or that an earlier sequence of the batch holds already, is
@@ -686,9 +686,10 @@ int head_split(int64_t blocks, int64_t G) {
 }
 int64_t segment_count(int64_t B, int64_t T, int sh) { return (T >> sh) + B; }
 
-// One token per sequence, bound by the state's traffic, read and written once: block = (sequence, kv head, slice of VC columns of the
-// state), the slice in registers between its one read and its one write.
-template <int D, int VC>
+// One token per sequence, bound by the state's traffic, read and written once: block = (sequence, kv head, slice of VC
+// columns of the state), the slice in registers between its one read and its one write.  NT: both with the
+// non-temporal hint.
+template <int D, int VC, bool NT>
 __global__ __launch_bounds__(256) void linear_attn_decode_kernel(LinAttnArgs a) {
   EZ_PROF_WAVE(kProfLinAttnDecode);
   constexpr int LPR = VC / 4;        // lanes per state row, 4 columns each
@@ -701,10 +702,13 @@ __global__ __launch_bounds__(256) void linear_attn_decode_kernel(LinAttnArgs a) 
   const int sl = blockIdx.x % NS, kvh = blockIdx.x / NS % a.Hkv, b = blockIdx.x / NS / a.Hkv;
   const int slot = slot_of<256>(a, b);
   if (slot < 0) return;
-  float4* st = reinterpret_cast<float4*>(a.state + (int64_t(slot) * a.Hkv + kvh) * D * D + sl * VC) + c;
-  float4 S[NI];
+  f32x4_t* st = reinterpret_cast<f32x4_t*>(a.state + (int64_t(slot) * a.Hkv + kvh) * D * D + sl * VC) + c;
+  f32x4_t S[NI];
 #pragma unroll
-  for (int i = 0; i < NI; ++i) S[i] = st[(r0 + i * RPI) * (D / 4)];
+  for (int i = 0; i < NI; ++i) {
+    if constexpr (NT) S[i] = __builtin_nontemporal_load(st + (r0 + i * RPI) * (D / 4));
+    else S[i] = st[(r0 + i * RPI) * (D / 4)];
+  }
   const Keep keep = keep_over(a.log_decay[kvh], 1.f);
   for (int i = tid; i < D; i += 256) ks[i] = bf2f(a.k[b * a.k_rs + kvh * D + i]);
   for (int i = tid; i < G * D; i += 256) qs[i / D][i % D] = bf2f(a.q[b * a.q_rs + kvh * G * D + i]) * a.scale;
@@ -718,7 +722,8 @@ __global__ __launch_bounds__(256) void linear_attn_decode_kernel(LinAttnArgs a) 
     S[i].y = decayed(keep, S[i].y, kk * v.y);
     S[i].z = decayed(keep, S[i].z, kk * v.z);
     S[i].w = decayed(keep, S[i].w, kk * v.w);
-    st[(r0 + i * RPI) * (D / 4)] = S[i];
+    if constexpr (NT) __builtin_nontemporal_store(S[i], st + (r0 + i * RPI) * (D / 4));
+    else st[(r0 + i * RPI) * (D / 4)] = S[i];
   }
   for (int g = 0; g < G; ++g) {
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -869,7 +874,17 @@ extern "C" int ezops_linear_attn_decode_bf16(const void* q, int64_t q_stride, co
   const int out_rc = ez::check_out(a, B, D, "linear_attn_decode");
   if (out_rc != EZ_OK) return out_rc;
   const dim3 grid(unsigned(B * Hkv));
-  if (D == 64) hipLaunchKernelGGL((ez::linear_attn_decode_kernel<64, 64>), grid, dim3(256), 0, stream, a);
-  else hipLaunchKernelGGL((ez::linear_attn_decode_kernel<128, 128>), grid, dim3(256), 0, stream, a);
+  // With the hint from 4 MB of states on: a step comes back to them after all other layers, from outside the caches
+  // (32 heads of 128, 2 / 8 / 32 / 128 / 400 MB: 4.8 / 7.4 / 17.3 / 53.8 / 169 us without, 5.1 / 5.8 / 12.7 / 51.1 / 155
+  // with it).  Only a layer alone, whose states the memory-side cache holds from step to step, is faster without it
+  // (128 MB 41 and 49 us, but 32 MB 10.6 and 9.9).
+  const bool nt = B * Hkv * D * D * 4 >= int64_t(4) << 20;
+  if (D == 64) {
+    if (nt) hipLaunchKernelGGL((ez::linear_attn_decode_kernel<64, 64, true>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((ez::linear_attn_decode_kernel<64, 64, false>), grid, dim3(256), 0, stream, a);
+  } else {
+    if (nt) hipLaunchKernelGGL((ez::linear_attn_decode_kernel<128, 128, true>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((ez::linear_attn_decode_kernel<128, 128, false>), grid, dim3(256), 0, stream, a);
+  }
   return ez::launch_status("linear_attn_decode");
 }
