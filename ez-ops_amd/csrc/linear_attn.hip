@@ -10,7 +10,7 @@
 // Over prompts the work is matrix products (a chunk of 64 tokens: 2 x 64 x 128 x (64 + 128) flops a query
 // head and 2 x 64 x 128 x 128 a kv head, in two or three bf16 parts), bound by the matrix cores and the
 // conversions beside them at two waves a SIMD; for single tokens it is the state's traffic.  Measured: 4096 tokens
-// of 32 / 8 heads of 128 50 us (84 MB: 1.7 TB/s), two prompts of 16384 x 32 / 32 406 us (1.08 GB: 2.7 TB/s; read
+// of 32 / 8 heads of 128 47 us (84 MB: 1.8 TB/s), two prompts of 16384 x 32 / 32 406 us (1.08 GB: 2.7 TB/s; read
 // and written once at a copy's rate 219), 200 single tokens x 32 states 153 us (845 MB: 5.5 TB/s).
 //
 // A sequence's state lives in a pool of slots.  A sequence whose slot lies
@@ -330,8 +330,12 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
   __shared__ __align__(1024) uint16_t Ks[2][kC * D], Vs[OUT ? 1 : 2][kC * D], Qs[OUT ? kC * D : 8];
   __shared__ __align__(1024) uint16_t Ps[OUT ? 3 * 4 * 512 : 8];  // block of P x (16-key step, part) x lane x 8
   __shared__ float pw[96];
-  const int split = OUT ? a.split : 1, part = blockIdx.x % split;
-  const int kvh = blockIdx.x / split % a.Hkv, id = blockIdx.x / split / a.Hkv;
+  // The blocks that share a kv head's K, V and state are 8 apart: on one XCD, whose L2 then reads them once, and the
+  // one that has summed the segment (4096 tokens of 32 / 8 heads 49.3 -> 47.0 us, 1024 30.6 -> 28.1).
+  const int split = OUT ? a.split : 1, units = a.segments * a.Hkv;
+  const int u0 = int(blockIdx.x) / (8 * split) * 8, within = int(blockIdx.x) - u0 * split, wide = min(8, units - u0);
+  const int part = within / wide, unit = u0 + within - part * wide;
+  const int kvh = unit % a.Hkv, id = unit / a.Hkv;
   Segment sg;
   if (!find_segment<THREADS>(a, id, sg)) return;
   if (!OUT && sg.s == sg.count - 1) return;
