@@ -173,6 +173,12 @@ def test_long_sequences(H, Hkv, D, lens):
     _prefill(lens, past, H, Hkv, D, seed=5, max_q_len=0)
 
 
+@pytest.mark.parametrize("H,Hkv,D,lens", [(32, 2, 128, [701, 1, 340]), (16, 16, 128, [130, 2000]), (32, 4, 64, [1500, 3, 650])])
+def test_many_segments(H, Hkv, D, lens):
+    """Many segments and heads: short first chunks, states taken on, rows behind the last sequence."""
+    _prefill(lens, [4 * (i % 2) for i in range(len(lens))], H, Hkv, D, seed=31, pad=7)
+
+
 @pytest.mark.parametrize("D", [64, 128])
 def test_more_sequences_than_threads(D):
     """Sequences are found by a block of 128 or 256 threads: 300 short ones, some empty, some continued, a slot twice."""
