@@ -10,7 +10,7 @@
 // Over prompts the work is matrix products (a chunk of 64 tokens: 2 x 64 x 128 x (64 + 128) flops a query
 // head and 2 x 64 x 128 x 128 a kv head, in two or three bf16 parts), bound by the matrix cores and the
 // conversions beside them at two waves a SIMD; for single tokens it is the state's traffic.  Measured: 4096 tokens
-// of 32 / 8 heads of 128 47 us (84 MB: 1.8 TB/s), two prompts of 16384 x 32 / 32 406 us (1.08 GB: 2.7 TB/s; read
+// of 32 / 8 heads of 128 47 us (84 MB: 1.8 TB/s), two prompts of 16384 x 32 / 32 397 us (1.08 GB: 2.7 TB/s; read
 // and written once at a copy's rate 219), 200 single tokens x 32 states 153 us (845 MB: 5.5 TB/s).
 //
 // A sequence's state lives in a pool of slots.  A sequence whose slot lies
@@ -674,10 +674,10 @@ __global__ __launch_bounds__(256) void linear_attn_scan_kernel(LinAttnArgs a) {
 }
 
 // log2 of the tokens per segment: the longest segments that still give about 512 blocks over the whole
-// batch, two a CU (32 / 8 heads, all three kernels: 16384 tokens 125 us, with 256 blocks 136); two chunks
-// as soon as that gives one block a CU (4096 tokens: 54 us, with 512 blocks of a chunk 57: each segment costs
-// 256 KiB of state traffic a kv head); at least a chunk.  Two chunks of one or two query heads a kv head are not
-// cut at all (128 tokens of 8 / 8 heads 13.9 us, cut 18.4).
+// batch, two a CU (2 x 16384 tokens of 32 / 32 heads, all three kernels: 401 us, with 256 blocks 525); two chunks
+// as soon as that gives one block a CU (4096 tokens of 32 / 8: 45.1 us, with 512 blocks of a chunk 50.5: each segment
+// costs 256 KiB of state traffic a kv head); at least a chunk.  Two chunks of one or two query heads a kv head are not
+// cut at all (128 tokens of 8 / 8 heads 12.9 us, cut 16.9).
 int segment_shift(int64_t T, int64_t G, int64_t Hkv, int64_t max_q) {
   int sh = 6;
   while ((T * Hkv) >> (sh + 1) >= (sh < 7 ? 256 : 512)) ++sh;
@@ -685,7 +685,7 @@ int segment_shift(int64_t T, int64_t G, int64_t Hkv, int64_t max_q) {
 }
 // Blocks a kv head's query heads are shared out to where the segments alone leave CUs without work (up to
 // about two a CU); each of them updates the state for itself, and the first leaves it.  64 tokens of
-// 32 / 8 heads: 9.6 us, in one block a kv head 16.4; 1024 tokens of 32 / 8: outputs 17.7, with 272 blocks 16.2.
+// 32 / 8 heads: 9.0 us, in one block a kv head 15.2; 4096 tokens 45.4, with 1056 blocks 53.3.
 int head_split(int64_t blocks, int64_t G) {
   int64_t n = 1;
   while (2 * n <= G && blocks * 2 * n <= 576) n *= 2;
