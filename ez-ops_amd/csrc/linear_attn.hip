@@ -21,6 +21,7 @@
 #include "common.h"
 #include "internal.h"
 #include "prof.h"
+#include "segments.h"
 #include "status.h"
 #include "../../include/ezops_hip.h"
 
@@ -271,15 +272,15 @@ __device__ __forceinline__ bool find_segment(const LinAttnArgs& a, int id, Segme
   const int T = int(a.T);
   // every thread looks at its sequences with all of their entries at once: one memory latency, not three
   int count = 0;  // sequences whose first segment number is at most id: the last of them is ours
-  int begin = 0, end = 0, slot = -1, past = 0;
+  int begin = 0, len = 0, slot = -1, past = 0;
   for (int c0 = 0; c0 < a.B; c0 += THREADS) {
     const int c = c0 + threadIdx.x;
     bool in = false;
     if (c < a.B) {
-      const int r = min(max(a.cu[c], 0), T), e = min(a.cu[c + 1], T);
+      const SeqRows r = seq_rows(a.cu[c], a.cu[c + 1], T, int(a.max_q));
       const int sl = a.state ? (a.state_slots ? a.state_slots[c] : c) : -1, p = a.past ? a.past[c] : 0;
-      in = (r >> a.seg_sh) + c <= id;
-      if (in) begin = r, end = e, slot = sl, past = p;
+      in = (r.first >> a.seg_sh) + c <= id;
+      if (in) begin = r.first, len = r.count, slot = sl, past = p;
     }
     count += __syncthreads_count(in);
   }
@@ -288,14 +289,14 @@ __device__ __forceinline__ bool find_segment(const LinAttnArgs& a, int id, Segme
   if (int(threadIdx.x) == b % THREADS) {
     // offsets that do not decrease: this thread's last sequence with a number at most id is b
     s_seq[0] = begin;
-    s_seq[1] = end;
+    s_seq[1] = len;
     s_seq[2] = slot;
     s_seq[3] = past;
   }
   __syncthreads();
   // out of LDS into scalar registers: every thread has the same
   const int r0 = __builtin_amdgcn_readfirstlane(s_seq[0]);
-  const int n = min(__builtin_amdgcn_readfirstlane(s_seq[1]) - r0, int(a.max_q));
+  const int n = __builtin_amdgcn_readfirstlane(s_seq[1]);
   slot = __builtin_amdgcn_readfirstlane(s_seq[2]);
   past = __builtin_amdgcn_readfirstlane(s_seq[3]);
   if (a.state) {
@@ -633,7 +634,8 @@ __global__ __launch_bounds__(256) void linear_attn_scan_kernel(LinAttnArgs a) {
   EZ_PROF_WAVE(kProfLinAttnState);
   constexpr int PARTS = D * D / 256, AHEAD = 8;
   const int kvh = blockIdx.x % a.Hkv, part = blockIdx.x / a.Hkv, b = blockIdx.y;
-  const int T = int(a.T), r0 = min(max(a.cu[b], 0), T), n = min(min(a.cu[b + 1], T) - r0, int(a.max_q));
+  const SeqRows rows = seq_rows(a.cu[b], a.cu[b + 1], int(a.T), int(a.max_q));
+  const int r0 = rows.first, n = rows.count;
   if (n <= 0) return;
   const bool cont = a.state && a.past && a.past[b] > 0;
   if (n <= a.seg && !cont) return;

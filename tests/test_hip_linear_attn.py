@@ -402,3 +402,29 @@ def test_argument_checks():
                  (q, k, v, _decay(Hkv), S8, torch.zeros(8, dtype=torch.int64, device=DEV))):
         with pytest.raises(ValueError):
             dec(*args)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("mq", [0, 400])
+def test_bad_offsets_of_long_sequences_stay_in_bounds(D, mq):
+    """Ends far below zero, and offsets that decrease, in calls whose sequences are cut into segments (with a workspace):
+    the good sequence gets its result, the bad one nothing, and the rows and states around the tensors stay as they were."""
+    H, Hkv, T, guard = 2, 2, 1100, 1200
+    qg, kg, vg = _inputs(T + guard, H, Hkv, D, 40)
+    for x in (qg, kg, vg):
+        x[T:] = float("nan")
+    q, k, v = qg[:T], kg[:T], vg[:T]
+    i32, lo = dict(dtype=torch.int32, device=DEV), -(1 << 31)
+    op = LinearAttnPrefillOp(2, T, H, Hkv, D, backend="hip", num_slots=2)
+    for end in (-1, lo, lo + 40, lo + 701, 3):
+        pool = torch.full((4, Hkv, D, D), 7.0, device=DEV)
+        rows = torch.full((T + guard, H, D), 7.0, dtype=torch.bfloat16, device=DEV)
+        S, out = pool[1:3], rows[:T]
+        S[0] = torch.randn(Hkv, D, D, generator=torch.Generator().manual_seed(3)).to(DEV)
+        first = n(S[0])
+        op(q, k, v, _decay(Hkv), torch.tensor([0, 700, end], **i32), S, None, torch.tensor([5, 9], **i32), max_q_len=mq, out=out)
+        m = mq or 700
+        o, S1, to, ts = _expect(q[:m], k[:m], v[:m], _decay(Hkv), first, D ** -0.5)
+        _close(n(out[:m]), o, to, end)
+        _close(n(S[0]), S1, ts, end)
+        assert bool((rows[m:] == 7).all()) and bool((pool[[0, 2, 3]] == 7).all()), end
