@@ -42,7 +42,9 @@ struct LinAttnArgs {
   int seg, seg_sh;            // prefill: tokens per segment (1 << seg_sh)
   int segments;               // prefill: segment numbers
   int split;                  // prefill: blocks that share the query heads of a kv head
-  float* ws;                  // prefill: [segments, Hkv, D, D] or NULL (one segment a sequence)
+  float* ws;                  // prefill: [ws_slots, Hkv, D, D] or NULL (one segment a sequence)
+  int ws_slots;
+  bool ws_rows, ws_all;       // prefill: slots by row, not by segment number; uncut sequences have one too
   int B, H, Hkv;
   float scale;
 };
@@ -91,10 +93,13 @@ __device__ __forceinline__ int slot_of(const LinAttnArgs& a, int b) {
 // first chunk of its first segment can be short, and it is filled up with zero
 // tokens at its front, which leaves every power below the same for all chunks.
 //
-// With one segment a sequence the output kernel alone runs (state from the pool,
-// state to the pool).  Otherwise: the state kernel sums every segment but the last
+// A sequence of one segment goes through the output kernel alone (state from the pool,
+// state to the pool).  Of the others the state kernel sums every segment but the last
 // from zero into the workspace, the scan turns these sums into the state before
-// each segment, and the output kernel starts each segment from there.
+// each segment, and the output kernel starts each segment from there.  Only where the
+// query heads of a kv head are shared out to several blocks (few blocks in all) does an
+// uncut sequence start from a copy of its state in the workspace as well: the block that
+// leaves the last state must not meet the others' reads of the first.
 //
 // Matrix layout (v_mfma_f32_32x32x16_bf16: lane 32h+i holds A[i][8h..8h+7] and
 // B[8h..8h+7][i]; register r of lane 32h+j holds C[8(r/4)+4h+r%4][j]).  Wave w owns
@@ -261,6 +266,7 @@ struct Segment {
   int b, s, count;     // sequence, index in it, its number of segments
   int slot;            // state slot (-1: no pool)
   bool cont;           // the sequence starts from its stored state
+  int ws;              // workspace slot of the state before the segment (-1: none)
   int row;             // first row of the segment
   int len;             // tokens
 };
@@ -314,6 +320,7 @@ __device__ __forceinline__ bool find_segment(const LinAttnArgs& a, int id, Segme
   g.count = cnt;
   g.slot = slot;
   g.cont = a.state && past > 0;
+  g.ws = a.ws && (cnt > 1 || a.ws_all) ? ws_first(r0, b, a.seg_sh, a.ws_rows) + s : -1;
   g.row = r0 + (s ? first + ((s - 1) << a.seg_sh) : 0);
   g.len = s ? a.seg : first;
   return true;
@@ -354,9 +361,9 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
     for (int r = 0; r < 16; ++r) S[t][r] = 0.f;
   const int elem = 8 * h * D + 32 * w + j;
   float* pool = sg.slot >= 0 ? a.state + (int64_t(sg.slot) * a.Hkv + kvh) * D * D : nullptr;
-  float* ws = a.ws + (int64_t(id) * a.Hkv + kvh) * D * D;
+  float* ws = a.ws + (int64_t(max(sg.ws, 0)) * a.Hkv + kvh) * D * D;
   if (OUT && (sg.s > 0 || sg.cont)) {
-    const float* src = a.ws ? ws : pool;
+    const float* src = sg.ws >= 0 ? ws : pool;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -410,7 +417,7 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
   const uint32_t pwrd = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const float*)(&pw[0]))) +
                         uint32_t(4 * (31 + j - 4 * h - 27));
   const int G = a.H / a.Hkv / split, h0 = kvh * (a.H / a.Hkv) + part * G;  // this block's query heads
-  float* dst = OUT ? (sg.s == sg.count - 1 && part == 0 ? pool : nullptr) : id + 1 < a.segments ? ws + int64_t(a.Hkv) * D * D : nullptr;
+  float* dst = OUT ? (sg.s == sg.count - 1 && part == 0 ? pool : nullptr) : sg.ws + 1 < a.ws_slots ? ws + int64_t(a.Hkv) * D * D : nullptr;
   const Keep keep_first = uniform(keep_over(g, float(kC - pad))), keep_full = uniform(keep_over(g, float(kC)));
   // One 32 x 32 block of P (0: first keys and queries, 1: first keys, second queries, 2: second keys and
   // queries), weighted, in two parts: the operand of the product with V, four fragments.
@@ -623,7 +630,8 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
 
 // The workspace's slot of segment s > 0 holds the sum of segment s - 1; becomes the state
 // before segment s.  Slot 0 gets the stored state where the sequence continues (the output
-// kernel overwrites the pool while blocks that start from there may still have to read it).
+// kernel overwrites the pool while blocks that start from there may still have to read it);
+// uncut sequences that no two blocks share have no slot and no part in this.
 // Block = (sequence, kv head, 256 elements), one element a thread: the chain over the segments is
 // short of work per step, so the chip is filled with threads, each eight loads ahead of its sums.
 // With Hkv a multiple of 8 a kv head is on one XCD in all three kernels (workgroups go round the XCDs in turn), and
@@ -638,14 +646,14 @@ __global__ __launch_bounds__(256) void linear_attn_scan_kernel(LinAttnArgs a) {
   const int r0 = rows.first, n = rows.count;
   if (n <= 0) return;
   const bool cont = a.state && a.past && a.past[b] > 0;
-  if (n <= a.seg && !cont) return;
+  if (n <= a.seg && !(cont && a.ws_all)) return;
   int slot = -1;
   if (a.state) {
     slot = slot_of<256>(a, b);
     if (slot < 0) return;
   }
-  const int cnt = (n + a.seg - 1) >> a.seg_sh, id = (r0 >> a.seg_sh) + b;
-  const int last = min(cnt, a.segments - id);  // decreasing offsets must not lead past the workspace
+  const int cnt = (n + a.seg - 1) >> a.seg_sh, id = ws_first(r0, b, a.seg_sh, a.ws_rows);
+  const int last = min(cnt, a.ws_slots - id);  // decreasing offsets must not lead past the workspace
   const int at = part * 256 + int(threadIdx.x);
   const int64_t step = int64_t(a.Hkv) * D * D;
   float* ws = a.ws + (int64_t(id) * a.Hkv + kvh) * D * D + at;
@@ -694,6 +702,27 @@ int head_split(int64_t blocks, int64_t G) {
   return int(n);
 }
 int64_t segment_count(int64_t B, int64_t T, int sh) { return (T >> sh) + B; }
+
+// How a call is cut up: segments, blocks a kv head's query heads are shared out to, workspace slots (0: no workspace).
+// Without a workspace the heads of continued states stay in one block.
+struct Cut {
+  int sh, split;
+  int64_t segments, slots;
+  bool by_row;
+};
+Cut cut_up(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t max_q, bool continued) {
+  Cut c{};
+  c.sh = segment_shift(T, H / Hkv, Hkv, max_q);
+  c.segments = segment_count(B, T, c.sh);
+  const bool need = max_q > int64_t(1) << c.sh;
+  c.split = need || !continued ? head_split(c.segments * Hkv, H / Hkv) : 1;
+  if (need) {
+    // shared out heads: a slot for every sequence, at most 288 states of a kv head then (head_split)
+    c.by_row = c.split == 1 && ws_by_row(c.segments, T, c.sh);
+    c.slots = c.split == 1 ? ws_slots(c.segments, T, c.sh) : c.segments;
+  }
+  return c;
+}
 
 // One token per sequence, bound by the state's traffic, read and written once: block = (sequence, kv head, slice of VC
 // columns of the state), the slice in registers between its one read and its one write.  NT: both with the
@@ -794,9 +823,7 @@ extern "C" size_t ezops_linear_attn_prefill_workspace_size(int64_t B, int64_t T,
                                                            int64_t max_q_len) {
   if (B < 1 || T < 1 || Hkv < 1 || D < 1) return 0;
   const int64_t max_q = max_q_len > 0 && max_q_len < T ? max_q_len : T;
-  const int sh = ez::segment_shift(T, H / Hkv, Hkv, max_q);
-  if (max_q <= int64_t(1) << sh) return 0;
-  return size_t(ez::segment_count(B, T, sh)) * Hkv * D * D * sizeof(float);
+  return size_t(ez::cut_up(B, T, H, Hkv, max_q, true).slots) * Hkv * D * D * sizeof(float);
 }
 
 extern "C" int ezops_linear_attn_prefill_bf16(const void* q, int64_t q_stride, const void* k, int64_t k_stride,
@@ -827,10 +854,11 @@ extern "C" int ezops_linear_attn_prefill_bf16(const void* q, int64_t q_stride, c
   a.scale = scale > 0.f ? scale : 1.f / sqrtf(float(D));
   EZ_REQUIRE(q_stride < (1 << 23) && k_stride < (1 << 23) && v_stride < (1 << 23),
              "linear_attn_prefill: token strides must be below 2^23");
-  a.seg_sh = ez::segment_shift(T, H / Hkv, Hkv, a.max_q);
+  const ez::Cut cut = ez::cut_up(B, T, H, Hkv, a.max_q, state && past_lens);
+  a.seg_sh = cut.sh;
   a.seg = 1 << a.seg_sh;
-  const int64_t segments = ez::segment_count(B, T, a.seg_sh);
-  const size_t need = ezops_linear_attn_prefill_workspace_size(B, T, H, Hkv, D, max_q_len);
+  const int64_t segments = cut.segments;
+  const size_t need = size_t(cut.slots) * Hkv * D * D * sizeof(float);
   EZ_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ez::aligned16(workspace)),
              "linear_attn_prefill: needs a 16-byte aligned workspace of %zu bytes", need);
   // a launch takes fewer than 2^32 threads along an axis; T / seg * Hkv is below 1024 by the rule above
@@ -840,8 +868,10 @@ extern "C" int ezops_linear_attn_prefill_bf16(const void* q, int64_t q_stride, c
   if (out_rc != EZ_OK) return out_rc;
   a.segments = int(segments);
   a.ws = need ? static_cast<float*>(workspace) : nullptr;
-  // without a workspace the first block's last state would meet the others' reads of the stored one
-  a.split = need || !state || !past_lens ? ez::head_split(segments * Hkv, H / Hkv) : 1;
+  a.ws_slots = int(cut.slots);
+  a.ws_rows = cut.by_row;
+  a.ws_all = cut.split > 1;
+  a.split = cut.split;
   const dim3 grid(unsigned(segments * Hkv)), outs(unsigned(segments * Hkv * a.split)), parts(unsigned(Hkv * (D * D / 256)), unsigned(B));
   if (D == 64) {
     if (need) {

@@ -428,3 +428,36 @@ def test_bad_offsets_of_long_sequences_stay_in_bounds(D, mq):
         _close(n(out[:m]), o, to, end)
         _close(n(S[0]), S1, ts, end)
         assert bool((rows[m:] == 7).all()) and bool((pool[[0, 2, 3]] == 7).all()), end
+
+
+@pytest.mark.parametrize("H,Hkv,D,lens", [
+    (16, 16, 64, [1] * 30 + [700] + [1] * 20 + [0, 64, 65, 1, 300]),     # more slots by number than by row
+    (32, 8, 64, [1] * 45 + [200, 1, 64, 0, 130]),                         # heads in groups, one block a kv head
+    (2, 2, 128, [1100, 1, 64, 900, 3]),                                   # few sequences
+    (8, 2, 128, [300, 1, 64, 70, 1]),                                     # heads shared out: copies of all states
+])
+def test_mixed_steps(H, Hkv, D, lens):
+    """Chunks of long prompts beside single tokens and idle rows, all continued or every other one: what is not cut into
+    segments goes from its state to its state."""
+    B = len(lens)
+    order = np.random.RandomState(B).permutation(B + 2)[:B].tolist()
+    for past in ([3] * B, [i % 2 for i in range(B)]):
+        for mq in (None, 0):
+            _prefill(lens, past, H, Hkv, D, slots=order, seed=41, pad=6, max_q_len=mq)
+
+
+def test_workspace_of_a_mixed_step():
+    """2048 tokens of one prompt beside 256 single tokens, 32 states of 128 x 128 each: a call takes less than 128 MiB."""
+    B, T, H, D = 257, 2304, 32, 128
+    q, k, v = _inputs(T, H, H, D, 5)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    S = torch.zeros(B, H, D, D, device=DEV)
+    cu, past = torch.tensor([0, *range(2048, T + 1)], **i32), torch.ones(B, **i32)
+    op = LinearAttnPrefillOp(B, T, H, H, D, backend="hip", num_slots=B)
+    out = torch.empty(T, H, D, dtype=torch.bfloat16, device=DEV)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    op(q, k, v, _decay(H), cu, S, None, past, max_q_len=2048, out=out)
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() - before < 128 << 20
