@@ -461,3 +461,29 @@ def test_workspace_of_a_mixed_step():
     op(q, k, v, _decay(H), cu, S, None, past, max_q_len=2048, out=out)
     torch.cuda.synchronize()
     assert torch.cuda.max_memory_allocated() - before < 128 << 20
+
+
+@pytest.mark.parametrize("H,D", [(8, 128), (16, 64)])
+def test_shared_query_heads_that_continue(H, D):
+    """One kv head's query heads in several blocks (more than a segment of tokens, few blocks), all of which start from
+    the stored state that one of them replaces: 65 tokens are the fewest."""
+    for lens in ([65], [66, 0, 64, 1], [130]):
+        _prefill(lens, [3] * len(lens), H, 1, D, seed=51)
+        _prefill(lens, [3 * (i % 2) for i in range(len(lens))], H, 1, D, seed=52, max_q_len=0)
+
+
+@pytest.mark.parametrize("H,D", [(8, 128), (16, 128), (8, 64), (16, 64)])
+def test_shared_query_heads_of_one_segment(H, D):
+    """The same without a workspace, which is where past_lens is None: every block starts from zero, one leaves the state;
+    and without states."""
+    T = 64
+    q, k, v = _inputs(T, H, 1, D, 53)
+    cu, g = torch.tensor([0, 40, T], dtype=torch.int32, device=DEV), _decay(1)
+    for slots in (None, torch.tensor([2, 0], dtype=torch.int32, device=DEV)):
+        S = torch.full((3, 1, D, D), float("nan"), device=DEV)
+        out = LinearAttnPrefillOp(2, T, H, 1, D, backend="hip", num_slots=3)(q, k, v, g, cu, S, slots, max_q_len=T)
+        for b, r in ((0, slice(0, 40)), (1, slice(40, T))):
+            o, S1, to, ts = _expect(q[r], k[r], v[r], g, np.zeros((1, D, D)), D ** -0.5)
+            _close(n(out[r]), o, to, b)
+            _close(n(S[b if slots is None else int(slots[b])]), S1, ts, b)
+    _prefill([40, 24], [0, 0], H, 1, D, state=False, seed=54, max_q_len=T)
