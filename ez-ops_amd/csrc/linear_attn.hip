@@ -14,7 +14,7 @@
 // and written once at a copy's rate 219), 200 single tokens x 32 states 153 us (845 MB: 5.5 TB/s).
 //
 // A sequence's state lives in a pool of slots.  A sequence whose slot lies
-// outside the pool, or that an earlier sequence of the batch holds already, is
+// outside the pool, or that an earlier sequence with tokens holds already, is
 // left out whole: nothing of it is read or written, so equal slots make no race.
 #include <type_traits>
 
@@ -71,6 +71,12 @@ __device__ __forceinline__ float decayed(const Keep& k, float S, float x) {
   return k.near ? S + y : y;
 }
 
+// Whether sequence c keeps `slot` from those behind it: only with tokens, of which a single token's call has one
+// for every sequence (an idle row of a padded prompt batch may carry any slot).
+__device__ __forceinline__ bool holds(const LinAttnArgs& a, int c, int slot) {
+  return a.state_slots[c] == slot && (!a.cu || seq_rows(a.cu[c], a.cu[c + 1], int(a.T), int(a.max_q)).count > 0);
+}
+
 // Slot of sequence b, -1 if it has none: outside the pool, or held by an earlier
 // sequence.  Every thread of the block calls it (barrier inside).
 template <int THREADS>
@@ -78,7 +84,7 @@ __device__ __forceinline__ int slot_of(const LinAttnArgs& a, int b) {
   const int s = a.state_slots ? a.state_slots[b] : b;
   int dup = 0;
   if (a.state_slots) {
-    for (int c = threadIdx.x; c < b; c += THREADS) dup |= a.state_slots[c] == s;
+    for (int c = threadIdx.x; c < b; c += THREADS) dup |= holds(a, c, s);
     dup = __syncthreads_or(dup);
   }
   return s < 0 || s >= a.num_slots || dup ? -1 : s;
@@ -308,7 +314,7 @@ __device__ __forceinline__ bool find_segment(const LinAttnArgs& a, int id, Segme
   if (a.state) {
     int dup = slot < 0 || slot >= a.num_slots;
     if (a.state_slots)
-      for (int c = threadIdx.x; c < b; c += THREADS) dup |= a.state_slots[c] == slot;
+      for (int c = threadIdx.x; c < b; c += THREADS) dup |= holds(a, c, slot);
     if (__syncthreads_or(dup)) return false;
   }
   const int s = id - ((r0 >> a.seg_sh) + b);

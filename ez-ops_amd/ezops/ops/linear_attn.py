@@ -12,8 +12,8 @@ and query head ``h`` reads the state of kv head ``h // (H / Hkv)``.  States live
 a pool ``state [num_slots, Hkv, D, D]``; sequence ``b`` owns slot
 ``state_slots[b]`` (None: slot ``b``), updated in place.  A sequence whose slot is
 outside the pool (-1: a padded row of the batch), or that an earlier sequence of
-the batch holds already, is left out whole: its rows of ``out`` and every state
-stay as they were.  In a prompt a token whose k or v is not finite leaves its own
+the batch with tokens holds already, is left out whole: its rows of ``out`` and
+every state stay as they were.  In a prompt a token whose k or v is not finite leaves its own
 sequence's outputs undefined from the first token of its 64-token chunk on; other
 sequences are not touched.
 """
@@ -27,10 +27,15 @@ from .utils.roofline import RooflineResult
 GROUPS = (1, 2, 4, 8, 16)
 
 
-def usable_slots(state_slots, batch: int, num_slots: int) -> list[int]:
-    """The slot of every sequence, -1 where it has none (outside the pool, or held by an earlier sequence)."""
-    slots = list(range(batch)) if state_slots is None else state_slots.tolist()
-    return [s if 0 <= s < num_slots and s not in slots[:b] else -1 for b, s in enumerate(slots)]
+def usable_slots(state_slots, lens: list[int], num_slots: int) -> list[int]:
+    """The slot of every sequence, -1 where it has none (outside the pool, or held by an earlier sequence with tokens)."""
+    slots = list(range(len(lens))) if state_slots is None else state_slots.tolist()
+    held, out = set(), []
+    for s, n in zip(slots, lens):
+        out.append(s if 0 <= s < num_slots and s not in held else -1)
+        if n > 0:
+            held.add(s)
+    return out
 
 
 def _check_heads(num_heads, num_kv_heads, head_dim):
@@ -118,11 +123,12 @@ class LinearAttnPrefillOp(Op):
         B, T, H, Hkv, D = self.batch, self.num_tokens, self.num_heads, self.num_kv_heads, self.head_dim
         out = torch.empty(T, H, D, dtype=q.dtype, device=q.device) if out is None else out
         lam = torch.exp(log_decay.float())[:, None, None]
-        slots = usable_slots(state_slots, B, self.num_slots) if state is not None else [-1] * B
         cu = [min(max(0, x), T) for x in cu_seqlens.tolist()]
+        lens = [min(e - s, max_q_len or T) for s, e in zip(cu, cu[1:])]
+        slots = usable_slots(state_slots, lens, self.num_slots) if state is not None else [-1] * B
         past = past_lens.tolist() if past_lens is not None else [0] * B
         for b in range(B):
-            n = min(cu[b + 1] - cu[b], max_q_len or T)
+            n = lens[b]
             if n <= 0 or (state is not None and slots[b] < 0):
                 continue
             keep = state is not None and past[b] > 0
@@ -193,7 +199,7 @@ class LinearAttnDecodeOp(Op):
         B, H, Hkv, D = self.batch, self.num_heads, self.num_kv_heads, self.head_dim
         out = torch.empty(B, H, D, dtype=q.dtype, device=q.device) if out is None else out
         lam = torch.exp(log_decay.float())[:, None, None]
-        for b, s in enumerate(usable_slots(state_slots, B, self.num_slots)):
+        for b, s in enumerate(usable_slots(state_slots, [1] * B, self.num_slots)):
             if s < 0:
                 continue
             S = lam * state[s] + k[b].float()[:, :, None] * v[b].float()[:, None, :]

@@ -257,8 +257,8 @@ int ezops_qk_norm_mrope_bf16(const void* q, int64_t q_stride, const void* k, int
  * state_slots[b] (NULL = slot b) if past_lens[b] > 0 (past_lens NULL = 0 for all),
  * starts from zero otherwise, and leaves its last state there; a sequence without
  * tokens leaves it alone.  A sequence whose slot is outside the pool, or that an
- * earlier sequence of the batch holds already, is left out whole (no row of out and
- * no state is written); rows of no sequence are not written.  log_decay [Hkv] fp32,
+ * earlier sequence of the batch with tokens holds already, is left out whole (no row
+ * of out and no state is written); rows of no sequence are not written.  log_decay [Hkv] fp32,
  * at most 0 (-inf: no memory).  H / Hkv in {1, 2, 4, 8, 16}, D in {64, 128}; q, k, v,
  * out, state and workspace 16-byte aligned; B <= 65536, T < 2^30; scale <= 0 selects
  * 1/sqrt(D).  The workspace (ezops_linear_attn_prefill_workspace_size bytes, 0 for

@@ -487,3 +487,29 @@ def test_shared_query_heads_of_one_segment(H, D):
             _close(n(out[r]), o, to, b)
             _close(n(S[b if slots is None else int(slots[b])]), S1, ts, b)
     _prefill([40, 24], [0, 0], H, 1, D, state=False, seed=54, max_q_len=T)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("mq", [0, 200, 64])
+def test_idle_rows_hold_no_slot(D, mq):
+    """Sequences without tokens that carry the slot of a later one (a default of 0) do not silence it; those with tokens
+    still keep a later one out.  With segments and without."""
+    H, Hkv = 4, 2
+    lens, slots, past = [0, 65, 0, 40, 200, 3, 0, 5], [0, 0, 1, 1, 2, 2, 3, 3], [2, 1, 0, 0, 4, 4, 9, 9]
+    T, B = sum(lens), len(lens)
+    cu = np.concatenate([[0], np.cumsum(lens)])
+    i32 = dict(dtype=torch.int32, device=DEV)
+    q, k, v = _inputs(T, H, Hkv, D, 61)
+    S = torch.randn(4, Hkv, D, D, generator=torch.Generator().manual_seed(6)).to(DEV)
+    before, out = S.clone(), torch.full((T, H, D), 7.0, dtype=torch.bfloat16, device=DEV)
+    LinearAttnPrefillOp(B, T, H, Hkv, D, backend="hip", num_slots=4)(
+        q, k, v, _decay(Hkv), torch.tensor(cu, **i32), S, torch.tensor(slots, **i32), torch.tensor(past, **i32), max_q_len=mq,
+        out=out)
+    for b in (1, 3, 4, 7):
+        m = min(lens[b], mq) if mq else lens[b]
+        r = slice(int(cu[b]), int(cu[b]) + m)
+        S0 = n(before[slots[b]]) if past[b] else np.zeros((Hkv, D, D))
+        o, S1, to, ts = _expect(q[r], k[r], v[r], _decay(Hkv), S0, D ** -0.5)
+        _close(n(out[r]), o, to, b)
+        _close(n(S[slots[b]]), S1, ts, b)
+    assert bool((out[cu[5]:cu[6]] == 7).all())

@@ -337,3 +337,22 @@ def test_rooflines():
     assert LinearAttnDecodeOp(3, 4, 2, 64, 8).get_roofline().bytes == 3 * (8 * 2 * 64 * 64 + 4 * 6 * 64 + 4)
     assert PagedBatchPlanOp(3, 10, 64, 4, 8).get_roofline().flops == 0
     assert LinearAttnPrefillOp(1, 10, 4, 2, 64).get_roofline().flops == 10 * (6 + 8) * 64 * 64
+
+
+def test_ref_idle_rows_hold_no_slot():
+    """Sequences without tokens that carry the slot of a later one (a default of 0) do not silence it."""
+    torch.manual_seed(4)
+    H, Hkv, D = 2, 1, 64
+    op = LinearAttnPrefillOp(5, 9, H, Hkv, D, num_slots=2)
+    q, k, v, g, _, state = op.gen_data("cpu")
+    i32 = dict(dtype=torch.int32)
+    cu, slots, past = torch.tensor([0, 0, 4, 4, 7, 9], **i32), torch.tensor([0, 0, 1, 1, 0], **i32), torch.tensor([3, 2, 0, 0, 1], **i32)
+    first = state.clone()
+    out = torch.full((9, H, D), 7.0, dtype=torch.bfloat16)
+    op(q, k, v, g, cu, state, slots, past, out=out)
+    lam = np.exp(_np(g))
+    for b, r, S0 in ((1, slice(0, 4), _np(first[0])), (3, slice(4, 7), np.zeros((Hkv, D, D)))):
+        want, S = ragged.linear_attn(_np(q[r]), _np(k[r]), _np(v[r]), lam, S0, D ** -0.5)
+        np.testing.assert_allclose(_np(out[r]), want, rtol=2 ** -8, atol=1e-4)
+        np.testing.assert_allclose(_np(state[slots[b]]), S, rtol=1e-5, atol=1e-5)
+    assert bool((out[7:] == 7).all())  # the last one's slot is held by one with tokens
