@@ -16,6 +16,7 @@
 // A sequence's state lives in a pool of slots.  A sequence whose slot lies
 // outside the pool, or that an earlier sequence with tokens holds already, is
 // left out whole: nothing of it is read or written, so equal slots make no race.
+#include <cmath>
 #include <type_traits>
 
 #include "common.h"
@@ -808,13 +809,14 @@ int check_out(const LinAttnArgs& a, int64_t rows, int64_t D, const char* what) {
   return EZ_OK;
 }
 
-int check_common(const LinAttnArgs& a, int64_t H, int64_t Hkv, int64_t D, const char* what) {
+int check_common(const LinAttnArgs& a, int64_t H, int64_t Hkv, int64_t D, float scale, const char* what) {
   EZ_REQUIRE(a.q && a.k && a.v && a.log_decay && a.out, "%s: null pointer", what);
   EZ_REQUIRE(Hkv >= 1 && H >= 1 && H <= 4096 && H % Hkv == 0, "%s: num_heads must be divisible by num_kv_heads", what);
   const int64_t G = H / Hkv;
   EZ_REQUIRE(G == 1 || G == 2 || G == 4 || G == 8 || G == 16, "%s: group size %d not supported (1, 2, 4, 8 or 16)", what,
              int(G));
   EZ_REQUIRE(D == 64 || D == 128, "%s: head_dim must be 64 or 128", what);
+  EZ_REQUIRE(std::isfinite(scale), "%s: scale must be finite", what);
   EZ_REQUIRE(a.q_rs >= H * D && a.k_rs >= Hkv * D && a.v_rs >= Hkv * D, "%s: token strides below the heads' size", what);
   EZ_REQUIRE(a.q_rs % 8 == 0 && a.k_rs % 8 == 0 && a.v_rs % 8 == 0 && aligned16(a.q) && aligned16(a.k) &&
                  aligned16(a.v) && aligned16(a.out) && aligned16(a.state),
@@ -848,7 +850,7 @@ extern "C" int ezops_linear_attn_prefill_bf16(const void* q, int64_t q_stride, c
   a.out = static_cast<uint16_t*>(out);
   a.T = T; a.num_slots = num_slots;
   a.max_q = max_q_len > 0 && max_q_len < T ? max_q_len : T;
-  const int rc = ez::check_common(a, H, Hkv, D, "linear_attn_prefill");
+  const int rc = ez::check_common(a, H, Hkv, D, scale, "linear_attn_prefill");
   if (rc != EZ_OK) return rc;
   EZ_REQUIRE(cu_seqlens, "linear_attn_prefill: null pointer");
   EZ_REQUIRE(B >= 1 && B <= 65536 && T >= 1 && T < (int64_t(1) << 30),
@@ -907,7 +909,7 @@ extern "C" int ezops_linear_attn_decode_bf16(const void* q, int64_t q_stride, co
   a.state = state; a.state_slots = state_slots;
   a.out = static_cast<uint16_t*>(out);
   a.num_slots = num_slots;
-  const int rc = ez::check_common(a, H, Hkv, D, "linear_attn_decode");
+  const int rc = ez::check_common(a, H, Hkv, D, scale, "linear_attn_decode");
   if (rc != EZ_OK) return rc;
   EZ_REQUIRE(state, "linear_attn_decode: null pointer");
   EZ_REQUIRE(B >= 1 && B <= 65536, "linear_attn_decode: batch must be in [1, 65536]");

@@ -18,6 +18,8 @@ sequence's outputs undefined from the first token of its 64-token chunk on; othe
 sequences are not touched.
 """
 
+import ctypes
+
 import torch
 
 from ..registry import get_kernel
@@ -50,8 +52,8 @@ def _check_heads(num_heads, num_kv_heads, head_dim):
 def _scale(scale, head_dim):
     if scale is None:
         return head_dim ** -0.5
-    if not 0 < scale < float("inf"):
-        raise ValueError(f"scale ({scale}) must be positive")
+    if not 0 < ctypes.c_float(scale).value < float("inf"):
+        raise ValueError(f"scale ({scale}) must be positive and in the range of fp32")
     return float(scale)
 
 

@@ -261,7 +261,7 @@ int ezops_qk_norm_mrope_bf16(const void* q, int64_t q_stride, const void* k, int
  * of out and no state is written); rows of no sequence are not written.  log_decay [Hkv] fp32,
  * at most 0 (-inf: no memory).  H / Hkv in {1, 2, 4, 8, 16}, D in {64, 128}; q, k, v,
  * out, state and workspace 16-byte aligned; B <= 65536, T < 2^30; scale <= 0 selects
- * 1/sqrt(D).  The workspace (ezops_linear_attn_prefill_workspace_size bytes, 0 for
+ * 1/sqrt(D), one that is not finite is rejected.  The workspace (ezops_linear_attn_prefill_workspace_size bytes, 0 for
  * some shapes, never above 2048 states of a kv head: it does not grow with the
  * sequences that are short) need not be zero-filled.  A token whose k or v is not finite leaves its
  * own sequence's outputs undefined from the first token of its 64-token chunk on

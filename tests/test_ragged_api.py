@@ -356,3 +356,21 @@ def test_ref_idle_rows_hold_no_slot():
         np.testing.assert_allclose(_np(out[r]), want, rtol=2 ** -8, atol=1e-4)
         np.testing.assert_allclose(_np(state[slots[b]]), S, rtol=1e-5, atol=1e-5)
     assert bool((out[7:] == 7).all())  # the last one's slot is held by one with tokens
+
+
+def test_scales_that_fp32_does_not_hold_are_refused():
+    """The kernels take the scale in fp32, where 0 selects the default: one that rounds to 0 or to infinity is no scale."""
+    for scale in (1e-50, 1e39, float("inf"), -1.0):
+        for args in ((LinearAttnPrefillOp, 1, 8, 4, 2, 64), (LinearAttnDecodeOp, 1, 4, 2, 64, 3)):
+            for backend in ("ref", "hip"):
+                with pytest.raises(ValueError, match="scale"):
+                    args[0](*args[1:], backend=backend, scale=scale)
+    lib, err = _hip.lib(), _hip.lib().ezops_hip_last_error
+    at = lambda i: (i + 1) << 24  # noqa: E731  addresses far apart, never touched
+    for scale in (float("nan"), float("inf")):
+        rc = lib.ezops_linear_attn_prefill_bf16(at(0), 256, at(1), 128, at(2), 128, at(3), at(4), None, None, None, 0, at(6), 1,
+                                                8, 4, 2, 64, 0, scale, None, 0, None)
+        assert rc == _hip.EINVAL and b"scale" in err(), err()
+        rc = lib.ezops_linear_attn_decode_bf16(at(0), 256, at(1), 128, at(2), 128, at(3), at(5), None, 8, at(6), 2, 4, 2, 64,
+                                               scale, None)
+        assert rc == _hip.EINVAL and b"scale" in err(), err()
