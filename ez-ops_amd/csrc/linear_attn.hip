@@ -793,10 +793,10 @@ __global__ __launch_bounds__(256) void linear_attn_decode_kernel(LinAttnArgs a) 
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// out [rows, H, D] and the states must not share memory with q, k, v or each other: other blocks may still have to
-// read them.
+// out [rows, H, D], the states and the workspace must not share memory with an input or each other: other blocks may
+// still have to read them.
 int check_out(const LinAttnArgs& a, int64_t rows, int64_t D, const char* what) {
-  const int64_t states = a.num_slots * a.Hkv * D * D * 4;
+  const int64_t states = a.num_slots * a.Hkv * D * D * 4, ws = int64_t(a.ws_slots) * a.Hkv * D * D * 4;
   bool states_meet = overlap(a.out, rows * a.H * D * 2, a.state, states);
   auto meets = [&](const uint16_t* x, int64_t rs, int64_t heads) {
     const int64_t n = ((rows - 1) * rs + heads * D) * 2;
@@ -806,6 +806,15 @@ int check_out(const LinAttnArgs& a, int64_t rows, int64_t D, const char* what) {
   EZ_REQUIRE(!meets(a.q, a.q_rs, a.H) && !meets(a.k, a.k_rs, a.Hkv) && !meets(a.v, a.v_rs, a.Hkv),
              "%s: out must not overlap q, k or v", what);
   EZ_REQUIRE(!states_meet, "%s: state must not overlap q, k, v or out", what);
+  const struct { const void* p; int64_t n; } in[] = {{a.log_decay, a.Hkv * 4}, {a.state_slots, a.B * int64_t(4)},
+      {a.cu, (a.B + 1) * int64_t(4)}, {a.past, a.B * int64_t(4)}, {a.q, ((rows - 1) * a.q_rs + a.H * D) * 2},
+      {a.k, ((rows - 1) * a.k_rs + a.Hkv * D) * 2}, {a.v, ((rows - 1) * a.v_rs + a.Hkv * D) * 2}};
+  for (const auto& x : in)
+    EZ_REQUIRE(!overlap(x.p, x.n, a.out, rows * a.H * D * 2) && !overlap(x.p, x.n, a.state, states) &&
+                   !overlap(x.p, x.n, a.ws, ws),
+               "%s: out, state or workspace overlaps an input", what);
+  EZ_REQUIRE(!overlap(a.ws, ws, a.out, rows * a.H * D * 2) && !overlap(a.ws, ws, a.state, states),
+             "%s: the workspace overlaps out or state", what);
   return EZ_OK;
 }
 
@@ -872,11 +881,11 @@ extern "C" int ezops_linear_attn_prefill_bf16(const void* q, int64_t q_stride, c
   // a launch takes fewer than 2^32 threads along an axis; T / seg * Hkv is below 1024 by the rule above
   EZ_REQUIRE(segments * Hkv < (int64_t(1) << 24),
              "linear_attn_prefill: too many sequences and heads for one launch");
-  const int out_rc = ez::check_out(a, T, D, "linear_attn_prefill");
-  if (out_rc != EZ_OK) return out_rc;
   a.segments = int(segments);
   a.ws = need ? static_cast<float*>(workspace) : nullptr;
   a.ws_slots = int(cut.slots);
+  const int out_rc = ez::check_out(a, T, D, "linear_attn_prefill");
+  if (out_rc != EZ_OK) return out_rc;
   a.ws_rows = cut.by_row;
   a.ws_all = cut.split > 1;
   a.split = cut.split;

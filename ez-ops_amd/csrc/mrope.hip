@@ -412,5 +412,12 @@ extern "C" int ezops_qk_norm_mrope_bf16(const void* q, int64_t q_stride, const v
                    !ez::overlap(c, pool, k_out, nk),
                "qk_norm_mrope: a cache overlaps another tensor");
   EZ_REQUIRE(!ez::overlap(K_cache, pool, V_cache, pool), "qk_norm_mrope: K_cache and V_cache overlap");
+  const int64_t table = S * D * (table_f32 ? 4 : 2);
+  const struct { const void* p; int64_t n; } small[] = {{cos, table}, {sin, table}, {positions, axes * T * 4},
+      {K_cache ? slot_mapping : nullptr, T * 8}, {norm ? q_norm_w : nullptr, D * 2}, {norm ? k_norm_w : nullptr, D * 2}};
+  for (const auto& x : small)
+    EZ_REQUIRE(!ez::overlap(x.p, x.n, q_out, nq) && !ez::overlap(x.p, x.n, k_out, nk) &&
+                   !ez::overlap(x.p, x.n, K_cache, pool) && !ez::overlap(x.p, x.n, V_cache, pool),
+               "qk_norm_mrope: an output overlaps a table, the positions, the slots or a weight");
   return ez::launch_mrope(a, stream);
 }

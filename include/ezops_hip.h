@@ -233,9 +233,9 @@ int ezops_paged_batch_plan(const int32_t* q_lens, const int32_t* past_lens, int3
  * caches [num_pages, Hkv, page_size, D], with v to slot slot_mapping[t] =
  * page * page_size + offset; slots outside the pool are skipped, and two tokens
  * must not share one.  A token with a position outside [0, S) on any axis writes
- * nothing.  q_out may be q (q_stride = H * D), k_out k; other overlaps, of the caches too, are rejected.
- * D even, at most 512;
- * page_size a power of two in [32, 2^20].
+ * nothing.  q_out may be q (q_stride = H * D), k_out k; other overlaps of an output or a
+ * cache with any tensor are rejected.  D even, at most 512; page_size a power of two in
+ * [32, 2^20].
  * No counterpart in the reference, which turns one token per sequence by one
  * position (ezops/ops/fused_qk_norm_rope.py:7-169). */
 int ezops_qk_norm_mrope_bf16(const void* q, int64_t q_stride, const void* k, int64_t k_stride,
@@ -265,8 +265,8 @@ int ezops_qk_norm_mrope_bf16(const void* q, int64_t q_stride, const void* k, int
  * some shapes, never above 2048 states of a kv head: it does not grow with the
  * sequences that are short) need not be zero-filled.  A token whose k or v is not finite leaves its
  * own sequence's outputs undefined from the first token of its 64-token chunk on
- * (chunks end at the sequence's end); other sequences are not touched.  out must not
- * overlap q, k or v, nor state any of them; B * Hkv < 2^24 - 1024 (EZOPS_EINVAL).
+ * (chunks end at the sequence's end); other sequences are not touched.  out,
+ * state and workspace must not overlap an input or each other; B * Hkv < 2^24 - 1024 (EZOPS_EINVAL).
  * No counterpart in the reference (softmax attention only,
  * ezops/ops/attn_decode.py:9-67). */
 size_t ezops_linear_attn_prefill_workspace_size(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t D,
@@ -281,7 +281,7 @@ int ezops_linear_attn_prefill_bf16(const void* q, int64_t q_stride, const void* 
 
 /* The recurrent form: one token per sequence, q [B, H, D], k / v [B, Hkv, D] (row
  * strides in elements, multiples of 8), the state required and updated in place,
- * slots as above.  out [B, H, D] bf16; out and state must not overlap q, k, v or each
+ * slots as above.  out [B, H, D] bf16; out and state must not overlap an input or each
  * other.  B * Hkv < 2^24.
  * No counterpart in the reference (softmax attention only,
  * ezops/ops/attn_decode.py:9-67). */

@@ -374,3 +374,53 @@ def test_scales_that_fp32_does_not_hold_are_refused():
         rc = lib.ezops_linear_attn_decode_bf16(at(0), 256, at(1), 128, at(2), 128, at(3), at(5), None, 8, at(6), 2, 4, 2, 64,
                                                scale, None)
         assert rc == _hip.EINVAL and b"scale" in err(), err()
+
+
+def test_c_entries_reject_outputs_over_small_inputs():
+    """Tables, positions, slots, weights, offsets and decays are read by blocks that run after others have written."""
+    lib, err = _hip.lib(), _hip.lib().ezops_hip_last_error
+    at = lambda i: (i + 1) << 24  # noqa: E731  addresses far apart, never touched
+    sec = (ctypes.c_int64 * 2)(20, 12)
+    T, H, Hkv, D, S = 4, 4, 2, 64, 16
+    pool = 4 * 2 * 64 * 64 * 2
+    good = dict(qw=at(10), kw=at(11), cos=at(5), sin=at(12), pos=at(6), slots=at(7), K=at(8), V=at(9), q_out=at(3), k_out=at(4))
+
+    def mrope(f32=0, **kw):
+        a = {**good, **kw}
+        return lib.ezops_qk_norm_mrope_bf16(at(0), 256, at(1), 128, at(2), 128, a["qw"], a["kw"], 1, a["cos"], a["sin"], f32,
+                                            a["pos"], 2, sec, 0, a["slots"], a["K"], a["V"], 4, 64, a["q_out"], a["k_out"], T,
+                                            H, Hkv, D, S, 1e-6, None)
+
+    size = dict(qw=2 * D, kw=2 * D, cos=2 * S * D, sin=2 * S * D, pos=2 * 4 * T, slots=8 * T)
+    for out, n in (("q_out", T * H * D * 2), ("k_out", T * Hkv * D * 2), ("K", pool), ("V", pool)):
+        for x, m in size.items():
+            for off in (0, m - 2, 2 - n):  # its start, its last element, the output's last element on its first
+                assert mrope(**{out: good[x] + off}) == _hip.EINVAL and b"overlap" in err(), (out, x, off, err())
+    assert mrope(f32=1, q_out=at(5) + 4 * S * D - 4) == _hip.EINVAL and b"overlap" in err(), err()
+
+    B, T, states = 2, 200, 8 * 2 * 64 * 64 * 4
+    need = lib.ezops_linear_attn_prefill_workspace_size(B, T, 4, 2, 64, 0)
+    assert need > 0
+    rows = dict(g=4 * 2, cu=4 * (B + 1), past=4 * B, slots=4 * B)
+    base = dict(g=at(3), cu=at(4), past=at(5), slots=at(6), state=at(7), out=at(9), ws=at(10))
+
+    def prefill(**kw):
+        a = {**base, **kw}
+        return lib.ezops_linear_attn_prefill_bf16(at(0), 256, at(1), 128, at(2), 128, a["g"], a["cu"], a["past"], a["state"],
+                                                  a["slots"], 8, a["out"], B, T, 4, 2, 64, 0, 0.0, a["ws"], need, None)
+
+    def decode(**kw):
+        a = {**base, **kw}
+        return lib.ezops_linear_attn_decode_bf16(at(0), 256, at(1), 128, at(2), 128, a["g"], a["state"], a["slots"], 8,
+                                                 a["out"], B, 4, 2, 64, 0.0, None)
+
+    for x, m in rows.items():
+        for out, n in (("out", T * 4 * 64 * 2), ("state", states), ("ws", need)):
+            for addr in (base[x] & ~15, base[x] - n + 16):
+                assert prefill(**{out: addr}) == _hip.EINVAL and b"overlap" in err(), (out, x, err())
+        if x in ("g", "slots"):
+            for out in ("out", "state"):
+                assert decode(**{out: base[x]}) == _hip.EINVAL and b"overlap" in err(), (out, x, err())
+    for x, n in ((at(0), 256 * 2 * T), (at(1), 128 * 2 * T), (at(2), 128 * 2 * T), (at(7), states), (at(9), 4 * 64 * 2 * T)):
+        for addr in (x, x + n - 16, x - need + 16):
+            assert prefill(ws=addr) == _hip.EINVAL and b"overlap" in err(), (x, err())
