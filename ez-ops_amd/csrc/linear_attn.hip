@@ -241,7 +241,8 @@ __device__ __forceinline__ bf16x8_t join(const i32x2_t& x, const i32x2_t& y) {
   return as_bf16x8(make_uint4(uint32_t(x[0]), uint32_t(x[1]), uint32_t(y[0]), uint32_t(y[1])));
 }
 
-// The next bf16 part of eight values: returned rounded, and taken off them.
+// The next bf16 part of eight values: returned rounded, and taken off them.  Values that round to infinity (from 2^128
+// (1 - 2^-9) on) leave NaN: the range that the entry documents ends below them.
 __device__ __forceinline__ bf16x8_t take_part(float (&x)[8]) {
   uint32_t w[4];
 #pragma unroll

@@ -15,7 +15,9 @@ outside the pool (-1: a padded row of the batch), or that an earlier sequence of
 the batch with tokens holds already, is left out whole: its rows of ``out`` and
 every state stay as they were.  In a prompt a token whose k or v is not finite leaves its own
 sequence's outputs undefined from the first token of its 64-token chunk on; other
-sequences are not touched.
+sequences are not touched.  States and the products ``q . k`` of a prompt have to stay
+below 2^127: past that a query's own outputs are undefined (a product), or the own
+sequence's outputs from there on (a state), also where the recurrence gives an infinity.
 """
 
 import ctypes

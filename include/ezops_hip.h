@@ -265,7 +265,10 @@ int ezops_qk_norm_mrope_bf16(const void* q, int64_t q_stride, const void* k, int
  * some shapes, never above 2048 states of a kv head: it does not grow with the
  * sequences that are short) need not be zero-filled.  A token whose k or v is not finite leaves its
  * own sequence's outputs undefined from the first token of its 64-token chunk on
- * (chunks end at the sequence's end); other sequences are not touched.  out,
+ * (chunks end at the sequence's end); other sequences are not touched.  States and
+ * products q . k have to stay below 2^127: past that a query's own outputs (a product)
+ * or its sequence's from there on (a state) are undefined, also where the recurrence
+ * gives an infinity.  out,
  * state and workspace must not overlap an input or each other; B * Hkv < 2^24 - 1024 (EZOPS_EINVAL).
  * No counterpart in the reference (softmax attention only,
  * ezops/ops/attn_decode.py:9-67). */

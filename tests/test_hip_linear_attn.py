@@ -513,3 +513,40 @@ def test_idle_rows_hold_no_slot(D, mq):
         _close(n(out[r]), o, to, b)
         _close(n(S[slots[b]]), S1, ts, b)
     assert bool((out[cu[5]:cu[6]] == 7).all())
+
+
+@pytest.mark.parametrize("H,D", [(4, 128), (2, 64)])
+def test_overflow_stays_in_its_query_and_sequence(H, D):
+    """Finite inputs whose products leave the range (states and powers enter the products in bf16 parts, whose remainder
+    of an infinity is NaN): a query that overflows with its keys leaves other queries and the states alone, a state past
+    the range other sequences; states of up to 2^126 give the recurrence's outputs."""
+    Hkv, lens = 2, [70, 40, 30]
+    T, g, i32 = sum(lens), _decay(Hkv), dict(dtype=torch.int32, device=DEV)
+    q, k, v = _inputs(T, H, Hkv, D, 71, packed=False)
+    q[20], q[75] = 3e38, -3e38  # with keys of the size of 1: past 2^128
+    cu, past = [0, 70, 110, 140], torch.tensor([1, 0, 2], **i32)
+    S = torch.randn(3, Hkv, D, D, generator=torch.Generator().manual_seed(7)).to(DEV)
+    S[2, 1] = 3.4e38  # rounds to infinity in bf16
+    before = S.clone()
+    out = LinearAttnPrefillOp(3, T, H, Hkv, D, backend="hip", num_slots=3)(q, k, v, g, torch.tensor(cu, **i32), S, None, past)
+    for b, bad in ((0, 20), (1, 5)):
+        r = slice(cu[b], cu[b + 1])
+        x = q[r].clone()
+        x[bad] = 0
+        o, S1, to, ts = _expect(x, k[r], v[r], g, n(before[b]) if b == 0 else np.zeros((Hkv, D, D)), D ** -0.5)
+        keep = np.arange(lens[b]) != bad
+        _close(n(out[r])[keep], o[keep], to[keep], b)
+        _close(n(S[b]), S1, ts, b)
+    r, G = slice(110, 140), H // Hkv  # the head whose state is in range
+    o, S1, to, ts = _expect(q[r, :G], k[r, :1], v[r, :1], g[:1], n(before[2, :1]), D ** -0.5)
+    _close(n(out[r, :G]), o, to, 2)
+    _close(n(S[2, :1]), S1, ts, 2)
+    # large, but in range
+    S = torch.randn(1, Hkv, D, D, generator=torch.Generator().manual_seed(8)).clamp(-4, 4).to(DEV) * 2.0 ** 124
+    x, first = q[:64] * 2.0 ** -20, n(S[0])
+    x[20] = 0
+    out = LinearAttnPrefillOp(1, 64, H, Hkv, D, backend="hip", num_slots=1)(x, k[:64], v[:64], g, torch.tensor([0, 64], **i32), S,
+                                                                        None, past[:1])
+    o, S1, to, ts = _expect(x, k[:64], v[:64], g, first, D ** -0.5)
+    _close(n(out), o, to, "large")
+    _close(n(S[0]), S1, ts, "large")
