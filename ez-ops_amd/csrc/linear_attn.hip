@@ -271,7 +271,7 @@ __device__ __forceinline__ float power(float g2, int n) { return n == 0 ? 1.f : 
 // Segment numbers: sequence b's segments are numbers cu[b] / seg + b, + 1, ...: distinct
 // for distinct sequences, and at most T / seg + B in all, so the host knows the grid.
 struct Segment {
-  int b, s, count;     // sequence, index in it, its number of segments
+  int s, count;        // index in its sequence, the sequence's number of segments
   int slot;            // state slot (-1: no pool)
   bool cont;           // the sequence starts from its stored state
   int ws;              // workspace slot of the state before the segment (-1: none)
@@ -323,7 +323,6 @@ __device__ __forceinline__ bool find_segment(const LinAttnArgs& a, int id, Segme
   if (n <= 0 || s < 0 || s >= (n + a.seg - 1) >> a.seg_sh) return false;
   const int cnt = (n + a.seg - 1) >> a.seg_sh;
   const int first = n - ((cnt - 1) << a.seg_sh);  // 1 .. seg
-  g.b = b;
   g.s = s;
   g.count = cnt;
   g.slot = slot;
@@ -732,23 +731,21 @@ Cut cut_up(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t max_q, bool con
   return c;
 }
 
-// One token per sequence, bound by the state's traffic, read and written once: block = (sequence, kv head, slice of VC
-// columns of the state), the slice in registers between its one read and its one write.  NT: both with the
-// non-temporal hint.
-template <int D, int VC, bool NT>
+// One token per sequence, bound by the state's traffic, read and written once: block = (sequence, kv head), the state
+// in registers between its one read and its one write.  NT: both with the non-temporal hint.
+template <int D, bool NT>
 __global__ __launch_bounds__(256) void linear_attn_decode_kernel(LinAttnArgs a) {
   EZ_PROF_WAVE(kProfLinAttnDecode);
-  constexpr int LPR = VC / 4;        // lanes per state row, 4 columns each
+  constexpr int LPR = D / 4;         // lanes per state row, 4 columns each
   constexpr int RPI = 256 / LPR;     // rows per step of the block
   constexpr int NI = D / RPI;        // rows per thread
-  constexpr int NS = D / VC;
   __shared__ float ks[D], qs[16][D];
   __shared__ float4 red[RPI][LPR];
   const int tid = threadIdx.x, c = tid % LPR, r0 = tid / LPR, G = a.H / a.Hkv;
-  const int sl = blockIdx.x % NS, kvh = blockIdx.x / NS % a.Hkv, b = blockIdx.x / NS / a.Hkv;
+  const int kvh = blockIdx.x % a.Hkv, b = blockIdx.x / a.Hkv;
   const int slot = slot_of<256>(a, b);
   if (slot < 0) return;
-  f32x4_t* st = reinterpret_cast<f32x4_t*>(a.state + (int64_t(slot) * a.Hkv + kvh) * D * D + sl * VC) + c;
+  f32x4_t* st = reinterpret_cast<f32x4_t*>(a.state + (int64_t(slot) * a.Hkv + kvh) * D * D) + c;
   f32x4_t S[NI];
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
@@ -758,7 +755,7 @@ __global__ __launch_bounds__(256) void linear_attn_decode_kernel(LinAttnArgs a) 
   const Keep keep = keep_over(a.log_decay[kvh], 1.f);
   for (int i = tid; i < D; i += 256) ks[i] = bf2f(a.k[b * a.k_rs + kvh * D + i]);
   for (int i = tid; i < G * D; i += 256) qs[i / D][i % D] = bf2f(a.q[b * a.q_rs + kvh * G * D + i]) * a.scale;
-  const uint2 vr = *reinterpret_cast<const uint2*>(a.v + b * a.v_rs + kvh * D + sl * VC + 4 * c);
+  const uint2 vr = *reinterpret_cast<const uint2*>(a.v + b * a.v_rs + kvh * D + 4 * c);
   const float4 v = make_float4(bf_lo(vr.x), bf_hi(vr.x), bf_lo(vr.y), bf_hi(vr.y));
   __syncthreads();
 #pragma unroll
@@ -784,10 +781,10 @@ __global__ __launch_bounds__(256) void linear_attn_decode_kernel(LinAttnArgs a) 
     __syncthreads();  // `red` of the previous head has been read
     red[r0][c] = o;
     __syncthreads();
-    if (tid < VC) {
+    if (tid < D) {
       float sum = 0.f;
       for (int r = 0; r < RPI; ++r) sum += reinterpret_cast<const float*>(&red[r][0])[tid];
-      a.out[(int64_t(b) * a.H + kvh * G + g) * D + sl * VC + tid] = f2bf(sum);
+      a.out[(int64_t(b) * a.H + kvh * G + g) * D + tid] = f2bf(sum);
     }
   }
 }
@@ -937,11 +934,11 @@ extern "C" int ezops_linear_attn_decode_bf16(const void* q, int64_t q_stride, co
   // (128 MB 41 and 49 us, but 32 MB 10.6 and 9.9).
   const bool nt = B * Hkv * D * D * 4 >= int64_t(4) << 20;
   if (D == 64) {
-    if (nt) hipLaunchKernelGGL((ez::linear_attn_decode_kernel<64, 64, true>), grid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((ez::linear_attn_decode_kernel<64, 64, false>), grid, dim3(256), 0, stream, a);
+    if (nt) hipLaunchKernelGGL((ez::linear_attn_decode_kernel<64, true>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((ez::linear_attn_decode_kernel<64, false>), grid, dim3(256), 0, stream, a);
   } else {
-    if (nt) hipLaunchKernelGGL((ez::linear_attn_decode_kernel<128, 128, true>), grid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((ez::linear_attn_decode_kernel<128, 128, false>), grid, dim3(256), 0, stream, a);
+    if (nt) hipLaunchKernelGGL((ez::linear_attn_decode_kernel<128, true>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((ez::linear_attn_decode_kernel<128, false>), grid, dim3(256), 0, stream, a);
   }
   return ez::launch_status("linear_attn_decode");
 }
