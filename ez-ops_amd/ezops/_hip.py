@@ -16,7 +16,7 @@ import torch
 LIB_PATH = Path(os.environ.get("EZOPS_HIP_LIB", Path(__file__).resolve().parent / "_lib" / "libezops_hip.so"))
 
 EINVAL = -22
-ABI_VERSION = 2
+ABI_VERSION = 3
 
 _p, _i64, _f32, _sz, _i32 = C.c_void_p, C.c_int64, C.c_float, C.c_size_t, C.c_int
 
@@ -97,12 +97,12 @@ def load(path: Path) -> C.CDLL:
             "`python ez-ops_amd/build.py --all` (hipcc, gfx950)"
         )
     l = C.CDLL(str(path))
+    if l.ezops_hip_abi_version() != ABI_VERSION:  # before the entries: another version may lack some
+        raise RuntimeError(f"{path}: ABI version {l.ezops_hip_abi_version()} != {ABI_VERSION}")
     for name, (res, args) in SIGNATURES.items():
         fn = getattr(l, name)
         fn.restype = res
         fn.argtypes = args
-    if l.ezops_hip_abi_version() != ABI_VERSION:
-        raise RuntimeError(f"{path}: ABI version {l.ezops_hip_abi_version()} != {ABI_VERSION}")
     return l
 
 

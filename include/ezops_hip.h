@@ -33,7 +33,9 @@
 extern "C" {
 #endif
 
-#define EZOPS_HIP_ABI_VERSION 2
+/* Raised with every entry that is added or changed; 3: batch plan, QK norm with
+ * several position axes, linear attention. */
+#define EZOPS_HIP_ABI_VERSION 3
 #define EZOPS_EINVAL (-22)
 #define EZOPS_ENOSYS (-38) /* feature not compiled into this build */
 

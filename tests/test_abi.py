@@ -181,3 +181,19 @@ def test_sum_blocks_by_length():
         assert blocks(n) == up(g), n
     sizes = [blocks(n) for n in range(1, 1 << 23, 4099)]
     assert sizes == sorted(sizes)
+
+
+def test_a_library_of_another_version_is_named_as_such(tmp_path):
+    """A build from before an entry was added lacks it: the loader says which version it met, not which name it missed."""
+    import subprocess
+
+    src, so = tmp_path / "old.c", tmp_path / "libold.so"
+    src.write_text("int ezops_hip_abi_version(void) { return %d; }\n" % (_hip.ABI_VERSION - 1))
+    subprocess.run(["gcc", "-shared", "-fPIC", str(src), "-o", str(so)], check=True, timeout=60)
+    with pytest.raises(RuntimeError, match="ABI version"):
+        _hip.load(so)
+
+
+def test_version_is_above_the_one_without_the_ragged_entries():
+    assert _hip.ABI_VERSION >= 3
+    assert f"#define EZOPS_HIP_ABI_VERSION {_hip.ABI_VERSION}\n" in HEADER.read_text()
