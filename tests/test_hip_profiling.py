@@ -67,3 +67,32 @@ def test_wave_trace_prefill():
     assert torch.equal(out, ref)
     # (SwiGLU runs in the gate/up GEMM's epilogue at Qwen3-8B's IS = 12288)
     check_records(tr.records, {"rmsnorm_bf16", "gemm", "qk_norm_rope", "prefill_attn"})
+
+
+def test_wave_trace_ragged_ops():
+    """Records of the ragged-batch ops: each names its kernels, and every wave of a launch ran once."""
+    from ezops import LinearAttnDecodeOp, LinearAttnPrefillOp, PagedBatchPlanOp, QkNormMropeOp
+
+    torch.manual_seed(0)
+    cases = [
+        (PagedBatchPlanOp(5, 600, 32, 8, 40, backend="hip"), {}, {"batch_plan": 3 * 4}),  # 256 rows a block
+        (QkNormMropeOp(50, 4, 2, 64, 99, (12, 10, 10), backend="hip", interleaved=True, page_size=32, num_pages=2), {},
+         {"qk_norm_mrope": 7 * 4}),  # 50 tokens x (4 + 2 * 2) heads in groups of four lanes, 64 groups a block
+        (QkNormMropeOp(9, 4, 2, 6, 99, (3,), backend="hip"), {}, {"qk_norm_mrope": 14 * 4}),  # 54 heads, a wave each
+        (LinearAttnPrefillOp(2, 600, 4, 4, 128, backend="hip", num_slots=2), {},
+         {"linear_attn_prefill": None, "linear_attn_state": None}),
+        (LinearAttnPrefillOp(2, 100, 4, 4, 128, backend="hip", num_slots=2), dict(max_q_len=50), {"linear_attn_prefill": None}),
+        (LinearAttnDecodeOp(3, 8, 2, 128, 4, backend="hip"), {}, {"linear_attn_decode": 3 * 2 * 4}),  # a block a state
+    ]
+    for op, kw, waves in cases:
+        data = op.gen_data()
+        again = [x if x is None else x.clone() for x in data]
+        want = op(*data, **kw)
+        with profiling.WaveTrace() as tr:
+            got = op(*again, **kw)
+        for a, w in zip(got if isinstance(got, tuple) else [got], want if isinstance(want, tuple) else [want]):
+            assert (a is None and w is None) or torch.equal(a, w), type(op)
+        check_records(tr.records, set(waves))
+        for k, count in waves.items():
+            if count is not None:
+                assert len(tr.records) == count, (k, len(tr.records))
