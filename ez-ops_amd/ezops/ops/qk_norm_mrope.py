@@ -13,7 +13,11 @@ in fp32 with one bf16 rounding.  ``sections`` gives each axis its number of
 pairs (their sum is D/2): consecutive runs of pairs, or with ``interleaved``
 pair ``i`` belongs to axis ``i % A`` while that axis has pairs left and to axis 0
 after that.  ``cos`` / ``sin`` are HF tables ``[max_position, D]`` (both halves
-equal; the first is read), bf16 or fp32.
+equal; the first is read), bf16 or fp32.  Column ``i`` belongs to pair ``i`` whatever
+its axis, so where each axis has the same frequencies ``f`` (vision encoders: rows
+and columns of the patches) the table repeats them: with two axes of ``n`` pairs
+``angles = arange(max_position)[:, None] * f.repeat(2)``, ``cos =
+angles.cos().repeat(1, 2)``; one run of D/2 frequencies is the text decoders' form.
 
 With a paged cache (``page_size``, ``num_pages``) token ``t`` goes to slot
 ``slot_mapping[t]`` (int64, page * page_size + offset, as PagedBatchPlanOp makes

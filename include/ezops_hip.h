@@ -230,7 +230,8 @@ int ezops_paged_batch_plan(const int32_t* q_lens, const int32_t* past_lens, int3
  * sections [axes] (host memory) holds the number of pairs of each axis, D/2 in
  * sum, as consecutive runs or (interleaved) pair i to axis i % axes while
  * i < axes * sections[i % axes], else to axis 0.  cos / sin [S, D] in the HF layout
- * (both halves equal; the first D/2 columns are read), bf16 or (table_f32) fp32.
+ * (both halves equal; the first D/2 columns are read), bf16 or (table_f32) fp32; column
+ * i is pair i's, so a table for axes that share their frequencies repeats them.
  * q_out [T, H, D]; k goes to k_out [T, Hkv, D] (may be NULL with a cache) and, with
  * caches [num_pages, Hkv, page_size, D], with v to slot slot_mapping[t] =
  * page * page_size + offset; slots outside the pool are skipped, and two tokens

@@ -424,3 +424,21 @@ def test_c_entries_reject_outputs_over_small_inputs():
     for x, n in ((at(0), 256 * 2 * T), (at(1), 128 * 2 * T), (at(2), 128 * 2 * T), (at(7), states), (at(9), 4 * 64 * 2 * T)):
         for addr in (x, x + n - 16, x - need + 16):
             assert prefill(ws=addr) == _hip.EINVAL and b"overlap" in err(), (x, err())
+
+
+def test_ref_mrope_repeated_frequencies():
+    """A vision encoder's rotation, the same frequencies for rows and for columns, with the table that the op's docstring
+    gives: pair i of the section of either axis turns by position * f[i]."""
+    torch.manual_seed(6)
+    T, H, D, S, n = 12, 2, 72, 30, 18
+    f = 1e4 ** (-torch.arange(n, dtype=torch.float64) / n)
+    angles = torch.arange(S)[:, None] * f.repeat(2)  # sections (18, 18): each begins with f[0] again
+    cos, sin = (x.repeat(1, 2).float() for x in (angles.cos(), angles.sin()))
+    op = QkNormMropeOp(T, H, H, D, S, (n, n), norm=False)
+    q, k = (torch.randn(T, H, D).to(torch.bfloat16) for _ in range(2))
+    pos = torch.stack([torch.arange(T) // 4 * 7, torch.arange(T) % 4 + 3]).to(torch.int32)
+    got, _ = op(q, k, None, None, None, cos, sin, pos)
+    turn = torch.cat([pos[0, :, None] * f, pos[1, :, None] * f], 1)[:, None]
+    a, b = q.double()[..., :D // 2], q.double()[..., D // 2:]
+    want = torch.cat([a * turn.cos() - b * turn.sin(), b * turn.cos() + a * turn.sin()], -1)
+    np.testing.assert_allclose(_np(got), want.numpy(), rtol=2 ** -8, atol=1e-5)
