@@ -72,10 +72,19 @@ __device__ __forceinline__ float decayed(const Keep& k, float S, float x) {
   return k.near ? S + y : y;
 }
 
-// Whether sequence c keeps `slot` from those behind it: only with tokens, of which a single token's call has one
-// for every sequence (an idle row of a padded prompt batch may carry any slot).
-__device__ __forceinline__ bool holds(const LinAttnArgs& a, int c, int slot) {
-  return a.state_slots[c] == slot && (!a.cu || seq_rows(a.cu[c], a.cu[c + 1], int(a.T), int(a.max_q)).count > 0);
+// Whether a sequence in front of b holds `slot`: one with tokens, of which a single token's call has one for every
+// sequence (an idle row of a padded prompt batch may carry any slot); lengths are looked at only where a slot is
+// equal.  Every thread of the block calls it (barriers inside).
+template <int THREADS>
+__device__ __forceinline__ bool slot_held(const LinAttnArgs& a, int b, int slot) {
+  int held = 0;
+  for (int c = threadIdx.x; c < b; c += THREADS) held |= a.state_slots[c] == slot;
+  held = __syncthreads_or(held);
+  if (!held || !a.cu) return held;
+  held = 0;
+  for (int c = threadIdx.x; c < b; c += THREADS)
+    held |= a.state_slots[c] == slot && seq_rows(a.cu[c], a.cu[c + 1], int(a.T), int(a.max_q)).count > 0;
+  return __syncthreads_or(held);
 }
 
 // Slot of sequence b, -1 if it has none: outside the pool, or held by an earlier
@@ -83,12 +92,8 @@ __device__ __forceinline__ bool holds(const LinAttnArgs& a, int c, int slot) {
 template <int THREADS>
 __device__ __forceinline__ int slot_of(const LinAttnArgs& a, int b) {
   const int s = a.state_slots ? a.state_slots[b] : b;
-  int dup = 0;
-  if (a.state_slots) {
-    for (int c = threadIdx.x; c < b; c += THREADS) dup |= holds(a, c, s);
-    dup = __syncthreads_or(dup);
-  }
-  return s < 0 || s >= a.num_slots || dup ? -1 : s;
+  const bool held = a.state_slots && slot_held<THREADS>(a, b, s);
+  return s < 0 || s >= a.num_slots || held ? -1 : s;
 }
 
 // ---- prompts: the chunked form ------------------------------------------
@@ -313,12 +318,7 @@ __device__ __forceinline__ bool find_segment(const LinAttnArgs& a, int id, Segme
   const int n = __builtin_amdgcn_readfirstlane(s_seq[1]);
   slot = __builtin_amdgcn_readfirstlane(s_seq[2]);
   past = __builtin_amdgcn_readfirstlane(s_seq[3]);
-  if (a.state) {
-    int dup = slot < 0 || slot >= a.num_slots;
-    if (a.state_slots)
-      for (int c = threadIdx.x; c < b; c += THREADS) dup |= holds(a, c, slot);
-    if (__syncthreads_or(dup)) return false;
-  }
+  if (a.state && (slot < 0 || slot >= a.num_slots || (a.state_slots && slot_held<THREADS>(a, b, slot)))) return false;
   const int s = id - ((r0 >> a.seg_sh) + b);
   if (n <= 0 || s < 0 || s >= (n + a.seg - 1) >> a.seg_sh) return false;
   const int cnt = (n + a.seg - 1) >> a.seg_sh;
