@@ -550,3 +550,35 @@ def test_overflow_stays_in_its_query_and_sequence(H, D):
     o, S1, to, ts = _expect(x, k[:64], v[:64], g, first, D ** -0.5)
     _close(n(out), o, to, "large")
     _close(n(S[0]), S1, ts, "large")
+
+
+def test_largest_batch():
+    """65536 sequences: a long prompt first (so that all kernels run), then fresh single tokens, one slot held already;
+    and 65536 single tokens of the recurrent form."""
+    B, D, L = 65536, 64, 300
+    T = B - 1 + L
+    q, k, v = _inputs(T, 1, 1, D, 81)
+    i32, g = dict(dtype=torch.int32, device=DEV), _decay(1)
+    cu = torch.cat([torch.zeros(1, **i32), torch.arange(L, T + 1, **i32)])
+    slots = torch.arange(B, **i32)
+    slots[-1] = 5
+    S = torch.full((B, 1, D, D), 7.0, device=DEV)
+    out = torch.full((T, 1, D), 7.0, dtype=torch.bfloat16, device=DEV)
+    LinearAttnPrefillOp(B, T, 1, 1, D, backend="hip", num_slots=B)(q, k, v, g, cu, S, slots, out=out)
+    o, S1, to, ts = _expect(q[:L], k[:L], v[:L], g, np.zeros((1, D, D)), D ** -0.5)
+    _close(n(out[:L]), o, to, "long")
+    _close(n(S[0]), S1, ts, "long")
+    x, y, z = (t[L:-1, 0].double() for t in (q, k, v))
+    want, most = (x * y).sum(-1, keepdim=True) * z * D ** -0.5, (x * y).abs().sum(-1, keepdim=True) * z.abs() * D ** -0.5
+    assert bool(((out[L:-1, 0].double() - want).abs() <= 2.0 ** -8 * want.abs() * 1.01 + 2.0 ** -14 * most).all())
+    assert bool(((S[1:-1, 0] - k[L:-1, 0].float()[:, :, None] * v[L:-1, 0].float()[:, None]).abs() <= 2.0 ** -15 * S[1:-1, 0].abs()).all())
+    assert bool((out[-1] == 7).all()) and bool((S[-1] == 7).all())
+    start = S.clone()
+    q, k, v = (t[L - 1:] for t in (q, k, v))
+    got = LinearAttnDecodeOp(B, 1, 1, D, B, backend="hip")(q, k, v, g, S, out=torch.empty_like(out[L - 1:]))
+    lam, b = torch.exp(g.double())[0], torch.tensor([0, 1, 77, 40000, B - 1], device=DEV)
+    S1 = lam * start[b, 0].double() + k[b, 0].double()[:, :, None] * v[b, 0].double()[:, None]
+    aS = lam * start[b, 0].double().abs() + (k[b, 0].double()[:, :, None] * v[b, 0].double()[:, None]).abs()
+    assert bool(((S[b, 0].double() - S1).abs() <= 8 * 2.0 ** -24 * aS).all())
+    o, ao = ((x[:, :, None] * s).sum(1) * D ** -0.5 for x, s in ((q[b, 0].double(), S1), (q[b, 0].double().abs(), aS)))
+    assert bool(((got[b, 0].double() - o).abs() <= 2.0 ** -8 * o.abs() * 1.01 + (D + 24) * 2.0 ** -24 * ao).all())
