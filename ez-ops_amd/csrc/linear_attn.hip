@@ -8,10 +8,12 @@
 // -inf) is allowed: only powers lambda^n with n >= 0 appear, and lambda^0 = 1.
 //
 // Over prompts the work is matrix products (a chunk of 64 tokens: 2 x 64 x 128 x (64 + 128) flops a query
-// head and 2 x 64 x 128 x 128 a kv head, in two or three bf16 parts), bound by the matrix cores and the
-// conversions beside them at two waves a SIMD; for single tokens it is the state's traffic.  Measured: 4096 tokens
-// of 32 / 8 heads of 128 47 us (84 MB: 1.8 TB/s), two prompts of 16384 x 32 / 32 397 us (1.08 GB: 2.7 TB/s; read
-// and written once at a copy's rate 219), 200 single tokens x 32 states 153 us (845 MB: 5.5 TB/s).
+// head and 2 x 64 x 128 x 128 a kv head, in two or three bf16 parts).  Prompts of some thousand tokens are bound by
+// latency: of the output kernel's time the matrix cores are busy for 30%, the VALU for 40%, and its two waves a SIMD
+// spend a third of theirs at waits and barriers (4096 tokens of 32 / 8 heads of 128: 47 us in all, 84 MB or 1.8
+// TB/s).  Longer ones come near the memory: its output kernel moves 1.09 GB at 4.1 TB/s for two prompts of 16384
+// x 32 / 32 heads, but the sums have read K and V before it (411 us in all; read and written once at a copy's
+// rate 219).  Single tokens are bound by the state's traffic (200 x 32 states 153 us, 845 MB: 5.5 TB/s).
 //
 // A sequence's state lives in a pool of slots.  A sequence whose slot lies
 // outside the pool, or that an earlier sequence with tokens holds already, is
@@ -346,7 +348,7 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
   __shared__ __align__(1024) uint16_t Ps[OUT ? 3 * 4 * 512 : 8];  // block of P x (16-key step, part) x lane x 8
   __shared__ float pw[96];
   // The blocks that share a kv head's K, V and state are 8 apart: on one XCD, whose L2 then reads them once, and the
-  // one that has summed the segment (4096 tokens of 32 / 8 heads 49.3 -> 47.0 us, 1024 30.6 -> 28.1).
+  // one that has summed the segment (all kernels, 4096 tokens of 32 / 8 heads: 5% less time, 1024 tokens 8%).
   const int split = OUT ? a.split : 1, units = a.segments * a.Hkv;
   const int u0 = int(blockIdx.x) / (8 * split) * 8, within = int(blockIdx.x) - u0 * split, wide = min(8, units - u0);
   const int part = within / wide, unit = u0 + within - part * wide;
@@ -459,7 +461,7 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
   };
   // Sums take the chunks from the last to the first, their weights counted from the segment's end: what the
   // memory-side cache still holds of K and V is then where the output kernel begins, and no sum has to be decayed
-  // (2 x 16384 tokens of 32 / 32 heads: 424 -> 405 us, all kernels; 4096 of 32 / 8: 49.7 -> 49.3).
+  // (all kernels, 2 x 16384 tokens of 32 / 32 heads: 4% less time, 4096 of 32 / 8 1%).
   const int c0 = OUT ? 0 : chunks - 1;
   load_k(c0);
   load_v(c0);
@@ -642,8 +644,8 @@ __global__ __launch_bounds__(2 * D) __attribute__((amdgpu_waves_per_eu(2))) void
 // Block = (sequence, kv head, 256 elements), one element a thread: the chain over the segments is
 // short of work per step, so the chip is filled with threads, each eight loads ahead of its sums.
 // With Hkv a multiple of 8 a kv head is on one XCD in all three kernels (workgroups go round the XCDs in turn), and
-// sums and states stay in its L2 (six sequences of up to 900 tokens, 32 / 8 heads, 34.7 -> 30.7 us; 1024 tokens 28.4 ->
-// 24.5, 4096 47.3 -> 45.4).
+// sums and states stay in its L2 (all kernels, 32 / 8 heads: six sequences of up to 260 tokens 12% less time, 1024 tokens
+// 14%, 4096 4%).
 template <int D>
 __global__ __launch_bounds__(256) void linear_attn_scan_kernel(LinAttnArgs a) {
   EZ_PROF_WAVE(kProfLinAttnState);
@@ -691,18 +693,21 @@ __global__ __launch_bounds__(256) void linear_attn_scan_kernel(LinAttnArgs a) {
 }
 
 // log2 of the tokens per segment: the longest segments that still give about 512 blocks over the whole
-// batch, two a CU (2 x 16384 tokens of 32 / 32 heads, all three kernels: 401 us, with 256 blocks 525); two chunks
-// as soon as that gives one block a CU (4096 tokens of 32 / 8: 45.1 us, with 512 blocks of a chunk 50.5: each segment
+// batch, two a CU (2 x 16384 tokens of 32 / 32 heads, all three kernels: with 256 blocks 31% slower, with 1024 7%); two
+// chunks as soon as that gives one block a CU (4096 tokens of 32 / 8: with 512 blocks of a chunk 12% slower, each segment
 // costs 256 KiB of state traffic a kv head); at least a chunk.  Two chunks of one or two query heads a kv head are not
-// cut at all (128 tokens of 8 / 8 heads 12.9 us, cut 16.9).
+// cut at all (128 tokens of 8 / 8 heads, cut: 31% slower).  The same numbers serve heads of 64, whose blocks are half
+// as many waves: with twice the blocks here and below 4096 and 16384 tokens of 32 / 8 heads take 33.5 and 86.7 us
+// (31.2 and 76.2), 16384 of 32 / 32 121.7 (118.8), 300 tokens 21.6 (22.2), 64 to 1024 otherwise the same.
 int segment_shift(int64_t T, int64_t G, int64_t Hkv, int64_t max_q) {
   int sh = 6;
   while ((T * Hkv) >> (sh + 1) >= (sh < 7 ? 256 : 512)) ++sh;
   return G <= 2 && max_q <= 2 * kC && sh < 7 ? 7 : sh;
 }
-// Blocks a kv head's query heads are shared out to where the segments alone leave CUs without work (up to
-// about two a CU); each of them updates the state for itself, and the first leaves it.  64 tokens of
-// 32 / 8 heads: 9.0 us, in one block a kv head 15.2; 4096 tokens 45.4, with 1056 blocks 53.3.
+// Blocks a kv head's query heads are shared out to where the segments alone leave CUs without work; each of them
+// updates the state for itself, and the first leaves it.  Up to two a CU and 64 for the last segments of the
+// sequences, which are blocks too (4096 tokens of 32 / 8 heads: 528).  64 fresh tokens of 32 / 8 heads: in one block
+// a kv head 69% slower; 4096 tokens with 1056 blocks 17% slower.
 int head_split(int64_t blocks, int64_t G) {
   int64_t n = 1;
   while (2 * n <= G && blocks * 2 * n <= 576) n *= 2;

@@ -13,8 +13,8 @@
 //
 // The work is memory traffic: q and k in and out, v into the cache, 2 D bytes a
 // head each; the table rows are shared by the heads of a token.  Measured: 16384
-// tokens of 32 + 2 x 8 heads of 128 80 us, 5.1 TB/s (a large copy reaches 4.9); 4097
-// tokens of 16 + 2 x 8 14.3 us; 16 tokens 5.3 us, a launch and three dependent loads.
+// tokens of 32 + 2 x 8 heads of 128 78 us, 5.2 TB/s (a large copy reaches 4.9); 4097
+// tokens of 16 + 2 x 8 14.4 us; 16 tokens 5.3 us, a launch and three dependent loads.
 #include "common.h"
 #include "internal.h"
 #include "prof.h"
