@@ -33,6 +33,7 @@ enum ProfKernel : uint16_t {
   kProfGemvRows = 1, kProfGemvValu, kProfLinearScalar, kProfLinearMfma, kProfAttnSplit, kProfAttnCombine,
   kProfPrefillAttn, kProfSiluMul, kProfQkRope, kProfRmsnormF32, kProfRmsnormBf16, kProfSoftmax, kProfSum, kProfGemm,
   kProfBatchPlan, kProfQkMrope, kProfLinAttnPrefill, kProfLinAttnDecode, kProfLinAttnState,
+  kProfKvQuant, kProfKvDequant, kProfQuantAttnDecode, kProfQuantAttnCombine, kProfQuantAttnPrefill,
 };
 
 // Records are appended per CU (region = XCC, SE, SH, CU from the hardware

@@ -16,7 +16,7 @@ import torch
 LIB_PATH = Path(os.environ.get("EZOPS_HIP_LIB", Path(__file__).resolve().parent / "_lib" / "libezops_hip.so"))
 
 EINVAL = -22
-ABI_VERSION = 3
+ABI_VERSION = 4
 
 _p, _i64, _f32, _sz, _i32 = C.c_void_p, C.c_int64, C.c_float, C.c_size_t, C.c_int
 
@@ -72,6 +72,14 @@ SIGNATURES: dict[str, tuple] = {
                                        + [_f32, _p, _sz, _p]),
     "ezops_linear_attn_decode_bf16": (_i32, [_p, _i64, _p, _i64, _p, _i64, _p, _p, _p, _i64, _p, _i64, _i64, _i64, _i64,
                                              _f32, _p]),
+    "ezops_kv_cache_quant_bf16": (_i32, [_p, _i64, _p, _i64] + [_p] * 5 + [_i32] + [_i64] * 6 + [_p]),
+    "ezops_kv_cache_dequant_bf16": (_i32, [_p] * 5 + [_i32] + [_i64] * 3 + [_p, _p] + [_i64] * 3 + [_p]),
+    "ezops_quant_paged_attn_decode_workspace_size": (_sz, [_i64] * 5),
+    "ezops_quant_paged_attn_decode_bf16": (_i32, [_p, _i64] + [_p] * 4 + [_i32] + [_p] * 3 + [_i64] * 9
+                                           + [_f32, _p, _sz, _p]),
+    "ezops_quant_prefill_attn_workspace_size": (_sz, [_i64] * 6),
+    "ezops_quant_prefill_attn_bf16": (_i32, [_p, _i64] + [_p] * 4 + [_i32] + [_p] * 4 + [_i64] * 10
+                                      + [_f32, _p, _sz, _p]),
     "ezops_o_proj_ffn_workspace_size": (_sz, [_i64, _i64, _i64, _i64]),
     "ezops_o_proj_ffn_bf16": (_i32, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _f32, _p, _sz, _p]),
     "ezops_qwen3_layer_workspace_size": (_sz, [C.POINTER(Qwen3LayerParams)]),

@@ -55,7 +55,8 @@ KERNEL_NAMES = {
     1: "gemv_rows", 2: "gemv_valu", 3: "linear_scalar", 4: "linear_mfma", 5: "attn_split", 6: "attn_combine",
     7: "prefill_attn", 8: "silu_mul", 9: "qk_norm_rope", 10: "rmsnorm_f32", 11: "rmsnorm_bf16", 12: "softmax",
     13: "sum", 14: "gemm", 15: "batch_plan", 16: "qk_norm_mrope", 17: "linear_attn_prefill", 18: "linear_attn_decode",
-    19: "linear_attn_state",
+    19: "linear_attn_state", 20: "kv_quant", 21: "kv_dequant", 22: "quant_attn_decode", 23: "quant_attn_combine",
+    24: "quant_attn_prefill",
 }
 TICKS_PER_US = 100.0  # s_memrealtime runs at 100 MHz
 MAX_RECORDS = 1 << 21  # host buffer of a WaveTrace (64 MiB)

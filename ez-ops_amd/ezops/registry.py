@@ -9,7 +9,9 @@ reference wraps ``__call__`` in a TileLang cache-naming scope
 registered unchanged.
 
 Ops come in families: ``"decode"`` (the decode path, what ``list_ops()`` has
-always listed) and ``"ragged"`` (the ragged-batch serving ops around it).
+always listed), ``"ragged"`` (the ragged-batch serving ops around it) and
+``"kv8"`` (the ops over a KV cache held in 8 bits).  ``list_ops(None)`` lists the
+first two, as it always has; ``list_ops("all")`` lists every op.
 ``get_kernel`` and ``list_backends`` know every op.
 """
 
@@ -51,5 +53,6 @@ def list_backends(op_name: str) -> list[str]:
 
 
 def list_ops(family: str | None = "decode") -> list[str]:
-    """Op names of one family (``None``: of all)."""
-    return sorted({n for (n, _) in _KERNEL_REGISTRY if family is None or _FAMILY[n] == family})
+    """Op names of one family (``None``: decode and ragged; ``"all"``: of every family)."""
+    want = {None: ("decode", "ragged"), "all": set(_FAMILY.values())}.get(family, (family,))
+    return sorted({n for (n, _) in _KERNEL_REGISTRY if _FAMILY[n] in want})

@@ -35,7 +35,7 @@ extern "C" {
 
 /* Raised with every entry that is added or changed; 3: batch plan, QK norm with
  * several position axes, linear attention. */
-#define EZOPS_HIP_ABI_VERSION 3
+#define EZOPS_HIP_ABI_VERSION 4
 #define EZOPS_EINVAL (-22)
 #define EZOPS_ENOSYS (-38) /* feature not compiled into this build */
 
@@ -296,6 +296,73 @@ int ezops_linear_attn_decode_bf16(const void* q, int64_t q_stride, const void* k
                                   const int32_t* state_slots, int64_t num_slots, void* out, int64_t B,
                                   int64_t H, int64_t Hkv, int64_t D, float scale, hipStream_t stream);
 
+/* KV cache held in 8 bits: codes [num_pages, Hkv, page_size, D] (cache_type 0 = int8,
+ * 1 = OCP e4m3) and exponents [num_pages, Hkv, page_size / block_size] of one byte, a row
+ * standing for code * 2^(e - 127), NaN where e = 255.
+ * Quantise k / v [T, Hkv, D] bf16 (token strides in elements, multiples of 8) into slots
+ * slot_mapping[t] = page * page_size + offset; slots outside the pool are skipped.  Over
+ * the tokens that a block of block_size rows gets in this call, need = the least e in
+ * [67, 187] with max|x| <= TOP 2^(e - 127), TOP = 127 or 448; e = need where the block's
+ * first row is among them, else max(need, e as it was), and where that grows, the rows
+ * held before become round(code 2^(e_old - e)); code = round(x 2^(127 - e)), to nearest
+ * even, saturating.  The tokens of a block must be consecutive with ascending slots; else,
+ * or where a slot comes twice, the rows and the scale of that block (and nothing else) are
+ * undefined.  Not finite: NaN code 0x7f (e4m3), or e = 255 for the block (int8).  D in {64,
+ * 128}; page_size a power of two in [32, 2^20], block_size one in [16, 256] and at most
+ * page_size; k, v and the caches 16-byte aligned; caches and scales must not overlap each
+ * other or an input.
+ * No counterpart in the reference (bf16 cache, ezops/ops/attn_decode.py:60-61). */
+int ezops_kv_cache_quant_bf16(const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                              const int64_t* slot_mapping, void* K_cache, void* V_cache,
+                              void* K_scale, void* V_scale, int cache_type, int64_t num_pages,
+                              int64_t page_size, int64_t block_size, int64_t T, int64_t Hkv,
+                              int64_t D, hipStream_t stream);
+
+/* Read back rows slot_mapping[t] (any order, repeats allowed) as bf16 into k_out / v_out
+ * [T, Hkv, D] (16-byte aligned); rows of slots outside the pool are not written. */
+int ezops_kv_cache_dequant_bf16(const void* K_cache, const void* V_cache, const void* K_scale,
+                                const void* V_scale, const int64_t* slot_mapping, int cache_type,
+                                int64_t num_pages, int64_t page_size, int64_t block_size,
+                                void* k_out, void* v_out, int64_t T, int64_t Hkv, int64_t D,
+                                hipStream_t stream);
+
+/* Attention of one token per sequence over that cache: q [B, H, D] bf16 (row stride in
+ * elements, a multiple of 8), block_table [B, max_pages] int32, kv_lens [B] int32, out
+ * [B, H, D] bf16; sequence b sees its first kv_lens[b] rows (at most max_kv_len, where
+ * that is > 0), one without rows gets zeros.  max_kv_len plans the work.  Page ids outside
+ * the pool are clamped into it; codes and scales of rows behind a length may hold
+ * anything.  H / Hkv in {1, 2, 4, 8, 16}, D in {64, 128}, B <= 65536, H <= 4096; scale <= 0
+ * selects 1/sqrt(D).  workspace: 16-byte aligned,
+ * ezops_quant_paged_attn_decode_workspace_size(B, H, Hkv, D, max_kv_len or max_pages *
+ * page_size) bytes, need not be zero-filled (NULL where that is 0).
+ * No counterpart in the reference (bf16 cache, ezops/ops/attn_decode.py:9-67). */
+size_t ezops_quant_paged_attn_decode_workspace_size(int64_t B, int64_t H, int64_t Hkv, int64_t D,
+                                                    int64_t kv_len);
+int ezops_quant_paged_attn_decode_bf16(const void* q, int64_t q_stride, const void* K_cache,
+                                       const void* V_cache, const void* K_scale,
+                                       const void* V_scale, int cache_type,
+                                       const int32_t* block_table, const int32_t* kv_lens, void* out,
+                                       int64_t B, int64_t H, int64_t Hkv, int64_t D,
+                                       int64_t num_pages, int64_t page_size, int64_t max_pages,
+                                       int64_t block_size, int64_t max_kv_len, float scale,
+                                       void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* The same for packed prompts and chunks, causal: q / out [T, H, D]; sequence b owns rows
+ * cu_seqlens[b] .. cu_seqlens[b+1]-1 (clamped into [0, T]; the offsets must not decrease),
+ * its token i stands at cache row past_lens[b] + i (past_lens NULL = 0) and sees the rows
+ * up to that one.  Rows of no sequence, and of tokens at or past max_pages * page_size or
+ * max_kv_len (where that is > 0), are not written. */
+size_t ezops_quant_prefill_attn_workspace_size(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t D,
+                                               int64_t kv_len);
+int ezops_quant_prefill_attn_bf16(const void* q, int64_t q_stride, const void* K_cache,
+                                  const void* V_cache, const void* K_scale, const void* V_scale,
+                                  int cache_type, const int32_t* block_table,
+                                  const int32_t* cu_seqlens, const int32_t* past_lens, void* out,
+                                  int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t D,
+                                  int64_t num_pages, int64_t page_size, int64_t max_pages,
+                                  int64_t block_size, int64_t max_kv_len, float scale,
+                                  void* workspace, size_t workspace_bytes, hipStream_t stream);
+
 /* Fused o_proj + post-norm + SwiGLU FFN (batch x 1 token), bf16:
  *   x2 = residual + attn @ Wo^T ; xn = rmsnorm(x2) * post_norm_w
  *   out = x2 + (silu(xn @ Wg^T) * (xn @ Wu^T)) @ Wd^T
@@ -439,7 +506,8 @@ int ezops_gemm_swiglu_bf16(const void* X, int64_t ldx, const void* Wgu, void* Y,
  *                   5 attn_split, 6 attn_combine, 7 prefill_attn, 8 silu_mul,
  *                   9 qk_norm_rope, 10 rmsnorm_f32, 11 rmsnorm_bf16, 12 softmax, 13 sum,
  *                   14 gemm, 15 batch_plan, 16 qk_norm_mrope, 17 linear_attn_prefill,
- *                   18 linear_attn_decode, 19 linear_attn_state)
+ *                   18 linear_attn_decode, 19 linear_attn_state, 20 kv_quant, 21 kv_dequant,
+ *                   22 quant_attn_decode, 23 quant_attn_combine, 24 quant_attn_prefill)
  *   uint16 wave     wave index in its block;  uint32 block  blockIdx.x
  * ezops_profile_reset clears the buffers; ezops_profile_read copies up to
  * `capacity` records to host memory and returns how many (both synchronise
