@@ -253,18 +253,6 @@ __device__ __forceinline__ int rank_to_seq(const int32_t* lens, int B, int r, in
   return b;
 }
 
-// Inclusive prefix sum over the 64 lanes (DPP row shifts, then the rows' totals
-// broadcast to the rows behind them).
-__device__ __forceinline__ int wave_scan(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // lane 15 of rows 0, 2 to rows 1, 3
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // lane 31 to rows 2, 3
-  return v;
-}
-
 // LAYER: q (and the decoded token's k, v) come from the bf16 QKV projection
 // row a.qkv + b*a.qkv_bs, columns [q | k | v]; q and k get the per-head
 // RMSNorm and RoPE at position kv_len - 1.  The unit's first block writes

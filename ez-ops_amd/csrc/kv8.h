@@ -54,8 +54,14 @@ inline void fill_kv8(Kv8Args& a, const void* K, const void* V, const void* Ks, c
 inline int64_t kv8_pool_bytes(const Kv8Args& a) { return a.num_slots * a.Hkv * a.D; }
 inline int64_t kv8_scale_bytes(const Kv8Args& a) { return (a.num_slots >> a.block_sh) * a.Hkv; }
 
-// 2^(e - 127); 255 is the NaN pattern, 0 gives zero.
-__device__ __forceinline__ float kv8_scale(uint32_t e) { return __uint_as_float(e == kKvNanExp ? 0x7fc00000u : e << 23); }
+// Exponents outside [67, 187], which no write makes, are read as the nearest end; 255 stays.
+__host__ __device__ __forceinline__ int kv8_exp(int e) {
+  return e == kKvNanExp ? e : e < kKvLowExp ? kKvLowExp : e > kKvHighExp ? kKvHighExp : e;
+}
+// 2^(e - 127), NaN for 255.
+__device__ __forceinline__ float kv8_scale(int e) {
+  return __uint_as_float(e == kKvNanExp ? 0x7fc00000u : uint32_t(kv8_exp(e)) << 23);
+}
 
 // ---- codes -> bf16 (exact: e4m3 has 4 significant bits, int8 at most 7 and a sign)
 template <int TYPE>
@@ -113,3 +119,15 @@ __device__ __forceinline__ int kv8_need(uint32_t m) {
 }
 
 }  // namespace ez
+
+// A launch for the head size D and the cache type of `a.c`.
+#define EZ_KV8_DISPATCH(LAUNCH)                                      \
+  do {                                                               \
+    if (a.c.type == ez::kKvInt8) {                                   \
+      if (D == 64) LAUNCH(64, ez::kKvInt8);                          \
+      else LAUNCH(128, ez::kKvInt8);                                 \
+    } else {                                                         \
+      if (D == 64) LAUNCH(64, ez::kKvE4m3);                          \
+      else LAUNCH(128, ez::kKvE4m3);                                 \
+    }                                                                \
+  } while (0)

@@ -71,12 +71,11 @@ __global__ __launch_bounds__(256) void kv_quant_kernel(KvQuantArgs a) {
     const int64_t row0 = ((page * a.c.Hkv + h) << a.c.page_sh) + (slot & ((int64_t(1) << a.c.page_sh) - 1));
     uint8_t* sp = (is_v ? a.c.Vs : a.c.Ks) + (row0 >> a.c.block_sh);
     uint8_t* dst = (is_v ? a.c.V : a.c.K) + row0 * D;
-    const int old = off ? int(*sp) : 0;
+    const int old = off ? kv8_exp(int(*sp)) : 0;
     int e = poison ? kKvNanExp : kv8_need<TYPE>(m);
     e = max(e, old);
     if (off && e > old) {
-      const int f = 127 + old - e;
-      const float r = e == kKvNanExp || f <= 0 ? 0.f : __uint_as_float(uint32_t(f) << 23);
+      const float r = e == kKvNanExp ? 0.f : __uint_as_float(uint32_t(127 + old - e) << 23);
       uint32_t* old_rows = reinterpret_cast<uint32_t*>(dst - int64_t(off) * D);
       for (int i = lane; i < off * D / 4; i += kWave) {
         float y[4];
@@ -85,7 +84,7 @@ __global__ __launch_bounds__(256) void kv_quant_kernel(KvQuantArgs a) {
         old_rows[i] = kv8_codes<TYPE, true>(y);
       }
     }
-    const float inv = e >= 254 ? 0.f : __uint_as_float(uint32_t(254 - e) << 23);
+    const float inv = e == kKvNanExp ? 0.f : __uint_as_float(uint32_t(254 - e) << 23);
     for (int i = lane; i < n * D / 4; i += kWave) {
       const uint16_t* p = src + (4 * i / D) * rs + 4 * i % D;
       float y[4];
@@ -130,17 +129,6 @@ int check_rows(const char* op, int64_t T, int64_t Hkv, int64_t D) {
 
 }  // namespace
 }  // namespace ez
-
-#define EZ_KV8_DISPATCH(LAUNCH)                                      \
-  do {                                                               \
-    if (a.c.type == ez::kKvInt8) {                                   \
-      if (D == 64) LAUNCH(64, ez::kKvInt8);                          \
-      else LAUNCH(128, ez::kKvInt8);                                 \
-    } else {                                                         \
-      if (D == 64) LAUNCH(64, ez::kKvE4m3);                          \
-      else LAUNCH(128, ez::kKvE4m3);                                 \
-    }                                                                \
-  } while (0)
 
 extern "C" int ezops_kv_cache_quant_bf16(const void* k, int64_t k_stride, const void* v, int64_t v_stride,
                                          const int64_t* slot_mapping, void* K_cache, void* V_cache, void* K_scale,

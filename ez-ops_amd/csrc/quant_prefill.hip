@@ -1,0 +1,485 @@
+// Causal attention of packed prompts and chunks over the 8-bit KV cache.
+//
+//   s_j = scale * q . kc_j 2^(ek - 127),  o = sum_j softmax(s)_j vc_j 2^(ev - 127)
+//
+// kc, vc are the codes, ek, ev the exponents of the key's block of rows (at least 16
+// rows each).  Both products run on v_mfma_f32_32x32x16_bf16 with the codes as they are
+// (int8 and e4m3 are exact in bf16), and the scales enter the softmax, whose weights
+// are taken in the exp2 domain: with c = scale log2(e) 2^(ek - 127) and v = ev - 127
+//
+//   w_j = 2^(c s'_j - m + v)   s' = q . kc      (the weight times the scale of v)
+//   o  += w_j vc_j,  l += w_j 2^-v
+//
+// so a scale costs nothing per key: c and v - m are the operands of the fused
+// multiply-add that the exponent needs anyway, 2^-v the other factor of the dot product
+// that sums the weights.  w is rounded to bf16 for the product; l sums the rounded
+// weights, so that rounding cancels in o / l but for its spread.
+//
+// A block owns 256 rows of one kv head: (query, head of the group) pairs, 256 / G
+// queries, 32 rows a wave; all share the K / V tiles of 64 keys.  A tile is read once
+// from memory in 8 bits (16 bytes a thread and tensor, two tiles ahead in registers),
+// widened to bf16 on its way into one of two LDS buffers, so the widening is done
+// once for the 8 waves.  Operand layouts (lane 32 h + j): S^T = K Q^T, then O^T = V^T P^T
+// with the weights staying in their lane; V^T by transposing LDS reads.
+//
+// Where the queries are few (a chunk on a long prefix) the keys are shared out over
+// nsplit blocks; they leave fp32 partials (O, m, l), which a second kernel joins.
+#include "common.h"
+#include "internal.h"
+#include "prof.h"
+#include "quant_attn.h"
+#include "status.h"
+#include "../../include/ezops_hip.h"
+
+namespace ez {
+
+EZ_PROF_DEFINE(quantprefill)
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLazy = 8.f;     // log2 headroom of the softmax reference, see below
+constexpr float kLowest = -3e38f;  // reference before any key: finite, so that differences are
+constexpr int kW = 8;            // waves of a block
+constexpr int kRows = 32 * kW;   // (query, head) rows of a block
+constexpr int kBK = 64;          // keys of a tile
+constexpr int kMaxSplits = 32;
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+
+struct SplitPlan {
+  int nsplit;
+  int tiles;   // query tiles of all sequences, at most
+  float* o;    // partials [nsplit][T * H][D]
+  float* ml;   // [nsplit][T * H][2]
+};
+
+__device__ __forceinline__ float halves_max(float v) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+__device__ __forceinline__ float halves_sum(float v) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+
+// A query tile: QT queries from query `first` on of the sequence whose rows begin at t0.
+struct QueryTile {
+  int b, t0, qlen, past, first;
+};
+
+// The idx-th query tile of the batch; false if there are fewer.  A sequence's last tiles,
+// which see the most keys, come first.  Offsets and lengths come from the device and may
+// hold anything: they are clamped into the rows and the cache.
+template <int QT>
+__device__ __forceinline__ bool find_tile(const QuantAttnArgs& a, int idx, QueryTile& q) {
+  const int lane = threadIdx.x & (kWave - 1), T = int(a.T), cap = int(a.cap);
+  for (int b0 = 0; b0 < int(a.B); b0 += kWave) {
+    const int b = b0 + lane;
+    int t0 = 0, n = 0, past = 0;
+    if (b < int(a.B)) {
+      t0 = min(max(a.cu[b], 0), T);
+      past = a.past ? min(max(a.past[b], 0), cap) : 0;
+      n = min(min(max(a.cu[b + 1], 0), T) - t0, cap - past);
+    }
+    const int tiles = n > 0 ? (n + QT - 1) / QT : 0;
+    const int end = wave_scan(tiles);
+    const uint64_t hit = __ballot(idx < end);
+    if (hit) {
+      const int l = __ffsll(static_cast<unsigned long long>(hit)) - 1;
+      q.b = b0 + l;
+      q.t0 = __builtin_amdgcn_readlane(t0, l);
+      q.qlen = __builtin_amdgcn_readlane(n, l);
+      q.past = __builtin_amdgcn_readlane(past, l);
+      q.first = (__builtin_amdgcn_readlane(end, l) - 1 - idx) * QT;
+      return true;
+    }
+    idx -= __builtin_amdgcn_readlane(end, kWave - 1);
+  }
+  return false;
+}
+
+// Key tiles of a split of the tile's `n` key tiles, and how many splits have any.
+__device__ __forceinline__ int split_tiles(int n, int nsplit) { return (n + nsplit - 1) / nsplit; }
+
+__device__ __forceinline__ bool has_nan_code(uint32_t w) {  // an e4m3 byte of 0x7f or 0xff
+  const uint32_t x = (w & 0x7f7f7f7fu) ^ 0x7f7f7f7fu;
+  return ((x - 0x01010101u) & ~x & 0x80808080u) != 0;
+}
+__device__ __forceinline__ uint32_t without_nan(uint32_t w) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (((w >> (8 * i)) & 0x7f) == 0x7f) w &= ~(0xffu << (8 * i));
+  return w;
+}
+
+template <int D, int TYPE, int G>
+__global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(2))) void quant_prefill_kernel(QuantAttnArgs a,
+                                                                                                          SplitPlan pl) {
+  EZ_PROF_WAVE(kProfQuantAttnPrefill);
+  constexpr int QT = kRows / G;     // queries of a block
+  constexpr int NS = D / 16;        // 16-dim steps of S
+  constexpr int ND = D / 32;        // 32-dim blocks of O^T
+  constexpr int CPR = D / 8;        // 16-byte chunks of a bf16 row in LDS
+  constexpr int TPR = D / 16;       // threads that stage a row
+  constexpr int NL = D / 64;        // 16-byte loads a thread: K and V (D = 128), or one of them (D = 64)
+  __shared__ __align__(16) uint16_t Ks[2][kBK * D];  // [key][chunk ^ key % CPR]
+  __shared__ __align__(16) uint16_t Vs[2][kBK * D];  // [key][chunk ^ vswz(key)]
+  __shared__ __align__(16) float Cs[2][12];          // of each 16 keys: c, v, 2^-v twice in bf16
+  __shared__ int nan_tile[2];                        // first key of the tile whose NaN codes of V were taken out
+
+  const int kvh = int(blockIdx.x % unsigned(a.c.Hkv));
+  const int rest = int(blockIdx.x / unsigned(a.c.Hkv));
+  const int split = rest % pl.nsplit;
+  QueryTile qt;
+  if (!find_tile<QT>(a, rest / pl.nsplit, qt)) return;
+  const int kend = qt.past + min(qt.qlen, qt.first + QT);  // keys [0, kend) serve this block
+  const int ntiles = (kend + kBK - 1) / kBK, per = split_tiles(ntiles, pl.nsplit);
+  const int tile0 = split * per, n = min(per, ntiles - tile0);
+  if (n <= 0) return;
+
+  const int tid = threadIdx.x, lane = tid & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int h = lane >> 5, j = lane & 31;
+  const int row = wave * 32 + j;
+  const int qi = min(qt.first + row / G, qt.qlen - 1);  // rows past the sequence compute, never store
+  const bool live = qt.first + row / G < qt.qlen;
+  const int hq = kvh * G + row % G;
+  const int qpos = qt.past + qi;
+  const int wave_q0 = qt.first + wave * 32 / G;
+  const bool wave_on = wave_q0 < qt.qlen;
+  const int wave_first = qt.past + wave_q0, wave_last = qt.past + min(qt.first + (wave * 32 + 31) / G, qt.qlen - 1);
+  const float sl2 = a.scale * kLog2e;
+
+  bf16x8_t qf[NS];
+  {
+    const uint16_t* qp = a.q + int64_t(qt.t0 + qi) * a.q_rs + int64_t(hq) * D + 8 * h;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) qf[s] = as_bf16x8(*reinterpret_cast<const uint4*>(qp + 16 * s));
+  }
+
+  // ---- staging: thread = (key sr of the tile, 16 dims from 16 sc on)
+  const int sid = NL == 2 ? tid : tid & (kBK * TPR - 1);
+  const int sr = sid / TPR, sc = sid % TPR;
+  const bool stage_v = NL == 1 && tid >= kBK * TPR;  // D = 64: the upper half of the block stages V
+  const bool stage_c = sr % 16 == 0 && sc == 0 && !stage_v;
+  const int32_t* table = a.table + int64_t(qt.b) * a.M;
+  const int pmask = (1 << a.c.page_sh) - 1;
+  auto key_row = [&](int t) { return min((tile0 + t) * kBK + sr, kend - 1); };
+  auto flat_row = [&](int r, int32_t id) {
+    const uint32_t page = min(uint32_t(id), uint32_t(a.c.num_pages - 1));
+    return ((int64_t(page) * a.c.Hkv + kvh) << a.c.page_sh) + (r & pmask);
+  };
+  uint4 raw[NL];
+  int ek = 0, ev = 0;
+  int32_t id = table[key_row(0) >> a.c.page_sh];
+  auto issue = [&](int t) {  // tile t's codes and exponents, and the page of tile t + 1
+    const int64_t at = flat_row(key_row(t), id);
+    if (NL == 2) {
+      raw[0] = *reinterpret_cast<const uint4*>(a.c.K + at * D + 16 * sc);
+      raw[NL - 1] = *reinterpret_cast<const uint4*>(a.c.V + at * D + 16 * sc);
+    } else {
+      raw[0] = *reinterpret_cast<const uint4*>((stage_v ? a.c.V : a.c.K) + at * D + 16 * sc);
+    }
+    if (stage_c) {
+      ek = a.c.Ks[at >> a.c.block_sh];
+      ev = a.c.Vs[at >> a.c.block_sh];
+    }
+    id = table[key_row(t + 1) >> a.c.page_sh];
+  };
+  auto vswz = [](int r) { return D == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); };
+  auto put = [&](uint16_t* dst, int swz, const uint4& v) {
+    const uint2 p0 = kv8_bf16x4<TYPE>(v.x), p1 = kv8_bf16x4<TYPE>(v.y), p2 = kv8_bf16x4<TYPE>(v.z), p3 = kv8_bf16x4<TYPE>(v.w);
+    *reinterpret_cast<uint4*>(dst + sr * D + ((2 * sc) ^ swz) * 8) = make_uint4(p0.x, p0.y, p1.x, p1.y);
+    *reinterpret_cast<uint4*>(dst + sr * D + ((2 * sc + 1) ^ swz) * 8) = make_uint4(p2.x, p2.y, p3.x, p3.y);
+  };
+  auto stage = [&](int t) {  // tile t from its registers into its buffer
+    const int buf = t & 1, k0 = (tile0 + t) * kBK;
+    if (TYPE == kKvE4m3 && k0 + kBK - 1 > qt.past + qt.first) {
+      // Some query of the block does not see some key of the tile: its weight of 0 must not
+      // meet a NaN.  The codes go, and fix_nan puts them back where they are seen.
+      if (NL == 2 || stage_v) {
+        uint4& v = raw[NL - 1];
+        if (has_nan_code(v.x) || has_nan_code(v.y) || has_nan_code(v.z) || has_nan_code(v.w)) {
+          v = make_uint4(without_nan(v.x), without_nan(v.y), without_nan(v.z), without_nan(v.w));
+          nan_tile[buf] = k0;
+        }
+      }
+    }
+    if (!stage_v) put(Ks[buf], sr % CPR, raw[0]);
+    if (NL == 2 || stage_v) put(Vs[buf], vswz(sr), raw[NL - 1]);
+    if (stage_c) {
+      const int k = kv8_exp(ek), v = kv8_exp(ev), u = sr / 16;
+      const bool nan = v == kKvNanExp;
+      Cs[buf][u] = sl2 * kv8_scale(k);
+      Cs[buf][4 + u] = nan ? __uint_as_float(0x7fc00000u) : float(v - 127);
+      Cs[buf][8 + u] = __uint_as_float(nan ? 0x3f803f80u : uint32_t(254 - v) << 7 | uint32_t(254 - v) << 23);
+    }
+  };
+  if (tid < 2) nan_tile[tid] = -1;
+  __syncthreads();
+  issue(0);
+  stage(0);
+  if (n > 1) issue(1);
+  __syncthreads();
+
+  // ---- operand addresses: K row 32 kk + j has the swizzle of row j; lane (i = 16 g1 + mm,
+  // half h) of the transposing reads takes key 4 h + mm / 4 (+ 8, + 16-key step), dims
+  // 32 d + 16 g1 + 4 (mm % 4) .. + 3.
+  int koff[NS], voff[ND];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) koff[s] = j * D + ((2 * s + h) ^ (j % CPR)) * 8;
+  {
+    const int mm = lane & 15, g1 = (lane >> 4) & 1, vrow = 4 * h + (mm >> 2);
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+      voff[d] = vrow * D + ((4 * d + 2 * g1 + ((mm & 3) >> 1)) ^ vswz(vrow)) * 8 + (mm & 1) * 4;
+  }
+
+  f32x16_t o[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+  float m = kLowest, l = 0.f;
+
+  auto compute = [&](int t) {
+    const int buf = t & 1, k0 = (tile0 + t) * kBK;
+    const bool edge = k0 + kBK - 1 > wave_first;  // some of the wave's queries do not see all of the tile
+    const uint16_t* ks = Ks[buf];
+    f32x16_t st[2];
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) st[kk][r] = 0.f;
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+        st[kk] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+            as_bf16x8(*reinterpret_cast<const uint4*>(ks + 32 * kk * D + koff[s])), qf[s], st[kk], 0, 0, 0);
+    // st[kk][r] = s' of (query j, key k0 + 32 kk + 8 (r / 4) + 4 h + r % 4); 16 keys u = 2 kk + r / 8 share a scale
+    float c[4], v[4], iv[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      c[u] = Cs[buf][u];
+      v[u] = Cs[buf][4 + u];
+      iv[u] = Cs[buf][8 + u];
+    }
+    if (edge) {
+      const int seen = qpos - k0;  // keys of the tile up to this one are seen
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {  // scales of keys that are not seen may be NaN
+        c[u] = 16 * u > seen ? 1.f : c[u];
+        v[u] = 16 * u > seen ? 0.f : v[u];
+      }
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (32 * kk + 8 * (r >> 2) + (r & 3) > seen - 4 * h) st[kk][r] = -INFINITY;
+    }
+    float mx = kLowest;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      float g = st[u >> 1][8 * (u & 1)];
+#pragma unroll
+      for (int r = 1; r < 8; ++r) g = fmaxf(g, st[u >> 1][8 * (u & 1) + r]);
+      mx = fmaxf(mx, g * c[u]);
+    }
+    mx = halves_max(mx);
+    // The reference m moves, and O and l are rescaled, only where a row's maximum passes
+    // it by more than kLazy: weights stay below 2^kLazy, exact in fp32 and of the same
+    // relative precision in bf16, and most tiles skip the rescale.
+    if (__builtin_amdgcn_ballot_w64(mx > m + kLazy)) {
+      const float mn = fmaxf(m, mx);
+      const float alpha = __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[d] *= alpha;
+    }
+    const uint16_t* vs = Vs[buf];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      // 16 keys: slots 8 h .. 8 h + 7 of the product are registers 8 (u % 2) .. + 7
+      uint32_t w[4];
+      const float off = v[u] - m;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(st[u >> 1][8 * (u & 1) + 2 * q], c[u], off));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(st[u >> 1][8 * (u & 1) + 2 * q + 1], c[u], off));
+        w[q] = cvt_bf2(p0, p1);
+        l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w[q]), __builtin_bit_cast(bf16x2_t, iv[u]), l, false);
+      }
+      const bf16x8_t pb = as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        const uint16_t* vp = vs + 16 * u * D + voff[d];
+        const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)vp);
+        const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(vp + 8 * D));
+        const bf16x8_t va = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, pb, o[d], 0, 0, 0);
+      }
+    }
+    if (TYPE == kKvE4m3 && nan_tile[buf] == k0) {  // corrupt rows only: NaN where a query sees one
+      for (int i = 0; i < kBK && k0 + i < kend; ++i) {
+        const int r = k0 + i;
+        const uint8_t* vr = a.c.V + flat_row(r, table[r >> a.c.page_sh]) * D + 4 * h;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const uint32_t x = *reinterpret_cast<const uint32_t*>(vr + 32 * d + 8 * q);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (r <= qpos && ((x >> (8 * e)) & 0x7f) == 0x7f) o[d][4 * q + e] = __uint_as_float(0x7fc00000u);
+          }
+      }
+    }
+  };
+
+  for (int t = 0; t < n; ++t) {
+    if (t + 1 < n) {
+      stage(t + 1);  // its buffer was read last before the barrier behind tile t - 1
+      if (t + 2 < n) issue(t + 2);
+    }
+    if (wave_on && (tile0 + t) * kBK <= wave_last) compute(t);
+    __syncthreads();
+  }
+
+  // ---- l: the two lane halves hold a share of query j's sum each
+  l = halves_sum(l);
+  if (!live) return;
+  if (pl.nsplit == 1) {
+    const float inv = 1.f / l;
+    uint16_t* op = a.out + (int64_t(qt.t0 + qi) * a.H + hq) * D + 4 * h;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)  // o[d][4q + e] = O^T[dim 32d + 8q + 4h + e][row j]
+        *reinterpret_cast<uint2*>(op + 32 * d + 8 * q) = make_uint2(cvt_bf2(o[d][4 * q] * inv, o[d][4 * q + 1] * inv),
+                                                                    cvt_bf2(o[d][4 * q + 2] * inv, o[d][4 * q + 3] * inv));
+  } else {
+    const int64_t at = (int64_t(split) * a.T + qt.t0 + qi) * a.H + hq;
+    float* op = pl.o + at * D + 4 * h;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<float4*>(op + 32 * d + 8 * q) =
+            make_float4(o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]);
+    if (h == 0) *reinterpret_cast<float2*>(pl.ml + at * 2) = make_float2(m, l);
+  }
+}
+
+// Joins the splits of one query tile's rows of a kv head: 4 dims a thread.
+template <int D, int G>
+__global__ __launch_bounds__(256) void quant_prefill_join_kernel(QuantAttnArgs a, SplitPlan pl) {
+  EZ_PROF_WAVE(kProfQuantAttnCombine);
+  constexpr int QT = kRows / G, TPR = D / 4, PER = 256 / TPR;  // rows a pass
+  const int parts = kRows / PER;
+  const int part = int(blockIdx.x) % parts, rest = int(blockIdx.x) / parts;
+  const int kvh = rest % a.c.Hkv;
+  QueryTile qt;
+  if (!find_tile<QT>(a, rest / a.c.Hkv, qt)) return;
+  const int row = part * PER + int(threadIdx.x) / TPR, d = int(threadIdx.x) % TPR * 4;
+  const int qi = qt.first + row / G;
+  if (qi >= qt.qlen) return;
+  const int kend = qt.past + min(qt.qlen, qt.first + QT), ntiles = (kend + kBK - 1) / kBK;
+  const int per = split_tiles(ntiles, pl.nsplit), used = (ntiles + per - 1) / per;
+  const int64_t at = int64_t(qt.t0 + qi) * a.H + kvh * G + row % G, step = a.T * a.H;
+  float m = kLowest;
+  for (int s = 0; s < used; ++s) m = fmaxf(m, pl.ml[(at + s * step) * 2]);
+  float o[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
+  for (int s = 0; s < used; ++s) {
+    const float2 x = *reinterpret_cast<const float2*>(pl.ml + (at + s * step) * 2);
+    const float4 p = *reinterpret_cast<const float4*>(pl.o + (at + s * step) * D + d);
+    const float f = __builtin_amdgcn_exp2f(x.x - m);
+    l = fmaf(f, x.y, l);
+    o[0] = fmaf(f, p.x, o[0]);
+    o[1] = fmaf(f, p.y, o[1]);
+    o[2] = fmaf(f, p.z, o[2]);
+    o[3] = fmaf(f, p.w, o[3]);
+  }
+  const float inv = 1.f / l;
+  *reinterpret_cast<uint2*>(a.out + at * D + d) = make_uint2(cvt_bf2(o[0] * inv, o[1] * inv), cvt_bf2(o[2] * inv, o[3] * inv));
+}
+
+// Query tiles at most (a sequence adds at most one that is not full), and the splits of
+// the keys: as many as give every CU a block, none below four tiles of 64 keys at full length.
+SplitPlan plan(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t kv_len) {
+  const int64_t qt = kRows / (H / Hkv);
+  const int64_t tiles = T / qt + (B < T ? B : T);
+  const int64_t blocks = tiles * Hkv, cus = num_cus();
+  int64_t ns = cus / blocks;
+  const int64_t most = kv_len / (4 * kBK);
+  ns = ns < most ? ns : most;
+  ns = ns < kMaxSplits ? ns : kMaxSplits;
+  return {int(ns < 1 ? 1 : ns), int(tiles), nullptr, nullptr};
+}
+int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
+
+}  // namespace
+}  // namespace ez
+
+extern "C" size_t ezops_quant_prefill_attn_workspace_size(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t D,
+                                                          int64_t kv_len) {
+  if (B < 1 || T < 1 || T >= (int64_t(1) << 30) || H < 1 || H > 4096 || Hkv < 1 || H % Hkv || H / Hkv > 16 || D < 1 || D > 128 ||
+      kv_len < 1)
+    return 0;
+  const ez::SplitPlan pl = ez::plan(B, T, H, Hkv, kv_len);
+  return pl.nsplit == 1 ? 0 : size_t(ez::up256(pl.nsplit * T * H * D * 4) + ez::up256(pl.nsplit * T * H * 8));
+}
+
+extern "C" int ezops_quant_prefill_attn_bf16(const void* q, int64_t q_stride, const void* K_cache, const void* V_cache,
+                                             const void* K_scale, const void* V_scale, int cache_type,
+                                             const int32_t* block_table, const int32_t* cu_seqlens, const int32_t* past_lens,
+                                             void* out, int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t D,
+                                             int64_t num_pages, int64_t page_size, int64_t max_pages, int64_t block_size,
+                                             int64_t max_kv_len, float scale, void* ws, size_t ws_bytes,
+                                             hipStream_t stream) {
+  const char* op = "quant_prefill_attn";
+  ez::QuantAttnArgs a{};
+  ez::fill_kv8(a.c, K_cache, V_cache, K_scale, V_scale, cache_type, num_pages, page_size, block_size, Hkv, D);
+  a.q = static_cast<const uint16_t*>(q); a.q_rs = q_stride;
+  a.out = static_cast<uint16_t*>(out);
+  a.table = block_table; a.cu = cu_seqlens; a.past = past_lens;
+  a.B = B; a.T = T; a.M = max_pages; a.H = int(H); a.scale = scale;
+  EZ_REQUIRE(cu_seqlens, "%s: null pointer", op);
+  const int rc = ez::check_attn8(op, a, page_size, block_size, H, max_kv_len);
+  if (rc != EZ_OK) return rc;
+  ez::finish_args(a, page_size, max_kv_len);
+ez::SplitPlan pl = ez::plan(B, T, H, Hkv, a.cap);
+  const int64_t blocks = int64_t(pl.tiles) * Hkv * pl.nsplit, joins = int64_t(pl.tiles) * Hkv * (ez::kRows * D / 1024);
+  EZ_REQUIRE(blocks < int64_t(1) << 23 && (pl.nsplit == 1 || joins < int64_t(1) << 24), "%s: tokens * heads past one launch", op);
+  if (pl.nsplit > 1) {
+    const size_t need = ezops_quant_prefill_attn_workspace_size(B, T, H, Hkv, D, a.cap);
+    EZ_REQUIRE(ws && ws_bytes >= need, "%s: workspace too small (%zu < %zu)", op, ws_bytes, need);
+    EZ_REQUIRE(ez::kv8_aligned16(ws), "%s: workspace must be 16-byte aligned", op);
+    for (const auto& x : ez::attn8_tensors(a, H))
+      EZ_REQUIRE(!ez::overlap(ws, int64_t(need), x.p, x.n), "%s: workspace overlaps a tensor", op);
+    pl.o = static_cast<float*>(ws);
+    pl.ml = reinterpret_cast<float*>(static_cast<char*>(ws) + ez::up256(pl.nsplit * T * H * D * 4));
+  }
+#define EZ_GROUP(DD, TY, GG)                                                                                              \
+  do {                                                                                                                    \
+    hipLaunchKernelGGL((ez::quant_prefill_kernel<DD, TY, GG>), dim3(unsigned(blocks)), dim3(ez::kW * ez::kWave), 0, stream, \
+                       a, pl);                                                                                            \
+    if (pl.nsplit > 1)                                                                                                    \
+      hipLaunchKernelGGL((ez::quant_prefill_join_kernel<DD, GG>), dim3(unsigned(joins)), dim3(256), 0, stream, a, pl);    \
+  } while (0)
+#define EZ_GO(DD, TY)                       \
+  do {                                      \
+    switch (H / Hkv) {                      \
+      case 1: EZ_GROUP(DD, TY, 1); break;   \
+      case 2: EZ_GROUP(DD, TY, 2); break;   \
+      case 4: EZ_GROUP(DD, TY, 4); break;   \
+      case 8: EZ_GROUP(DD, TY, 8); break;   \
+      default: EZ_GROUP(DD, TY, 16); break; \
+    }                                       \
+  } while (0)
+  EZ_KV8_DISPATCH(EZ_GO);
+#undef EZ_GO
+#undef EZ_GROUP
+  return ez::launch_status(op);
+}

@@ -8,7 +8,8 @@ Codes live in pools ``K_cache`` / ``V_cache`` ``[num_pages, Hkv, page_size, D]``
 ``int8`` or ``float8_e4m3fn``; ``K_scale`` / ``V_scale``
 ``[num_pages, Hkv, page_size / block_size]`` (uint8) hold one exponent for each block of
 ``block_size`` rows of a page and kv head: a row stands for ``code * 2^(e - 127)``, all
-NaN where e = 255 (the encoding of ``torch.float8_e8m0fnu``).  With TOP = 127 (int8) or
+NaN where e = 255 (the encoding of ``torch.float8_e8m0fnu``; an exponent outside [67, 187]
+is read as the nearer of the two).  With TOP = 127 (int8) or
 448 (e4m3)
 
     need = least e with max|x| <= TOP * 2^(e - 127) over the rows a block gets in a call, in [67, 187]
@@ -70,10 +71,16 @@ def alloc_pools(num_pages, num_kv_heads, page_size, head_dim, block_size, cache_
     return make(codes, cache_dtype), make(codes, cache_dtype), make(scales, torch.uint8), make(scales, torch.uint8)
 
 
-def exp2_of(e):
-    """2^(e - 127) in fp32, from the bits: 255 is NaN, 0 and below zero."""
+def read_exp(e):
+    """Exponents as they are read: 255 as it is, others within [67, 187]."""
     e = e.to(torch.int32)
-    return torch.where(e == NAN_EXP, torch.nan, (e.clamp(0, 254) << 23).view(torch.float32))
+    return torch.where(e == NAN_EXP, e, e.clamp(LOW_EXP, HIGH_EXP))
+
+
+def exp2_of(e):
+    """2^(e - 127) in fp32, from the bits; 255 is NaN."""
+    e = e.to(torch.int32)
+    return torch.where(e == NAN_EXP, torch.nan, (e.clamp(1, 254) << 23).view(torch.float32))
 
 
 def needed_exponent(amax, cache_dtype):
@@ -98,7 +105,7 @@ def read_rows(cache, scale, slots, block_size):
     P = cache.shape[2]
     page, row = slots // P, slots % P
     codes = cache.view(torch.uint8)[page, :, row].view(cache.dtype).float()
-    return codes * exp2_of(scale[page, :, row // block_size])[..., None]
+    return codes * exp2_of(read_exp(scale[page, :, row // block_size]))[..., None]
 
 
 def random_cache(num_pages, num_kv_heads, page_size, head_dim, block_size, cache_dtype, device):
@@ -207,15 +214,14 @@ class KvCacheQuantOp(_CacheRowsOp):
         e = needed_exponent(torch.where(finite, x.abs(), 0.0).amax((0, 2)), dt)
         if dt == torch.int8:
             e = torch.where(finite.all(2).all(0), e, NAN_EXP)
-        old = scale.to(torch.int32) if off else torch.zeros_like(e)
+        old = read_exp(scale) if off else torch.zeros_like(e)
         e = torch.maximum(e, old)
         if off:
             held = rows[:, :off].view(dt).float()
-            factor = torch.where(e == NAN_EXP, 0.0, exp2_of((127 + old - e).clamp(0, 254)))
+            factor = torch.where(e == NAN_EXP, 0.0, exp2_of(127 + old - e))
             turned = to_codes(held * factor[:, None, None], dt)
             rows[:, :off] = torch.where((e > old)[:, None, None], turned, rows[:, :off])
-        inv = exp2_of((254 - e).clamp(0, 254))
-        y = x * inv[None, :, None]
+        y = x * torch.where(e == NAN_EXP, 0.0, exp2_of(254 - e))[None, :, None]
         if dt == torch.int8:
             y = torch.where((e == NAN_EXP)[None, :, None], 0.0, y)
         rows[:, off:off + n] = to_codes(y, dt).transpose(0, 1)

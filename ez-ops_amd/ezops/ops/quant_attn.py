@@ -20,7 +20,7 @@ import torch
 
 from ..registry import get_kernel
 from .base_op import Op, default_device, randn
-from .kv_cache_quant import check_cache, exp2_of, random_cache
+from .kv_cache_quant import check_cache, exp2_of, random_cache, read_exp
 from .linear_attn import GROUPS, _scale
 from .utils.roofline import RooflineResult
 
@@ -28,7 +28,7 @@ from .utils.roofline import RooflineResult
 def cache_rows(cache, scale, table, block_size):
     """Rows of the pages of ``table`` [n] in fp32: [Hkv, n * page_size, D]."""
     x = cache.view(torch.uint8)[table].view(cache.dtype).float()
-    x = x * exp2_of(scale[table]).repeat_interleave(block_size, -1)[..., None]
+    x = x * exp2_of(read_exp(scale[table])).repeat_interleave(block_size, -1)[..., None]
     return x.transpose(0, 1).flatten(1, 2)
 
 

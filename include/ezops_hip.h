@@ -298,7 +298,8 @@ int ezops_linear_attn_decode_bf16(const void* q, int64_t q_stride, const void* k
 
 /* KV cache held in 8 bits: codes [num_pages, Hkv, page_size, D] (cache_type 0 = int8,
  * 1 = OCP e4m3) and exponents [num_pages, Hkv, page_size / block_size] of one byte, a row
- * standing for code * 2^(e - 127), NaN where e = 255.
+ * standing for code * 2^(e - 127), NaN where e = 255; an e outside [67, 187] is read as the
+ * nearer of the two.
  * Quantise k / v [T, Hkv, D] bf16 (token strides in elements, multiples of 8) into slots
  * slot_mapping[t] = page * page_size + offset; slots outside the pool are skipped.  Over
  * the tokens that a block of block_size rows gets in this call, need = the least e in

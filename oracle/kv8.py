@@ -48,8 +48,13 @@ def encode(y, kind):
     return np.where(np.isfinite(y), code, 127).astype(np.uint8)
 
 
+def clamped(e):
+    """An exponent as it is read: 255, or within [67, 187]."""
+    return 255 if e == 255 else min(max(int(e), 67), 187)
+
+
 def decode(codes, e, kind):
-    return VALUES[kind][codes] * (math.nan if e == 255 else 2.0 ** (int(e) - 127) if e else 0.0)
+    return VALUES[kind][codes] * (math.nan if e == 255 else 2.0 ** (clamped(e) - 127))
 
 
 def write(x, cache, scale, slots, block, kind):
@@ -69,14 +74,14 @@ def write(x, cache, scale, slots, block, kind):
                 e = need(np.abs(np.where(fine, new, 0)).max(), kind)
                 if kind == "int8" and not fine.all():
                     e = 255
-                old = int(scale[page, h, row // block]) if off else 0
+                old = clamped(scale[page, h, row // block]) if off else 0
                 e = max(e, old)
                 first = row - off
                 if off and e > old:
                     held = VALUES[kind][cache[page, h, first:row]]
-                    f = 0.0 if e == 255 or 127 + old - e <= 0 else 2.0 ** (old - e)
+                    f = 0.0 if e == 255 else 2.0 ** (old - e)
                     cache[page, h, first:row] = encode(held * f, kind)
-                y = new * (0.0 if e >= 254 else 2.0 ** (127 - e)) if e != 255 or kind == "e4m3" else np.zeros_like(new)
+                y = new * (0.0 if e == 255 else 2.0 ** (127 - e)) if e != 255 or kind == "e4m3" else np.zeros_like(new)
                 cache[page, h, row:row + n] = encode(y, kind)
                 scale[page, h, row // block] = e
         t += n
