@@ -1,13 +1,31 @@
-// Attention over the 8-bit KV cache: one token per sequence (decode) and packed
-// prompts or chunks, causal (prefill).
+// Attention of one token per sequence over the 8-bit KV cache.
 //
-//   s_j = scale * q . (kc_j 2^(ek - 127)),  o = sum_j softmax(s)_j vc_j 2^(ev - 127)
+//   s_j = scale * q . kc_j 2^(ek - 127),  o = sum_j softmax(s)_j vc_j 2^(ev - 127)
 //
-// over the rows j that the query sees, in fp32.
+// kc, vc are the codes, ek, ev the exponents of the row's block (at least 16 rows each).
+// The work is reading the codes once: 2 D bytes a row and kv head.
+//
+// A sequence is cut into chunks of rows; a block of 4 waves takes one chunk of one kv
+// head for all G query heads of the group, so the codes cross memory once a group.
+// Chunks are counted over the sequences' lengths on the device (block -> sequence, chunk
+// by a wave scan), so a ragged batch is shared out by rows.  A wave's tiles of 32 rows
+// lie 4 tiles apart.  Per tile:
+//   * codes by 16-byte loads of whole rows, one tile ahead in registers, through the
+//     wave's own LDS slab still in 8 bits
+//   * S^T = K Q^T on v_mfma_f32_16x16x32_bf16: 16 rows of K (16 bytes of LDS a lane are two
+//     operands, widened to bf16 in registers: int8 and e4m3 are exact there) against the
+//     query heads, padded to 16 columns
+//   * softmax in the exp2 domain, one head a lane column, scales as in the exponent:
+//     w = 2^(c s' - m + v), c = scale log2(e) 2^(ek - 127), v = ev - 127: the weight times
+//     the scale of v; l += w 2^-v
+//   * O^T += V^T W^T, V^T by transposing 8-bit LDS reads (ds_read_b64_tr_b8) and widened
+//     behind them; w as two bf16 parts, so that weights carry 16 significant bits
+// The waves join (m, l, O) through LDS; a sequence of more than one chunk leaves fp32
+// partials, which a second kernel joins.
 #include "common.h"
 #include "internal.h"
-#include "quant_attn.h"
 #include "prof.h"
+#include "quant_attn.h"
 #include "status.h"
 #include "../../include/ezops_hip.h"
 
@@ -16,69 +34,347 @@ namespace ez {
 EZ_PROF_DEFINE(quantdecode)
 namespace {
 
-__device__ __forceinline__ int64_t cache_at(const QuantAttnArgs& a, int64_t b, int h, int64_t row) {
-  const uint32_t id = min(uint32_t(a.table[b * a.M + (row >> a.c.page_sh)]), uint32_t(a.c.num_pages - 1));
-  return ((int64_t(id) * a.c.Hkv + h) << a.c.page_sh) + (row & ((int64_t(1) << a.c.page_sh) - 1));
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLowest = -3e38f;  // reference before any row: finite, so that differences are
+constexpr int kW = 4;              // waves of a block
+constexpr int kT = 32;             // rows of a wave's tile
+constexpr int kMaxSplits = 64;
+
+struct SplitPlan {
+  int chunk;   // rows of a block, a multiple of kW * kT
+  int nsplit;  // chunks of the longest sequence
+  float* o;    // partials [B * H][nsplit][D]
+  float* ml;   // [B * H][nsplit][2]
+};
+
+__device__ __forceinline__ int seq_len(const QuantAttnArgs& a, int b) { return min(max(a.kv_lens[b], 0), int(a.cap)); }
+__device__ __forceinline__ int chunks(int len, int chunk) { return len > chunk ? (len + chunk - 1) / chunk : 1; }
+
+// Sequence and chunk of the idx-th block of a kv head; false behind the last one.  A
+// sequence without rows has one (which writes its zeros).  256 lengths a step.
+__device__ __forceinline__ bool find_chunk(const QuantAttnArgs& a, int chunk, int idx, int& b, int& split, int& len) {
+  const int lane = threadIdx.x & (kWave - 1), B = int(a.B);
+  for (int b0 = 0; b0 < B; b0 += 4 * kWave) {
+    int n[4], L[4], sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int s = b0 + 4 * lane + i;
+      L[i] = s < B ? seq_len(a, s) : 0;
+      n[i] = s < B ? chunks(L[i], chunk) : 0;
+      sum += n[i];
+    }
+    const int end = wave_scan(sum);
+    const uint64_t hit = __ballot(idx < end);
+    if (hit) {
+      const int l = __ffsll(static_cast<unsigned long long>(hit)) - 1;
+      int at = idx - (__builtin_amdgcn_readlane(end, l) - __builtin_amdgcn_readlane(sum, l));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int ni = __builtin_amdgcn_readlane(n[i], l);
+        if (at >= 0 && at < ni) {
+          b = b0 + 4 * l + i;
+          split = at;
+          len = __builtin_amdgcn_readlane(L[i], l);
+        }
+        at -= ni;
+      }
+      return true;
+    }
+    idx -= __builtin_amdgcn_readlane(end, kWave - 1);
+  }
+  return false;
 }
 
-// One block per (query row, head): its waves take every fourth cache row.
-template <int D, int TYPE>
-__device__ void attend(const QuantAttnArgs& a, int64_t b, int64_t t, int hq, int64_t L) {
-  constexpr int E = D / kWave;
-  __shared__ float Os[4][D], Ms[4], Ls[4];
-  const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x >> 6;
-  const int h = hq / (a.H / a.c.Hkv);
-  float q[E], o[E] = {}, m = -INFINITY, l = 0.f;
-  for (int e = 0; e < E; ++e) q[e] = bf2f(a.q[t * a.q_rs + int64_t(hq) * D + lane * E + e]);
-  for (int64_t j = w; j < L; j += 4) {
-    const int64_t at = cache_at(a, b, h, j);
-    float k[4], v[4], s = 0.f;
-    uint32_t kw = 0, vw = 0;
-    for (int e = 0; e < E; ++e) {
-      kw |= uint32_t(a.c.K[at * D + lane * E + e]) << (8 * e);
-      vw |= uint32_t(a.c.V[at * D + lane * E + e]) << (8 * e);
-    }
-    kv8_f32x4<TYPE>(kw, k);
-    kv8_f32x4<TYPE>(vw, v);
-    for (int e = 0; e < E; ++e) s += q[e] * k[e];
-    s = wave_sum(s) * kv8_scale(a.c.Ks[at >> a.c.block_sh]) * a.scale;
-    const float mn = fmaxf(m, s), al = m == -INFINITY ? 0.f : expf(m - mn), p = expf(s - mn);
-    const float vs = kv8_scale(a.c.Vs[at >> a.c.block_sh]);
-    l = l * al + p;
-    for (int e = 0; e < E; ++e) o[e] = o[e] * al + p * vs * v[e];
-    m = mn;
+template <int D, int TYPE, int G>
+__global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(3))) void quant_decode_kernel(QuantAttnArgs a,
+                                                                                                         SplitPlan pl) {
+  EZ_PROF_WAVE(kProfQuantAttnDecode);
+  constexpr int CPR = D / 16;            // 16-byte chunks of a row of codes
+  constexpr int RPL = kWave / CPR;       // rows of a load
+  constexpr int NL = kT / RPL;           // loads of a tile
+  constexpr int NX = D / 64;             // 16-byte operand pairs of a K row a lane
+  constexpr int NDB = D / 16;            // 16-dim blocks of O^T
+  struct Slabs {
+    uint8_t K[kW][kT * D], V[kW][kT * D];  // [row][chunk ^ kswz(row)], [row][chunk ^ vswz(row)]
+  };
+  struct Joined {
+    float O[kW][G][D], M[kW][G], L[kW][G];
+  };
+  __shared__ __align__(16) union {
+    Slabs s;
+    Joined j;
+  } lds;
+  // Chunk swizzles: 8 lanes that read one chunk of 8 rows (K), 16 lanes that read 16 bytes
+  // of 8 rows (V), meet every bank once.
+  auto kswz = [](int r) { return D == 128 ? r & 7 : (r >> 2) & 3; };
+  auto vswz = [](int r) { return D == 128 ? ((r >> 1) & 1) | ((r >> 4) & 1) << 1 : (r >> 4) & 1; };
+
+  const int kvh = int(blockIdx.x % unsigned(a.c.Hkv)), idx = int(blockIdx.x / unsigned(a.c.Hkv));
+  int b = idx, split = 0, L = 0;
+  if (pl.nsplit == 1) L = seq_len(a, b);
+  else if (!find_chunk(a, pl.chunk, idx, b, split, L)) return;
+  b = __builtin_amdgcn_readfirstlane(b);
+  split = __builtin_amdgcn_readfirstlane(split);
+  L = __builtin_amdgcn_readfirstlane(L);
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int li = lane & 15, lg = lane >> 4;
+  const int h0 = kvh * G;
+  if (L == 0) {
+    for (int i = threadIdx.x; i < G * D / 8; i += kW * kWave)
+      *reinterpret_cast<uint4*>(a.out + (int64_t(b) * a.H + h0) * D + i * 8) = make_uint4(0, 0, 0, 0);
+    return;
   }
-  for (int e = 0; e < E; ++e) Os[w][lane * E + e] = o[e];
-  if (lane == 0) {
-    Ms[w] = m;
-    Ls[w] = l;
+  const int r0 = split * pl.chunk, r1 = min(L, r0 + pl.chunk), last = r1 - 1;
+
+  // ---- loads of a tile: its page id one tile ahead (a vector load, so that it is waited
+  // for in order with the codes), then codes and exponents
+  const int32_t* table = a.table + int64_t(b) * a.M;
+  const int pmask = (1 << a.c.page_sh) - 1;
+  int lane0;
+  asm volatile("v_mov_b32 %0, 0" : "=v"(lane0));
+  auto start = [&](int t) { return t <= last ? t : last & ~(kT - 1); };  // tiles behind the end: the last one again
+  auto page_id = [&](int t) { return table[(start(t) >> a.c.page_sh) + lane0]; };
+  auto flat_row = [&](int t, int32_t id) {
+    const uint32_t page = min(uint32_t(__builtin_amdgcn_readfirstlane(id)), uint32_t(a.c.num_pages - 1));
+    return ((int64_t(page) * a.c.Hkv + kvh) << a.c.page_sh) + (start(t) & pmask);
+  };
+  uint4 kn[NL], vn[NL];
+  int en;  // lanes 0, 1: exponents of the tile's two halves of K; 2, 3: of V
+  auto load_k = [&](int t, int64_t at) {
+    const int rows = last - start(t);
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int p = i * RPL + lane / CPR;
+      kn[i] = ld16_stream(a.c.K + (at + min(p, rows)) * D + ((lane % CPR) ^ kswz(p)) * 16);
+    }
+    en = ((lane & 2) ? a.c.Vs : a.c.Ks)[(at + 16 * (lane & 1)) >> a.c.block_sh];
+  };
+  auto load_v = [&](int t, int64_t at) {
+    const int rows = last - start(t);
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int p = i * RPL + lane / CPR;
+      vn[i] = ld16_stream(a.c.V + (at + min(p, rows)) * D + ((lane % CPR) ^ vswz(p)) * 16);
+    }
+  };
+  int t0 = r0 + wave * kT;
+  int64_t at = flat_row(t0, page_id(t0));
+  load_k(t0, at);
+  load_v(t0, at);
+  int32_t id = page_id(t0 + kW * kT);
+
+  // Q operand of the pair (x, half): k-slot 8 lg + e is dim 64 x + 16 lg + 8 half + e, as K has it
+  bf16x8_t qf[NX][2];
+  {
+    const uint16_t* qp = a.q + int64_t(b) * a.q_rs + int64_t(h0 + min(li, G - 1)) * D + 16 * lg;
+#pragma unroll
+    for (int x = 0; x < NX; ++x)
+#pragma unroll
+      for (int f = 0; f < 2; ++f) {
+        const uint4 v = *reinterpret_cast<const uint4*>(qp + 64 * x + 8 * f);
+        qf[x][f] = as_bf16x8(li < G ? v : make_uint4(0, 0, 0, 0));
+      }
+  }
+  uint8_t* ks = lds.s.K[wave];
+  uint8_t* vs = lds.s.V[wave];
+  int koff[NX], voff[NDB];
+#pragma unroll
+  for (int x = 0; x < NX; ++x) koff[x] = li * D + (((4 * x + lg) ^ kswz(li)) * 16);
+  static_assert(kT == 32, "the swizzle of K row 16 + li is that of li");
+  {
+    const int i = li >> 1, row = 4 * lg + (i & 3) + 16 * (i >> 2);
+#pragma unroll
+    for (int d = 0; d < NDB; ++d) voff[d] = row * D + ((d ^ vswz(row)) * 16) + 8 * (li & 1);
+  }
+  const float sl2 = a.scale * kLog2e;
+
+  // Lane (li, lg): head li's reference m, its share of the sum, O^T[16 d + 4 lg + r][li] in o[d][r]
+  float m = kLowest, l = 0.f;
+  f32x4_t o[NDB];
+#pragma unroll
+  for (int d = 0; d < NDB; ++d) o[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+  for (; t0 < r1; t0 += kW * kT) {
+    const int tn = t0 + kW * kT;
+    const bool tail = t0 + kT > r1;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) *reinterpret_cast<uint4*>(ks + (i * kWave + lane) * 16) = kn[i];
+    const int e = kv8_exp(en);
+    const float cv = lane & 2 ? (e == kKvNanExp ? __uint_as_float(0x7fc00000u) : float(e - 127)) : sl2 * kv8_scale(e);
+    const int iv = e == kKvNanExp ? 127 : 254 - e;
+    at = flat_row(tn, id);
+    load_k(tn, at);
+    id = page_id(tn + kW * kT);
+    f32x4_t s[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      s[u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int x = 0; x < NX; ++x) {
+        const uint4 k = *reinterpret_cast<const uint4*>(ks + 16 * u * D + koff[x]);
+        const uint2 w0 = kv8_bf16x4<TYPE>(k.x), w1 = kv8_bf16x4<TYPE>(k.y), w2 = kv8_bf16x4<TYPE>(k.z), w3 = kv8_bf16x4<TYPE>(k.w);
+        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(make_uint4(w0.x, w0.y, w1.x, w1.y)), qf[x][0], s[u], 0, 0, 0);
+        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(make_uint4(w2.x, w2.y, w3.x, w3.y)), qf[x][1], s[u], 0, 0, 0);
+      }
+    }
+    // s[u][r] = s' of (head li, row t0 + 16 u + 4 lg + r)
+    float c[2], v[2], inv[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      c[u] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(cv), u));
+      v[u] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(cv), 2 + u));
+      inv[u] = __int_as_float(__builtin_amdgcn_readlane(iv, 2 + u) << 23);
+    }
+    if (tail) {
+      if (t0 + 16 >= r1) c[1] = 1.f, v[1] = 0.f;  // no row of this half: its exponents may be anything
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (t0 + 16 * u + 4 * lg + r >= r1) s[u][r] = -INFINITY;
+    }
+    float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])) * c[0],
+                     fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])) * c[1]);
+    mx = colgroup_max(mx);
+    if (__builtin_amdgcn_ballot_w64(mx > m)) {  // rescale only where a reference moves
+      const float mn = fmaxf(m, mx);
+      const float alpha = __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < NDB; ++d) o[d] *= alpha;
+    }
+    // W^T operand: k-slot 8 lg + e is row 16 (e / 4) + 4 lg + e % 4, w = hi + lo in bf16
+    uint32_t wh[4], wl[4];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const float off = v[u] - m;
+      float sum = 0.f;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[u][2 * q], c[u], off));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[u][2 * q + 1], c[u], off));
+        wh[2 * u + q] = cvt_bf2(p0, p1);
+        wl[2 * u + q] = cvt_bf2(p0 - bf_lo(wh[2 * u + q]), p1 - bf_hi(wh[2 * u + q]));
+        sum += p0 + p1;
+      }
+      l = fmaf(sum, inv[u], l);
+    }
+    const bf16x8_t ph = as_bf16x8(make_uint4(wh[0], wh[1], wh[2], wh[3]));
+    const bf16x8_t pw = as_bf16x8(make_uint4(wl[0], wl[1], wl[2], wl[3]));
+
+    if (tail) {  // rows behind the end weigh 0, but 0 * NaN would not: they are zeros
+#pragma unroll
+      for (int i = 0; i < NL; ++i)
+        if (t0 + i * RPL + lane / CPR >= r1) vn[i] = make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < NL; ++i) *reinterpret_cast<uint4*>(vs + (i * kWave + lane) * 16) = vn[i];
+    load_v(tn, at);
+#pragma unroll
+    for (int d = 0; d < NDB; ++d) {
+      typedef int i32x2_t __attribute__((ext_vector_type(2)));
+      const i32x2_t x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2_t*)(vs + voff[d]));
+      const uint2 w0 = kv8_bf16x4<TYPE>(uint32_t(x[0])), w1 = kv8_bf16x4<TYPE>(uint32_t(x[1]));
+      const bf16x8_t va = as_bf16x8(make_uint4(w0.x, w0.y, w1.x, w1.y));
+      o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, ph, o[d], 0, 0, 0);
+      o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pw, o[d], 0, 0, 0);
+    }
+  }
+
+  // ---- join the waves: each writes (m, l, O), then a thread takes 4 dims of a head
+  l = rowgroup_sum<16>(l);
+  __syncthreads();  // the slabs are read no more
+  if (li < G) {
+#pragma unroll
+    for (int d = 0; d < NDB; ++d)
+      *reinterpret_cast<float4*>(&lds.j.O[wave][li][16 * d + 4 * lg]) = make_float4(o[d][0], o[d][1], o[d][2], o[d][3]);
+    if (lg == 0) {
+      lds.j.M[wave][li] = m;
+      lds.j.L[wave][li] = l;
+    }
   }
   __syncthreads();
-  if (threadIdx.x < D) {
-    const float M = fmaxf(fmaxf(Ms[0], Ms[1]), fmaxf(Ms[2], Ms[3]));
-    float ov = 0.f, lv = 0.f;
-    for (int i = 0; i < 4; ++i) {
-      const float f = Ms[i] == -INFINITY && Ls[i] == 0.f ? 0.f : expf(Ms[i] - M);
-      ov += f * Os[i][threadIdx.x];
-      lv += f * Ls[i];
+  const bool whole = L <= pl.chunk;
+  for (int i = threadIdx.x; i < G * D / 4; i += kW * kWave) {
+    const int h = i / (D / 4), d = i % (D / 4) * 4;
+    float M = kLowest;
+#pragma unroll
+    for (int w = 0; w < kW; ++w) M = fmaxf(M, lds.j.M[w][h]);
+    float ov[4] = {0.f, 0.f, 0.f, 0.f}, lv = 0.f;
+#pragma unroll
+    for (int w = 0; w < kW; ++w) {
+      const float f = __builtin_amdgcn_exp2f(lds.j.M[w][h] - M);
+      lv = fmaf(f, lds.j.L[w][h], lv);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) ov[k] = fmaf(f, lds.j.O[w][h][d + k], ov[k]);
     }
-    a.out[(t * a.H + hq) * D + threadIdx.x] = f2bf(L > 0 ? ov / lv : 0.f);
+    const int64_t hq = int64_t(b) * a.H + h0 + h;
+    if (whole) {
+      const float r = 1.f / lv;
+      *reinterpret_cast<uint2*>(a.out + hq * D + d) = make_uint2(cvt_bf2(ov[0] * r, ov[1] * r), cvt_bf2(ov[2] * r, ov[3] * r));
+    } else {
+      *reinterpret_cast<float4*>(pl.o + (hq * pl.nsplit + split) * D + d) = make_float4(ov[0], ov[1], ov[2], ov[3]);
+      if (d == 0) *reinterpret_cast<float2*>(pl.ml + (hq * pl.nsplit + split) * 2) = make_float2(M, lv);
+    }
   }
 }
 
-template <int D, int TYPE>
-__global__ __launch_bounds__(256) void quant_decode_kernel(QuantAttnArgs a) {
-  EZ_PROF_WAVE(kProfQuantAttnDecode);
-  const int64_t b = blockIdx.x / a.H;
-  attend<D, TYPE>(a, b, b, int(blockIdx.x % a.H), min(max(int64_t(a.kv_lens[b]), int64_t(0)), a.cap));
+// Joins the chunks of a (sequence, query head): 4 dims a thread.  Sequences of one chunk
+// are written already.
+template <int D>
+__global__ __launch_bounds__(256) void quant_decode_join_kernel(QuantAttnArgs a, SplitPlan pl) {
+  EZ_PROF_WAVE(kProfQuantAttnCombine);
+  constexpr int TPR = D / 4;
+  const int64_t hq = int64_t(blockIdx.x) * (256 / TPR) + threadIdx.x / TPR;
+  if (hq >= a.B * a.H) return;
+  const int L = seq_len(a, int(hq / a.H)), d = int(threadIdx.x) % TPR * 4;
+  if (L <= pl.chunk) return;
+  const int n = chunks(L, pl.chunk);
+  const float2* ml = reinterpret_cast<const float2*>(pl.ml) + hq * pl.nsplit;
+  const float4* op = reinterpret_cast<const float4*>(pl.o + hq * pl.nsplit * D + d);
+  float m = kLowest;
+  for (int s = 0; s < n; ++s) m = fmaxf(m, ml[s].x);
+  float o[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
+#pragma unroll 8
+  for (int s = 0; s < n; ++s) {
+    const float2 x = ml[s];
+    const float4 p = op[s * (D / 4)];
+    const float f = __builtin_amdgcn_exp2f(x.x - m);
+    l = fmaf(f, x.y, l);
+    o[0] = fmaf(f, p.x, o[0]);
+    o[1] = fmaf(f, p.y, o[1]);
+    o[2] = fmaf(f, p.z, o[2]);
+    o[3] = fmaf(f, p.w, o[3]);
+  }
+  const float r = 1.f / l;
+  *reinterpret_cast<uint2*>(a.out + hq * D + d) = make_uint2(cvt_bf2(o[0] * r, o[1] * r), cvt_bf2(o[2] * r, o[3] * r));
 }
+
+// Chunks: enough blocks for every CU to hold its fill at the longest length, none below a
+// tile a wave.
+SplitPlan plan(int64_t B, int64_t Hkv, int64_t kv_len) {
+  const int64_t unit = kW * kT, cus = num_cus();
+  int64_t ns = (4 * cus + B * Hkv - 1) / (B * Hkv);
+  const int64_t most = (kv_len + unit - 1) / unit;
+  ns = ns < most ? ns : most;
+  ns = ns < kMaxSplits ? ns : kMaxSplits;
+  const int64_t chunk = ((kv_len + ns - 1) / ns + unit - 1) / unit * unit;
+  return {int(chunk), int((kv_len + chunk - 1) / chunk), nullptr, nullptr};
+}
+int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
 
 }  // namespace
 }  // namespace ez
 
 extern "C" size_t ezops_quant_paged_attn_decode_workspace_size(int64_t B, int64_t H, int64_t Hkv, int64_t D,
                                                                int64_t kv_len) {
-  return 0;
+  if (B < 1 || B > 65536 || H < 1 || H > 4096 || Hkv < 1 || H % Hkv || D < 1 || D > 128 || kv_len < 1 ||
+      kv_len > (int64_t(1) << 30))
+    return 0;
+  const ez::SplitPlan pl = ez::plan(B, Hkv, kv_len);
+  return pl.nsplit == 1 ? 0 : size_t(ez::up256(B * H * pl.nsplit * D * 4) + ez::up256(B * H * pl.nsplit * 8));
 }
 
 extern "C" int ezops_quant_paged_attn_decode_bf16(const void* q, int64_t q_stride, const void* K_cache, const void* V_cache,
@@ -97,10 +393,35 @@ extern "C" int ezops_quant_paged_attn_decode_bf16(const void* q, int64_t q_strid
   EZ_REQUIRE(kv_lens, "%s: null pointer", op);
   const int rc = ez::check_attn8(op, a, page_size, block_size, H, max_kv_len);
   if (rc != EZ_OK) return rc;
-  EZ_REQUIRE(B * H < int64_t(1) << 24, "%s: batch * heads past one launch", op);
   ez::finish_args(a, page_size, max_kv_len);
-#define EZ_GO(DD, TY) hipLaunchKernelGGL((ez::quant_decode_kernel<DD, TY>), dim3(unsigned(B * H)), dim3(256), 0, stream, a)
+  ez::SplitPlan pl = ez::plan(B, Hkv, a.cap);
+  const int64_t blocks = B * Hkv * pl.nsplit, joins = (B * H * (D / 4) + 255) / 256;
+  EZ_REQUIRE(blocks < int64_t(1) << 24, "%s: batch * heads past one launch", op);
+  if (pl.nsplit > 1) {
+    const size_t need = ezops_quant_paged_attn_decode_workspace_size(B, H, Hkv, D, a.cap);
+    EZ_REQUIRE(ws && ws_bytes >= need, "%s: workspace too small (%zu < %zu)", op, ws_bytes, need);
+    EZ_REQUIRE(ez::kv8_aligned16(ws), "%s: workspace must be 16-byte aligned", op);
+    for (const auto& x : ez::attn8_tensors(a, H))
+      EZ_REQUIRE(!ez::overlap(ws, int64_t(need), x.p, x.n), "%s: workspace overlaps a tensor", op);
+    pl.o = static_cast<float*>(ws);
+    pl.ml = reinterpret_cast<float*>(static_cast<char*>(ws) + ez::up256(B * H * pl.nsplit * D * 4));
+  }
+#define EZ_GROUP(DD, TY, GG)                                                                                                  \
+  hipLaunchKernelGGL((ez::quant_decode_kernel<DD, TY, GG>), dim3(unsigned(blocks)), dim3(ez::kW * ez::kWave), 0, stream, a, pl)
+#define EZ_GO(DD, TY)                                                                                                         \
+  do {                                                                                                                        \
+    switch (H / Hkv) {                                                                                                        \
+      case 1: EZ_GROUP(DD, TY, 1); break;                                                                                     \
+      case 2: EZ_GROUP(DD, TY, 2); break;                                                                                     \
+      case 4: EZ_GROUP(DD, TY, 4); break;                                                                                     \
+      case 8: EZ_GROUP(DD, TY, 8); break;                                                                                     \
+      default: EZ_GROUP(DD, TY, 16); break;                                                                                   \
+    }                                                                                                                         \
+    if (pl.nsplit > 1)                                                                                                        \
+      hipLaunchKernelGGL((ez::quant_decode_join_kernel<DD>), dim3(unsigned(joins)), dim3(256), 0, stream, a, pl);             \
+  } while (0)
   EZ_KV8_DISPATCH(EZ_GO);
 #undef EZ_GO
+#undef EZ_GROUP
   return ez::launch_status(op);
 }
