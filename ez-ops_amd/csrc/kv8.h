@@ -109,6 +109,35 @@ __device__ __forceinline__ uint32_t kv8_codes(const float (&y)[4]) {
   }
 }
 
+// Eight finite bf16 values of magnitude at most TOP 2^(e - 127) -> codes in scale 2^(e - 127).
+// e4m3: one conversion with the scale for two values.  int8: x 2^-e + 1.5 2^23 leaves the
+// nearest whole number, ties to even, in the low bits of the sum, as a signed byte.
+template <int TYPE>
+__device__ __forceinline__ uint2 kv8_codes8(const uint4& x, int e) {
+  if constexpr (TYPE == kKvE4m3) {
+    typedef short s16x2_t __attribute__((ext_vector_type(2)));
+    const float s = __uint_as_float(uint32_t(e) << 23);
+    s16x2_t lo{0, 0}, hi{0, 0};
+    lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(lo, __builtin_bit_cast(bf16x2_t, x.x), s, false);
+    lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(lo, __builtin_bit_cast(bf16x2_t, x.y), s, true);
+    hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(hi, __builtin_bit_cast(bf16x2_t, x.z), s, false);
+    hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(hi, __builtin_bit_cast(bf16x2_t, x.w), s, true);
+    return make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
+  } else {
+    const float inv = __uint_as_float(uint32_t(254 - e) << 23);
+    float f[8];
+    unpack8(x, f);
+    uint32_t b[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) b[i] = __float_as_uint(fmaf(f[i], inv, 12582912.f));
+    auto pack = [](uint32_t b0, uint32_t b1, uint32_t b2, uint32_t b3) {
+      const uint32_t lo = __builtin_amdgcn_perm(b1, b0, 0x0c0c0400u), hi = __builtin_amdgcn_perm(b3, b2, 0x0c0c0400u);
+      return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+    };
+    return make_uint2(pack(b[0], b[1], b[2], b[3]), pack(b[4], b[5], b[6], b[7]));
+  }
+}
+
 // Least e with amax <= TOP 2^(e - 127) for the bf16 magnitude `m` (sign bit clear,
 // finite): TOP = 127 = (1 + 126/128) 2^6 for int8, 448 = (1 + 96/128) 2^8 for e4m3.
 template <int TYPE>

@@ -8,8 +8,11 @@
 //   code = round(x 2^-e)
 // so every row is rounded against the scale that its block has after the call.
 //
-// One wave a unit: the wave that stands on a run's first token takes it, waves on
-// other tokens leave after reading two slots.
+// Both directions are memory traffic: 2 bytes a value in, 1 out, or the reverse.  A unit
+// is one wave (blocks of up to 64 tokens) or the four waves of a block (128 and 256):
+// the run's rows are read once, whole rows by 16-byte loads, and wait in registers (64
+// at most) for the maximum over all of them.  A wave looks at a window of tokens: one
+// load of 64 slots tells which of them begin a run and how long it is.
 #include "common.h"
 #include "internal.h"
 #include "kv8.h"
@@ -39,81 +42,210 @@ struct KvDequantArgs {
 
 __device__ __forceinline__ bool slot_ok(int64_t s, int64_t n) { return s >= 0 && s < n; }
 
-template <int D, int TYPE>
-__global__ __launch_bounds__(256) void kv_quant_kernel(KvQuantArgs a) {
-  EZ_PROF_WAVE(kProfKvQuant);
-  const int lane = threadIdx.x & (kWave - 1);
-  const int64_t units = a.T * a.c.Hkv * 2;
-  for (int64_t u = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6); u < units; u += int64_t(gridDim.x) * 4) {
-    const bool is_v = u & 1;
-    const int h = int((u >> 1) % a.c.Hkv);
-    const int64_t t = (u >> 1) / a.c.Hkv;
-    const int block = 1 << a.c.block_sh;
-    const int64_t slot = a.slots[t];
-    if (!slot_ok(slot, a.c.num_slots)) continue;
-    const int off = int(slot & (block - 1));
-    if (off != 0 && t > 0 && a.slots[t - 1] == slot - 1) continue;  // inside a run
-    int n = 1;
-    while (n < block - off && t + n < a.T && a.slots[t + n] == slot + n) ++n;
+constexpr int kChunk = 32;  // rows of a wave's registers at a time
 
-    const uint16_t* src = (is_v ? a.v + t * a.v_rs : a.k + t * a.k_rs) + int64_t(h) * D;
-    const int64_t rs = is_v ? a.v_rs : a.k_rs;
-    uint32_t m = 0;
-    bool nan = false;
-    for (int i = lane; i < n * D; i += kWave) {
-      const uint32_t b = src[(i / D) * rs + i % D] & 0x7fffu;
-      if (b >= 0x7f80u) nan = true;
-      else m = max(m, b);
+__device__ __forceinline__ uint32_t pk_max_u16(uint32_t a, uint32_t b) {
+  typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t,
+                            __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, a), __builtin_bit_cast(u16x2_t, b)));
+}
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+#define EZ_DPP_STEP(ctrl) v = max(v, uint32_t(__builtin_amdgcn_mov_dpp(int(v), ctrl, 0xF, 0xF, true)));
+  EZ_DPP_STEP(0xB1)   // quad_perm [1,0,3,2]
+  EZ_DPP_STEP(0x4E)   // quad_perm [2,3,0,1]
+  EZ_DPP_STEP(0x141)  // row_half_mirror
+  EZ_DPP_STEP(0x140)  // row_mirror
+#undef EZ_DPP_STEP
+  const uint32_t a = max(uint32_t(__builtin_amdgcn_readlane(int(v), 0)), uint32_t(__builtin_amdgcn_readlane(int(v), 16)));
+  const uint32_t b = max(uint32_t(__builtin_amdgcn_readlane(int(v), 32)), uint32_t(__builtin_amdgcn_readlane(int(v), 48)));
+  return max(a, b);
+}
+
+// Rows [t, t + n) of one head into the block that holds slot `slot`, WPU waves of the
+// block together, `part` of them this one; NC chunks of rows a wave (n <= 32 NC WPU).
+template <int D, int TYPE, int NC, int WPU>
+__device__ __forceinline__ void quant_run(const KvQuantArgs& a, int64_t t, int64_t slot, int n, int h, bool is_v, int part,
+                                          uint32_t* shared_max) {
+  constexpr int LPR = D / 8, RPI = kWave / LPR, NI = kChunk / RPI;  // lanes of a row, rows and loads
+  const int lane = threadIdx.x & (kWave - 1);
+  const int off = int(slot) & ((1 << a.c.block_sh) - 1);
+  const int64_t rs = is_v ? a.v_rs : a.k_rs;
+  const uint16_t* src = (is_v ? a.v : a.k) + t * rs + int64_t(h) * D + lane % LPR * 8;
+  const int64_t row0 = (((slot >> a.c.page_sh) * a.c.Hkv + h) << a.c.page_sh) + (slot & ((int64_t(1) << a.c.page_sh) - 1));
+  uint8_t* sp = (is_v ? a.c.Vs : a.c.Ks) + (row0 >> a.c.block_sh);
+  uint8_t* dst = (is_v ? a.c.V : a.c.K) + row0 * D;
+  const int r0 = part * NC * kChunk + lane / LPR;
+  int old = off ? int(*sp) : 0;
+  uint4 x[NC][NI];
+  uint32_t m2 = 0;
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      x[c][i] = make_uint4(0, 0, 0, 0);
+      if (part * NC * kChunk + c * kChunk + i * RPI < n) {
+        const int r = r0 + c * kChunk + i * RPI;
+        if (r < n) x[c][i] = *reinterpret_cast<const uint4*>(src + r * rs);
+      }
     }
-    for (int o = 32; o > 0; o >>= 1) m = max(m, uint32_t(__shfl_xor(int(m), o, kWave)));
-    const bool poison = TYPE == kKvInt8 && __ballot(nan) != 0;
-    const int64_t page = slot >> a.c.page_sh;
-    const int64_t row0 = ((page * a.c.Hkv + h) << a.c.page_sh) + (slot & ((int64_t(1) << a.c.page_sh) - 1));
-    uint8_t* sp = (is_v ? a.c.Vs : a.c.Ks) + (row0 >> a.c.block_sh);
-    uint8_t* dst = (is_v ? a.c.V : a.c.K) + row0 * D;
-    const int old = off ? kv8_exp(int(*sp)) : 0;
-    int e = poison ? kKvNanExp : kv8_need<TYPE>(m);
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const uint32_t mask = 0x7fff7fffu;
+      const uint4 v = x[c][i];
+      m2 = pk_max_u16(m2, pk_max_u16(pk_max_u16(v.x & mask, v.y & mask), pk_max_u16(v.z & mask, v.w & mask)));
+    }
+  auto all_waves = [&](uint32_t m) {
+    m = wave_max_u32(m);
+    if constexpr (WPU > 1) {
+      if (lane == 0) shared_max[part] = m;
+      __syncthreads();
+      for (int w = 0; w < WPU; ++w) m = max(m, shared_max[w]);
+      __syncthreads();
+    }
+    return uint32_t(__builtin_amdgcn_readfirstlane(int(m)));
+  };
+  uint32_t m = all_waves(max(m2 & 0xffffu, m2 >> 16));
+  const bool finite = m < 0x7f80u;
+  if (TYPE == kKvE4m3 && !finite) {  // the finite values alone set the scale
+    m = 0;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const uint32_t w[4] = {x[c][i].x, x[c][i].y, x[c][i].z, x[c][i].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t lo = w[k] & 0x7fffu, hi = (w[k] >> 16) & 0x7fffu;
+          m = max(m, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
+        }
+      }
+    m = all_waves(m);
+  }
+  int e = TYPE == kKvInt8 && !finite ? kKvNanExp : kv8_need<TYPE>(m);
+  if (off) {
+    old = kv8_exp(__builtin_amdgcn_readfirstlane(old));
     e = max(e, old);
-    if (off && e > old) {
+    if (e > old) {  // rows held before, in 4 codes a lane
       const float r = e == kKvNanExp ? 0.f : __uint_as_float(uint32_t(127 + old - e) << 23);
-      uint32_t* old_rows = reinterpret_cast<uint32_t*>(dst - int64_t(off) * D);
-      for (int i = lane; i < off * D / 4; i += kWave) {
+      uint32_t* held = reinterpret_cast<uint32_t*>(dst - int64_t(off) * D);
+      for (int i = part * kWave + lane; i < off * D / 4; i += WPU * kWave) {
         float y[4];
-        kv8_f32x4<TYPE>(old_rows[i], y);
-        for (int j = 0; j < 4; ++j) y[j] *= r;
-        old_rows[i] = kv8_codes<TYPE, true>(y);
+        kv8_f32x4<TYPE>(held[i], y);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) y[k] *= r;
+        held[i] = kv8_codes<TYPE, true>(y);
       }
     }
-    const float inv = e == kKvNanExp ? 0.f : __uint_as_float(uint32_t(254 - e) << 23);
-    for (int i = lane; i < n * D / 4; i += kWave) {
-      const uint16_t* p = src + (4 * i / D) * rs + 4 * i % D;
-      float y[4];
-      for (int j = 0; j < 4; ++j) {
-        y[j] = bf2f(p[j]) * inv;
-        if (poison) y[j] = 0.f;
+  }
+  // Values that are finite and inside the scale (but for one at the upper end of scales)
+  // take the short conversion.
+  const bool plain = finite && e < kKvHighExp;
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+      if (part * NC * kChunk + c * kChunk + i * RPI < n) {
+        const int r = r0 + c * kChunk + i * RPI;
+        uint2 w;
+        if (plain) {
+          w = kv8_codes8<TYPE>(x[c][i], e);
+        } else {
+          const float inv = e == kKvNanExp ? 0.f : __uint_as_float(uint32_t(254 - e) << 23);
+          float f[8];
+          unpack8(x[c][i], f);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) f[k] = TYPE == kKvInt8 && e == kKvNanExp ? 0.f : f[k] * inv;
+          const float lo[4] = {f[0], f[1], f[2], f[3]}, hi[4] = {f[4], f[5], f[6], f[7]};
+          w = make_uint2(kv8_codes<TYPE, true>(lo), kv8_codes<TYPE, true>(hi));
+        }
+        if (r < n) *reinterpret_cast<uint2*>(dst + r * D + lane % LPR * 8) = w;
       }
-      reinterpret_cast<uint32_t*>(dst)[i] = kv8_codes<TYPE, true>(y);
+  if (lane == 0 && part == 0) *sp = uint8_t(e);
+}
+
+template <int D, int TYPE, int NC, int WPU>
+__global__ __launch_bounds__(256) void kv_quant_kernel(KvQuantArgs a, int window) {
+  EZ_PROF_WAVE(kProfKvQuant);
+  __shared__ uint32_t shared_max[4];
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t u = WPU == 1 ? int64_t(blockIdx.x) * 4 + wave : int64_t(blockIdx.x);
+  const int units = 2 * a.c.Hkv;  // of a window
+  const int64_t t0 = u / units * window;
+  if (t0 >= a.T) return;
+  const int hv = int(u % units), h = hv >> 1;
+  // Lane i holds the slot of token t0 - 1 + i.
+  const int64_t ti = t0 - 1 + lane;
+  const int64_t s = ti >= 0 && ti < a.T ? a.slots[ti] : -1;
+  const bool ok = slot_ok(s, a.c.num_slots);
+  const int64_t before = __shfl_up(s, 1, kWave);
+  const int bmask = (1 << a.c.block_sh) - 1;
+  const uint64_t cont = __ballot(ok && lane > 0 && slot_ok(before, a.c.num_slots) && before + 1 == s && (int(s) & bmask) != 0);
+  uint64_t first = __ballot(ok) & ~cont & (((uint64_t(1) << window) - 1) << 1);  // tokens of the window that begin a run
+  while (first) {
+    const int i = __ffsll(static_cast<unsigned long long>(first)) - 1;
+    first &= first - 1;
+    const int64_t t = t0 - 1 + i;
+    const uint64_t sb = uint64_t(s);
+    const int64_t slot = int64_t(uint64_t(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(sb)), i))) |
+                                 uint64_t(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(sb >> 32)), i))) << 32);
+    const uint64_t after = i < 63 ? ~(cont >> (i + 1)) : ~uint64_t(0);
+    int n = min(1 + __ffsll(static_cast<unsigned long long>(after)) - 1, 64 - i);
+    if (i + n == 64) {  // the run may go on behind the slots at hand
+      const int most = int(min(int64_t(bmask + 1 - (int(slot) & bmask)), a.T - t));
+      while (n < most) {
+        const int r = n + lane;
+        const uint64_t same = __ballot(r < most && a.slots[t + min(r, most - 1)] == slot + r);
+        const int more = ~same ? __ffsll(static_cast<unsigned long long>(~same)) - 1 : 64;
+        n += more;
+        if (more < 64) break;
+      }
     }
-    if (lane == 0) *sp = uint8_t(e);
+    quant_run<D, TYPE, NC, WPU>(a, t, slot, n, h, hv & 1, WPU == 1 ? 0 : wave, shared_max);
   }
 }
 
+// Rows back to bf16: 8 values a thread and tensor, kPer of them in flight.
 template <int D, int TYPE>
-__global__ __launch_bounds__(256) void kv_dequant_kernel(KvDequantArgs a) {
+__global__ __launch_bounds__(256) void kv_dequant_kernel(KvDequantArgs a, int tokens) {
   EZ_PROF_WAVE(kProfKvDequant);
-  const int64_t n = a.T * a.c.Hkv * (D / 4);
-  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) {
-    const int64_t row = i / (D / 4), t = row / a.c.Hkv;
-    const int d = int(i % (D / 4)) * 4, h = int(row % a.c.Hkv);
-    const int64_t slot = a.slots[t];
-    if (!slot_ok(slot, a.c.num_slots)) continue;
-    const int64_t at = (((slot >> a.c.page_sh) * a.c.Hkv + h) << a.c.page_sh) + (slot & ((int64_t(1) << a.c.page_sh) - 1));
-    for (int w = 0; w < 2; ++w) {
-      const float s = kv8_scale((w ? a.c.Vs : a.c.Ks)[at >> a.c.block_sh]);
-      float y[4];
-      kv8_f32x4<TYPE>(*reinterpret_cast<const uint32_t*>((w ? a.c.V : a.c.K) + at * D + d), y);
-      *reinterpret_cast<uint2*>((w ? a.v_out : a.k_out) + row * D + d) =
-          make_uint2(cvt_bf2(y[0] * s, y[1] * s), cvt_bf2(y[2] * s, y[3] * s));
+  constexpr int kPer = 4;
+  const int cpt = a.c.Hkv * (D / 8);  // 16-byte pieces of a token's row
+  const int64_t t0 = int64_t(blockIdx.x) * tokens;
+  const int total = int(min(int64_t(tokens), a.T - t0)) * cpt;
+  for (int i0 = threadIdx.x; i0 < total; i0 += kPer * 256) {
+    uint2 k[kPer], v[kPer];
+    int ek[kPer], ev[kPer];
+    bool on[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int i = min(i0 + j * 256, total - 1);
+      const int t = i / cpt, c = i - t * cpt, h = c / (D / 8), d = c % (D / 8) * 8;
+      const int64_t slot = a.slots[t0 + t];
+      on[j] = slot_ok(slot, a.c.num_slots) && i0 + j * 256 < total;
+      const int64_t s = on[j] ? slot : 0;
+      const int64_t at = (((s >> a.c.page_sh) * a.c.Hkv + h) << a.c.page_sh) + (s & ((int64_t(1) << a.c.page_sh) - 1));
+      k[j] = *reinterpret_cast<const uint2*>(a.c.K + at * D + d);
+      v[j] = *reinterpret_cast<const uint2*>(a.c.V + at * D + d);
+      ek[j] = a.c.Ks[at >> a.c.block_sh];
+      ev[j] = a.c.Vs[at >> a.c.block_sh];
+    }
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      auto wide = [](const uint2& w, int e) {
+        const float s = kv8_scale(e);
+        float y[4], z[4];
+        kv8_f32x4<TYPE>(w.x, y);
+        kv8_f32x4<TYPE>(w.y, z);
+        return make_uint4(cvt_bf2(y[0] * s, y[1] * s), cvt_bf2(y[2] * s, y[3] * s), cvt_bf2(z[0] * s, z[1] * s),
+                          cvt_bf2(z[2] * s, z[3] * s));
+      };
+      if (on[j]) {
+        const int64_t out = t0 * cpt + i0 + j * 256;
+        reinterpret_cast<uint4*>(a.k_out)[out] = wide(k[j], ek[j]);
+        reinterpret_cast<uint4*>(a.v_out)[out] = wide(v[j], ev[j]);
+      }
     }
   }
 }
@@ -156,10 +288,24 @@ extern "C" int ezops_kv_cache_quant_bf16(const void* k, int64_t k_stride, const 
   a.k = static_cast<const uint16_t*>(k); a.k_rs = k_stride;
   a.v = static_cast<const uint16_t*>(v); a.v_rs = v_stride;
   a.slots = slot_mapping; a.T = T;
-  const int64_t blocks = std::min<int64_t>((T * Hkv * 2 + 3) / 4, 1 << 20);
-#define EZ_GO(DD, TY) hipLaunchKernelGGL((ez::kv_quant_kernel<DD, TY>), dim3(unsigned(blocks)), dim3(256), 0, stream, a)
+  // Tokens a wave looks at: more where there are enough to fill the card all the same
+  // (in a prompt most tokens begin no run, and a wave that finds none is only a launch).
+  int window = 1;
+  while (window < 8 && T * Hkv * 2 / window > 16384) window *= 2;
+  const int64_t units = (T + window - 1) / window * Hkv * 2, blocks = block_size <= 64 ? (units + 3) / 4 : units;
+  EZ_REQUIRE(blocks < int64_t(1) << 24, "%s: tokens * heads past one launch", op);
+#define EZ_RUN(DD, TY, NC, WPU) \
+  hipLaunchKernelGGL((ez::kv_quant_kernel<DD, TY, NC, WPU>), dim3(unsigned(blocks)), dim3(256), 0, stream, a, window)
+#define EZ_GO(DD, TY)                               \
+  do {                                              \
+    if (block_size <= 32) EZ_RUN(DD, TY, 1, 1);     \
+    else if (block_size == 64) EZ_RUN(DD, TY, 2, 1); \
+    else if (block_size == 128) EZ_RUN(DD, TY, 1, 4); \
+    else EZ_RUN(DD, TY, 2, 4);                      \
+  } while (0)
   EZ_KV8_DISPATCH(EZ_GO);
 #undef EZ_GO
+#undef EZ_RUN
   return ez::launch_status(op);
 }
 
@@ -184,8 +330,11 @@ extern "C" int ezops_kv_cache_dequant_bf16(const void* K_cache, const void* V_ca
   EZ_REQUIRE(!ez::overlap(k_out, nb, v_out, nb), "%s: the outputs overlap", op);
   a.slots = slot_mapping; a.T = T;
   a.k_out = static_cast<uint16_t*>(k_out); a.v_out = static_cast<uint16_t*>(v_out);
-  const int64_t blocks = std::min<int64_t>((T * Hkv * (D / 4) + 255) / 256, 1 << 20);
-#define EZ_GO(DD, TY) hipLaunchKernelGGL((ez::kv_dequant_kernel<DD, TY>), dim3(unsigned(blocks)), dim3(256), 0, stream, a)
+  const int cpt = int(Hkv * (D / 8));
+  const int tokens = cpt >= 1024 ? 1 : 1024 / cpt;  // of a block: 4 pieces a thread
+  const int64_t blocks = (T + tokens - 1) / tokens;
+  EZ_REQUIRE(blocks < int64_t(1) << 24, "%s: tokens past one launch", op);
+#define EZ_GO(DD, TY) hipLaunchKernelGGL((ez::kv_dequant_kernel<DD, TY>), dim3(unsigned(blocks)), dim3(256), 0, stream, a, tokens)
   EZ_KV8_DISPATCH(EZ_GO);
 #undef EZ_GO
   return ez::launch_status(op);
