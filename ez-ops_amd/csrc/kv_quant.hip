@@ -12,7 +12,8 @@
 // is one wave (blocks of up to 64 tokens) or the four waves of a block (128 and 256):
 // the run's rows are read once, whole rows by 16-byte loads, and wait in registers (64
 // at most) for the maximum over all of them.  A wave looks at a window of tokens: one
-// load of 64 slots tells which of them begin a run and how long it is.
+// load of 64 slots tells which of them begin a run and how long it is; runs of one token
+// (a decode step) go several to a wave, a row to each 8 or 16 lanes.
 #include "common.h"
 #include "internal.h"
 #include "kv8.h"
@@ -59,6 +60,34 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
   const uint32_t a = max(uint32_t(__builtin_amdgcn_readlane(int(v), 0)), uint32_t(__builtin_amdgcn_readlane(int(v), 16)));
   const uint32_t b = max(uint32_t(__builtin_amdgcn_readlane(int(v), 32)), uint32_t(__builtin_amdgcn_readlane(int(v), 48)));
   return max(a, b);
+}
+
+// 8 values -> codes of scale 2^(e - 127).  Values that are finite and inside the scale (but
+// for one at the upper end of scales) take the short conversion.
+template <int TYPE>
+__device__ __forceinline__ uint2 to_codes(const uint4& x, int e, bool finite) {
+  if (finite && e < kKvHighExp) return kv8_codes8<TYPE>(x, e);
+  const float inv = e == kKvNanExp ? 0.f : __uint_as_float(uint32_t(254 - e) << 23);
+  float f[8];
+  unpack8(x, f);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) f[k] = TYPE == kKvInt8 && e == kKvNanExp ? 0.f : f[k] * inv;
+  const float lo[4] = {f[0], f[1], f[2], f[3]}, hi[4] = {f[4], f[5], f[6], f[7]};
+  return make_uint2(kv8_codes<TYPE, true>(lo), kv8_codes<TYPE, true>(hi));
+}
+
+// The n rows a block held before, from scale `old` to the larger e: 4 codes a lane, `of` lanes.
+template <int D, int TYPE>
+__device__ __forceinline__ void turn_rows(uint8_t* rows, int n, int old, int e, int lane, int of) {
+  const float r = e == kKvNanExp ? 0.f : __uint_as_float(uint32_t(127 + old - e) << 23);
+  uint32_t* held = reinterpret_cast<uint32_t*>(rows);
+  for (int i = lane; i < n * D / 4; i += of) {
+    float y[4];
+    kv8_f32x4<TYPE>(held[i], y);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) y[k] *= r;
+    held[i] = kv8_codes<TYPE, true>(y);
+  }
 }
 
 // Rows [t, t + n) of one head into the block that holds slot `slot`, WPU waves of the
@@ -127,47 +156,72 @@ __device__ __forceinline__ void quant_run(const KvQuantArgs& a, int64_t t, int64
   if (off) {
     old = kv8_exp(__builtin_amdgcn_readfirstlane(old));
     e = max(e, old);
-    if (e > old) {  // rows held before, in 4 codes a lane
-      const float r = e == kKvNanExp ? 0.f : __uint_as_float(uint32_t(127 + old - e) << 23);
-      uint32_t* held = reinterpret_cast<uint32_t*>(dst - int64_t(off) * D);
-      for (int i = part * kWave + lane; i < off * D / 4; i += WPU * kWave) {
-        float y[4];
-        kv8_f32x4<TYPE>(held[i], y);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) y[k] *= r;
-        held[i] = kv8_codes<TYPE, true>(y);
-      }
-    }
+    if (e > old) turn_rows<D, TYPE>(dst - int64_t(off) * D, off, old, e, part * kWave + lane, WPU * kWave);
   }
-  // Values that are finite and inside the scale (but for one at the upper end of scales)
-  // take the short conversion.
-  const bool plain = finite && e < kKvHighExp;
 #pragma unroll
   for (int c = 0; c < NC; ++c)
 #pragma unroll
     for (int i = 0; i < NI; ++i)
       if (part * NC * kChunk + c * kChunk + i * RPI < n) {
         const int r = r0 + c * kChunk + i * RPI;
-        uint2 w;
-        if (plain) {
-          w = kv8_codes8<TYPE>(x[c][i], e);
-        } else {
-          const float inv = e == kKvNanExp ? 0.f : __uint_as_float(uint32_t(254 - e) << 23);
-          float f[8];
-          unpack8(x[c][i], f);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) f[k] = TYPE == kKvInt8 && e == kKvNanExp ? 0.f : f[k] * inv;
-          const float lo[4] = {f[0], f[1], f[2], f[3]}, hi[4] = {f[4], f[5], f[6], f[7]};
-          w = make_uint2(kv8_codes<TYPE, true>(lo), kv8_codes<TYPE, true>(hi));
-        }
+        const uint2 w = to_codes<TYPE>(x[c][i], e, finite);
         if (r < n) *reinterpret_cast<uint2*>(dst + r * D + lane % LPR * 8) = w;
       }
   if (lane == 0 && part == 0) *sp = uint8_t(e);
 }
 
+// Runs of one token: the lanes of a row (D / 8) take one each, so a wave takes RPI of them
+// at a time.  `i` is the lane that holds the token's slot, `on` whether these lanes have one.
+template <int D, int TYPE>
+__device__ __forceinline__ void quant_singles(const KvQuantArgs& a, int64_t t, int64_t slot, bool on, int h, bool is_v) {
+  constexpr int LPR = D / 8;
+  const int c = threadIdx.x % LPR;
+  uint8_t *sp = nullptr, *dst = nullptr;
+  uint4 x = make_uint4(0, 0, 0, 0);
+  int off = 0, old = 0;
+  if (on) {
+    off = int(slot) & ((1 << a.c.block_sh) - 1);
+    const int64_t row0 = (((slot >> a.c.page_sh) * a.c.Hkv + h) << a.c.page_sh) + (slot & ((int64_t(1) << a.c.page_sh) - 1));
+    sp = (is_v ? a.c.Vs : a.c.Ks) + (row0 >> a.c.block_sh);
+    dst = (is_v ? a.c.V : a.c.K) + row0 * D;
+    x = *reinterpret_cast<const uint4*>((is_v ? a.v + t * a.v_rs : a.k + t * a.k_rs) + int64_t(h) * D + 8 * c);
+    old = off ? kv8_exp(int(*sp)) : 0;
+  }
+  auto row_max = [](uint32_t v) {
+#define EZ_DPP_STEP(ctrl) v = max(v, uint32_t(__builtin_amdgcn_mov_dpp(int(v), ctrl, 0xF, 0xF, true)));
+    EZ_DPP_STEP(0xB1)
+    EZ_DPP_STEP(0x4E)
+    EZ_DPP_STEP(0x141)
+    if constexpr (LPR == 16) { EZ_DPP_STEP(0x140) }
+#undef EZ_DPP_STEP
+    return v;
+  };
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  uint32_t m = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) m = max(m, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
+  m = row_max(m);
+  const bool finite = m < 0x7f80u;
+  if (TYPE == kKvE4m3 && __ballot(!finite)) {  // the finite values alone set the scale
+    uint32_t f = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t lo = w[k] & 0x7fffu, hi = (w[k] >> 16) & 0x7fffu;
+      f = max(f, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
+    }
+    m = row_max(f);
+  }
+  if (!on) return;
+  const int e = max(TYPE == kKvInt8 && !finite ? kKvNanExp : kv8_need<TYPE>(m), old);
+  if (off && e > old) turn_rows<D, TYPE>(dst - int64_t(off) * D, off, old, e, c, LPR);
+  *reinterpret_cast<uint2*>(dst + 8 * c) = to_codes<TYPE>(x, e, finite);
+  if (c == 0) *sp = uint8_t(e);
+}
+
 template <int D, int TYPE, int NC, int WPU>
 __global__ __launch_bounds__(256) void kv_quant_kernel(KvQuantArgs a, int window) {
   EZ_PROF_WAVE(kProfKvQuant);
+  constexpr int LPR = D / 8, RPI = kWave / LPR;
   __shared__ uint32_t shared_max[4];
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t u = WPU == 1 ? int64_t(blockIdx.x) * 4 + wave : int64_t(blockIdx.x);
@@ -175,23 +229,39 @@ __global__ __launch_bounds__(256) void kv_quant_kernel(KvQuantArgs a, int window
   const int64_t t0 = u / units * window;
   if (t0 >= a.T) return;
   const int hv = int(u % units), h = hv >> 1;
-  // Lane i holds the slot of token t0 - 1 + i.
-  const int64_t ti = t0 - 1 + lane;
-  const int64_t s = ti >= 0 && ti < a.T ? a.slots[ti] : -1;
+  // Lane i holds the slot of token t0 + i.
+  const int64_t ti = t0 + lane;
+  const int64_t s = ti < a.T ? a.slots[ti] : -1;
+  const int64_t back = t0 > 0 ? a.slots[t0 - 1] : -1;
   const bool ok = slot_ok(s, a.c.num_slots);
-  const int64_t before = __shfl_up(s, 1, kWave);
+  const int64_t up = __shfl_up(s, 1, kWave), before = lane ? up : back;
   const int bmask = (1 << a.c.block_sh) - 1;
-  const uint64_t cont = __ballot(ok && lane > 0 && slot_ok(before, a.c.num_slots) && before + 1 == s && (int(s) & bmask) != 0);
-  uint64_t first = __ballot(ok) & ~cont & (((uint64_t(1) << window) - 1) << 1);  // tokens of the window that begin a run
-  while (first) {
-    const int i = __ffsll(static_cast<unsigned long long>(first)) - 1;
-    first &= first - 1;
-    const int64_t t = t0 - 1 + i;
+  // tokens that go on with the run of the token before them
+  const uint64_t cont = __ballot(ok && slot_ok(before, a.c.num_slots) && before + 1 == s && (int(s) & bmask) != 0);
+  const uint64_t mine = window == 64 ? ~uint64_t(0) : (uint64_t(1) << window) - 1;
+  const uint64_t first = __ballot(ok) & ~cont & mine;
+  // a run of one token, but for one that ends where the slots at hand end
+  uint64_t single = first & ~(cont >> 1) & ~(uint64_t(1) << 63);
+  uint64_t many = first & ~single;
+  for (int p = 0; single; ++p) {
+    int i = -1;
+#pragma unroll
+    for (int g = 0; g < RPI; ++g) {
+      if (single && lane / LPR == g) i = __ffsll(static_cast<unsigned long long>(single)) - 1;
+      single &= single - 1;
+    }
+    const int64_t slot = __shfl(s, i < 0 ? 0 : i, kWave);
+    if (p % WPU == (WPU == 1 ? 0 : wave)) quant_singles<D, TYPE>(a, t0 + i, slot, i >= 0, h, hv & 1);
+  }
+  while (many) {
+    const int i = __ffsll(static_cast<unsigned long long>(many)) - 1;
+    many &= many - 1;
+    const int64_t t = t0 + i;
     const uint64_t sb = uint64_t(s);
     const int64_t slot = int64_t(uint64_t(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(sb)), i))) |
                                  uint64_t(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(sb >> 32)), i))) << 32);
     const uint64_t after = i < 63 ? ~(cont >> (i + 1)) : ~uint64_t(0);
-    int n = min(1 + __ffsll(static_cast<unsigned long long>(after)) - 1, 64 - i);
+    int n = min(__ffsll(static_cast<unsigned long long>(after)), 64 - i);
     if (i + n == 64) {  // the run may go on behind the slots at hand
       const int most = int(min(int64_t(bmask + 1 - (int(slot) & bmask)), a.T - t));
       while (n < most) {
@@ -288,10 +358,12 @@ extern "C" int ezops_kv_cache_quant_bf16(const void* k, int64_t k_stride, const 
   a.k = static_cast<const uint16_t*>(k); a.k_rs = k_stride;
   a.v = static_cast<const uint16_t*>(v); a.v_rs = v_stride;
   a.slots = slot_mapping; a.T = T;
-  // Tokens a wave looks at: more where there are enough to fill the card all the same
-  // (in a prompt most tokens begin no run, and a wave that finds none is only a launch).
+  // Tokens a wave looks at: as many as leave 4096 waves.  In a prompt most tokens begin no
+  // run, and a wave that finds none still holds its place for two loads (16384 tokens of
+  // 8 heads in blocks of 64: 82 us with 8 tokens a wave, 47, 33 and 27 with 16, 32 and 64;
+  // a mixed step of 3500 tokens 10.6, 9.2, 8.8 and 10.0 us at 2, 4, 8 and 16).
   int window = 1;
-  while (window < 8 && T * Hkv * 2 / window > 16384) window *= 2;
+  while (window < 64 && T * Hkv * 2 / window > 4096) window *= 2;
   const int64_t units = (T + window - 1) / window * Hkv * 2, blocks = block_size <= 64 ? (units + 3) / 4 : units;
   EZ_REQUIRE(blocks < int64_t(1) << 24, "%s: tokens * heads past one launch", op);
 #define EZ_RUN(DD, TY, NC, WPU) \

@@ -3,6 +3,7 @@
 
 #include <array>
 
+#include "common.h"
 #include "kv8.h"
 
 namespace ez {
@@ -21,6 +22,46 @@ struct QuantAttnArgs {
 };
 
 inline bool kv8_aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+constexpr float kLowest = -3e38f;  // softmax reference before any row: finite, so that differences are
+
+// Joins n partials of a query row: (m, l) ml_step apart, 4 dims of O o_step apart, kPer of
+// each in flight.  out = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s.
+template <int kPer>
+__device__ __forceinline__ void join_parts(const float2* ml, const float4* po, int64_t ml_step, int64_t o_step, int n,
+                                           float (&out)[4]) {
+  float m = kLowest, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < n; s0 += kPer) {
+    float2 x[kPer];
+    float4 p[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int s = min(s0 + i, n - 1);
+      x[i] = ml[s * ml_step];
+      p[i] = po[s * o_step];
+    }
+    float mn = m;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) mn = fmaxf(mn, x[i].x);
+    const float back = __builtin_amdgcn_exp2f(m - mn);
+    m = mn;
+    l *= back;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] *= back;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const float f = s0 + i < n ? __builtin_amdgcn_exp2f(x[i].x - m) : 0.f;  // behind the last: the last again
+      l = fmaf(f, x[i].y, l);
+      o[0] = fmaf(f, p[i].x, o[0]);
+      o[1] = fmaf(f, p[i].y, o[1]);
+      o[2] = fmaf(f, p[i].z, o[2]);
+      o[3] = fmaf(f, p[i].w, o[3]);
+    }
+  }
+  const float inv = 1.f / l;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) out[k] = o[k] * inv;
+}
 
 struct Range {
   const void* p;

@@ -35,32 +35,79 @@ EZ_PROF_DEFINE(quantdecode)
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLowest = -3e38f;  // reference before any row: finite, so that differences are
 constexpr int kW = 4;              // waves of a block
 constexpr int kT = 32;             // rows of a wave's tile
-constexpr int kMaxSplits = 64;
+constexpr int kMaxSplits = 32;     // chunks of a sequence
+constexpr int kSumSeqs = 1024;     // sequences whose lengths every block sums
+constexpr int kAimMany = 4096;     // rows of a chunk where there are more
 
 struct SplitPlan {
-  int chunk;   // rows of a block, a multiple of kW * kT
-  int nsplit;  // chunks of the longest sequence
-  float* o;    // partials [B * H][nsplit][D]
-  float* ml;   // [B * H][nsplit][2]
+  int target;       // chunks of a kv head to aim at; 0: a block per sequence
+  int blocks;       // chunks at most
+  float* o;         // partials [chunk][Hkv][G][D]
+  float2* ml;       // [chunk][Hkv][G]
+  int2* head;       // [B][Hkv]: block of a sequence's first chunk, number of chunks
 };
 
 __device__ __forceinline__ int seq_len(const QuantAttnArgs& a, int b) { return min(max(a.kv_lens[b], 0), int(a.cap)); }
-__device__ __forceinline__ int chunks(int len, int chunk) { return len > chunk ? (len + chunk - 1) / chunk : 1; }
 
-// Sequence and chunk of the idx-th block of a kv head; false behind the last one.  A
-// sequence without rows has one (which writes its zeros).  256 lengths a step.
-__device__ __forceinline__ bool find_chunk(const QuantAttnArgs& a, int chunk, int idx, int& b, int& split, int& len) {
+// Rows of a chunk of a sequence of L rows, given the rows to aim at: equal ones, a whole
+// number of tiles for every wave.
+__device__ __forceinline__ int chunk_rows(int L, int aim) {
+  const int n = min((L + aim - 1) / aim, kMaxSplits);
+  return ((L + n - 1) / n + kW * kT - 1) / (kW * kT) * (kW * kT);
+}
+__device__ __forceinline__ int chunk_count(int L, int aim) {
+  if (L <= aim) return 1;
+  const int rows = chunk_rows(L, aim);
+  return (L + rows - 1) / rows;
+}
+
+struct Chunk {
+  int b, split, len, rows, count;
+};
+
+// The idx-th chunk of the batch; false behind the last one.  The rows to aim at are all the
+// batch's over the chunks to aim at, so a ragged batch is shared out by rows (above 1024
+// sequences 4096, without the sum).  A sequence without rows has one (which writes its zeros).
+__device__ __forceinline__ bool find_chunk(const QuantAttnArgs& a, int target, int idx, Chunk& c) {
+  constexpr int kPer = 4;  // lengths of a lane and step
   const int lane = threadIdx.x & (kWave - 1), B = int(a.B);
-  for (int b0 = 0; b0 < B; b0 += 4 * kWave) {
-    int n[4], L[4], sum = 0;
+  if (B == 1) {  // the usual case of few blocks and little time
+    c.len = seq_len(a, 0);
+    const int aim = (c.len / target / (kW * kT) + 1) * (kW * kT);
+    c.b = 0;
+    c.split = idx;
+    c.count = chunk_count(c.len, aim);
+    c.rows = c.count == 1 ? c.len : chunk_rows(c.len, aim);
+    return idx < c.count;
+  }
+  int L[kPer];
+  auto lengths = [&](int b0) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int s = b0 + 4 * lane + i;
-      L[i] = s < B ? seq_len(a, s) : 0;
-      n[i] = s < B ? chunks(L[i], chunk) : 0;
+    for (int i = 0; i < kPer; ++i) {
+      const int s = b0 + kPer * lane + i;
+      L[i] = s < B ? seq_len(a, s) : -1;
+    }
+  };
+  int aim = kAimMany;
+  if (B <= kSumSeqs) {
+    float sum = 0.f;  // up to 2^10 lengths of 2^30
+    for (int b0 = 0; b0 < B; b0 += kPer * kWave) {
+      lengths(b0);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) sum += float(max(L[i], 0));
+    }
+    // rounded up past the sums' rounding, so that the chunks stay within the blocks
+    const float per = wave_reduce_uniform<false>(sum) * 1.0001f / float(target);
+    aim = (int(per) / (kW * kT) + 1) * (kW * kT);
+  }
+  for (int b0 = 0; b0 < B; b0 += kPer * kWave) {
+    if (B > kPer * kWave || B > kSumSeqs) lengths(b0);
+    int n[kPer], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      n[i] = L[i] < 0 ? 0 : chunk_count(L[i], aim);
       sum += n[i];
     }
     const int end = wave_scan(sum);
@@ -69,15 +116,17 @@ __device__ __forceinline__ bool find_chunk(const QuantAttnArgs& a, int chunk, in
       const int l = __ffsll(static_cast<unsigned long long>(hit)) - 1;
       int at = idx - (__builtin_amdgcn_readlane(end, l) - __builtin_amdgcn_readlane(sum, l));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < kPer; ++i) {
         const int ni = __builtin_amdgcn_readlane(n[i], l);
         if (at >= 0 && at < ni) {
-          b = b0 + 4 * l + i;
-          split = at;
-          len = __builtin_amdgcn_readlane(L[i], l);
+          c.b = b0 + kPer * l + i;
+          c.split = at;
+          c.len = __builtin_amdgcn_readlane(L[i], l);
+          c.count = ni;
         }
         at -= ni;
       }
+      c.rows = c.count == 1 ? c.len : chunk_rows(c.len, aim);
       return true;
     }
     idx -= __builtin_amdgcn_readlane(end, kWave - 1);
@@ -110,12 +159,13 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(3)))
   auto vswz = [](int r) { return D == 128 ? ((r >> 1) & 1) | ((r >> 4) & 1) << 1 : (r >> 4) & 1; };
 
   const int kvh = int(blockIdx.x % unsigned(a.c.Hkv)), idx = int(blockIdx.x / unsigned(a.c.Hkv));
-  int b = idx, split = 0, L = 0;
-  if (pl.nsplit == 1) L = seq_len(a, b);
-  else if (!find_chunk(a, pl.chunk, idx, b, split, L)) return;
-  b = __builtin_amdgcn_readfirstlane(b);
-  split = __builtin_amdgcn_readfirstlane(split);
-  L = __builtin_amdgcn_readfirstlane(L);
+  Chunk ck{idx, 0, 0, 0, 1};
+  if (pl.target == 0) ck.len = ck.rows = seq_len(a, idx);
+  else if (!find_chunk(a, pl.target, idx, ck)) return;
+  const int b = __builtin_amdgcn_readfirstlane(ck.b), split = __builtin_amdgcn_readfirstlane(ck.split);
+  const int L = __builtin_amdgcn_readfirstlane(ck.len), rows = __builtin_amdgcn_readfirstlane(ck.rows);
+  const int count = __builtin_amdgcn_readfirstlane(ck.count);
+  if (pl.target != 0 && split == 0 && threadIdx.x == 0) pl.head[int64_t(b) * a.c.Hkv + kvh] = make_int2(int(blockIdx.x), count);
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int li = lane & 15, lg = lane >> 4;
@@ -125,7 +175,7 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(3)))
       *reinterpret_cast<uint4*>(a.out + (int64_t(b) * a.H + h0) * D + i * 8) = make_uint4(0, 0, 0, 0);
     return;
   }
-  const int r0 = split * pl.chunk, r1 = min(L, r0 + pl.chunk), last = r1 - 1;
+  const int r0 = split * rows, r1 = min(L, r0 + rows), last = r1 - 1;
 
   // ---- loads of a tile: its page id one tile ahead (a vector load, so that it is waited
   // for in order with the codes), then codes and exponents
@@ -296,7 +346,6 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(3)))
     }
   }
   __syncthreads();
-  const bool whole = L <= pl.chunk;
   for (int i = threadIdx.x; i < G * D / 4; i += kW * kWave) {
     const int h = i / (D / 4), d = i % (D / 4) * 4;
     float M = kLowest;
@@ -311,12 +360,13 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(3)))
       for (int k = 0; k < 4; ++k) ov[k] = fmaf(f, lds.j.O[w][h][d + k], ov[k]);
     }
     const int64_t hq = int64_t(b) * a.H + h0 + h;
-    if (whole) {
+    if (count == 1) {
       const float r = 1.f / lv;
       *reinterpret_cast<uint2*>(a.out + hq * D + d) = make_uint2(cvt_bf2(ov[0] * r, ov[1] * r), cvt_bf2(ov[2] * r, ov[3] * r));
     } else {
-      *reinterpret_cast<float4*>(pl.o + (hq * pl.nsplit + split) * D + d) = make_float4(ov[0], ov[1], ov[2], ov[3]);
-      if (d == 0) *reinterpret_cast<float2*>(pl.ml + (hq * pl.nsplit + split) * 2) = make_float2(M, lv);
+      const int64_t part = int64_t(blockIdx.x) * G + h;
+      *reinterpret_cast<float4*>(pl.o + part * D + d) = make_float4(ov[0], ov[1], ov[2], ov[3]);
+      if (d == 0) pl.ml[part] = make_float2(M, lv);
     }
   }
 }
@@ -329,39 +379,34 @@ __global__ __launch_bounds__(256) void quant_decode_join_kernel(QuantAttnArgs a,
   constexpr int TPR = D / 4;
   const int64_t hq = int64_t(blockIdx.x) * (256 / TPR) + threadIdx.x / TPR;
   if (hq >= a.B * a.H) return;
-  const int L = seq_len(a, int(hq / a.H)), d = int(threadIdx.x) % TPR * 4;
-  if (L <= pl.chunk) return;
-  const int n = chunks(L, pl.chunk);
-  const float2* ml = reinterpret_cast<const float2*>(pl.ml) + hq * pl.nsplit;
-  const float4* op = reinterpret_cast<const float4*>(pl.o + hq * pl.nsplit * D + d);
-  float m = kLowest;
-  for (int s = 0; s < n; ++s) m = fmaxf(m, ml[s].x);
-  float o[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
-#pragma unroll 8
-  for (int s = 0; s < n; ++s) {
-    const float2 x = ml[s];
-    const float4 p = op[s * (D / 4)];
-    const float f = __builtin_amdgcn_exp2f(x.x - m);
-    l = fmaf(f, x.y, l);
-    o[0] = fmaf(f, p.x, o[0]);
-    o[1] = fmaf(f, p.y, o[1]);
-    o[2] = fmaf(f, p.z, o[2]);
-    o[3] = fmaf(f, p.w, o[3]);
-  }
-  const float r = 1.f / l;
-  *reinterpret_cast<uint2*>(a.out + hq * D + d) = make_uint2(cvt_bf2(o[0] * r, o[1] * r), cvt_bf2(o[2] * r, o[3] * r));
+  const int d = int(threadIdx.x) % TPR * 4, G = a.H / a.c.Hkv;
+  const int2 head = pl.head[hq / G];
+  if (head.y == 1) return;
+  const int64_t part = int64_t(head.x) * G + hq % G, step = int64_t(a.c.Hkv) * G;
+  const float4* po = reinterpret_cast<const float4*>(pl.o + part * D + d);
+  float o[4];
+  if (head.y <= 4) join_parts<4>(pl.ml + part, po, step, step * (D / 4), head.y, o);
+  else join_parts<16>(pl.ml + part, po, step, step * (D / 4), head.y, o);
+  *reinterpret_cast<uint2*>(a.out + hq * D + d) = make_uint2(cvt_bf2(o[0], o[1]), cvt_bf2(o[2], o[3]));
 }
 
-// Chunks: enough blocks for every CU to hold its fill at the longest length, none below a
-// tile a wave.
+// Chunks of a kv head to aim at: what fills the three places that a CU has for blocks, less
+// the half chunk that a sequence adds on average (two places where a sequence would get more
+// chunks than the join takes at once: 4 x 8192 rows of 32 / 8 heads 38.7 to 35.8 us); with many sequences,
+// chunks of twice the mean length, so that a long one among them is shared out.  None below a
+// tile a wave.  Sequences that are short and fill the card whole stay whole, without a join
+// (64 x 1024 rows 42.7 to 38 us, 200 of up to 1500 79 to 71).
 SplitPlan plan(int64_t B, int64_t Hkv, int64_t kv_len) {
-  const int64_t unit = kW * kT, cus = num_cus();
-  int64_t ns = (4 * cus + B * Hkv - 1) / (B * Hkv);
-  const int64_t most = (kv_len + unit - 1) / unit;
-  ns = ns < most ? ns : most;
-  ns = ns < kMaxSplits ? ns : kMaxSplits;
-  const int64_t chunk = ((kv_len + ns - 1) / ns + unit - 1) / unit * unit;
-  return {int(chunk), int((kv_len + chunk - 1) / chunk), nullptr, nullptr};
+  const int64_t cus = num_cus();
+  if (kv_len <= kW * kT || (B * Hkv >= 2 * cus && kv_len <= 2048)) return {0, int(B), nullptr, nullptr, nullptr};
+  int64_t places = 3 * cus / Hkv;
+  if (places > 16 * B) places = 2 * cus / Hkv > 16 * B ? 2 * cus / Hkv : 16 * B;
+  int64_t target = places - B / 2 > B / 2 ? places - B / 2 : B / 2;
+  target = target < 1 ? 1 : target;
+  int64_t most = (kv_len + kW * kT - 1) / (kW * kT);  // of a sequence
+  most = most < kMaxSplits ? most : kMaxSplits;
+  const int64_t blocks = B <= kSumSeqs && target + B < B * most ? target + B : B * most;
+  return {int(target), int(blocks), nullptr, nullptr, nullptr};
 }
 int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
 
@@ -374,7 +419,7 @@ extern "C" size_t ezops_quant_paged_attn_decode_workspace_size(int64_t B, int64_
       kv_len > (int64_t(1) << 30))
     return 0;
   const ez::SplitPlan pl = ez::plan(B, Hkv, kv_len);
-  return pl.nsplit == 1 ? 0 : size_t(ez::up256(B * H * pl.nsplit * D * 4) + ez::up256(B * H * pl.nsplit * 8));
+  return pl.target == 0 ? 0 : size_t(ez::up256(pl.blocks * H * D * 4) + ez::up256(pl.blocks * H * 8) + ez::up256(B * Hkv * 8));
 }
 
 extern "C" int ezops_quant_paged_attn_decode_bf16(const void* q, int64_t q_stride, const void* K_cache, const void* V_cache,
@@ -395,16 +440,18 @@ extern "C" int ezops_quant_paged_attn_decode_bf16(const void* q, int64_t q_strid
   if (rc != EZ_OK) return rc;
   ez::finish_args(a, page_size, max_kv_len);
   ez::SplitPlan pl = ez::plan(B, Hkv, a.cap);
-  const int64_t blocks = B * Hkv * pl.nsplit, joins = (B * H * (D / 4) + 255) / 256;
+  const int64_t blocks = Hkv * pl.blocks, joins = (B * H * (D / 4) + 255) / 256;
   EZ_REQUIRE(blocks < int64_t(1) << 24, "%s: batch * heads past one launch", op);
-  if (pl.nsplit > 1) {
+  if (pl.target) {
     const size_t need = ezops_quant_paged_attn_decode_workspace_size(B, H, Hkv, D, a.cap);
     EZ_REQUIRE(ws && ws_bytes >= need, "%s: workspace too small (%zu < %zu)", op, ws_bytes, need);
     EZ_REQUIRE(ez::kv8_aligned16(ws), "%s: workspace must be 16-byte aligned", op);
     for (const auto& x : ez::attn8_tensors(a, H))
       EZ_REQUIRE(!ez::overlap(ws, int64_t(need), x.p, x.n), "%s: workspace overlaps a tensor", op);
-    pl.o = static_cast<float*>(ws);
-    pl.ml = reinterpret_cast<float*>(static_cast<char*>(ws) + ez::up256(B * H * pl.nsplit * D * 4));
+    char* at = static_cast<char*>(ws);
+    pl.o = reinterpret_cast<float*>(at);
+    pl.ml = reinterpret_cast<float2*>(at += ez::up256(pl.blocks * H * D * 4));
+    pl.head = reinterpret_cast<int2*>(at += ez::up256(pl.blocks * H * 8));
   }
 #define EZ_GROUP(DD, TY, GG)                                                                                                  \
   hipLaunchKernelGGL((ez::quant_decode_kernel<DD, TY, GG>), dim3(unsigned(blocks)), dim3(ez::kW * ez::kWave), 0, stream, a, pl)
@@ -417,7 +464,7 @@ extern "C" int ezops_quant_paged_attn_decode_bf16(const void* q, int64_t q_strid
       case 8: EZ_GROUP(DD, TY, 8); break;                                                                                     \
       default: EZ_GROUP(DD, TY, 16); break;                                                                                   \
     }                                                                                                                         \
-    if (pl.nsplit > 1)                                                                                                        \
+    if (pl.target)                                                                                                            \
       hipLaunchKernelGGL((ez::quant_decode_join_kernel<DD>), dim3(unsigned(joins)), dim3(256), 0, stream, a, pl);             \
   } while (0)
   EZ_KV8_DISPATCH(EZ_GO);

@@ -38,9 +38,9 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.f;     // log2 headroom of the softmax reference, see below
-constexpr float kLowest = -3e38f;  // reference before any key: finite, so that differences are
-constexpr int kW = 8;            // waves of a block
-constexpr int kRows = 32 * kW;   // (query, head) rows of a block
+// Waves of a block, 32 (query, head) rows each.
+constexpr int waves_of(int64_t D) { return D == 64 ? 4 : 8; }
+constexpr int rows_of(int64_t D) { return 32 * waves_of(D); }
 constexpr int kBK = 64;          // keys of a tile
 constexpr int kMaxSplits = 32;
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
@@ -113,15 +113,15 @@ __device__ __forceinline__ uint32_t without_nan(uint32_t w) {
 }
 
 template <int D, int TYPE, int G>
-__global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(2))) void quant_prefill_kernel(QuantAttnArgs a,
+__global__ __launch_bounds__(waves_of(D) * kWave) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2))) void quant_prefill_kernel(QuantAttnArgs a,
                                                                                                           SplitPlan pl) {
   EZ_PROF_WAVE(kProfQuantAttnPrefill);
-  constexpr int QT = kRows / G;     // queries of a block
+  constexpr int QT = rows_of(D) / G;  // queries of a block
   constexpr int NS = D / 16;        // 16-dim steps of S
   constexpr int ND = D / 32;        // 32-dim blocks of O^T
   constexpr int CPR = D / 8;        // 16-byte chunks of a bf16 row in LDS
   constexpr int TPR = D / 16;       // threads that stage a row
-  constexpr int NL = D / 64;        // 16-byte loads a thread: K and V (D = 128), or one of them (D = 64)
+  static_assert(kBK * TPR == waves_of(D) * kWave, "a thread stages 16 bytes of K and of V");
   __shared__ __align__(16) uint16_t Ks[2][kBK * D];  // [key][chunk ^ key % CPR]
   __shared__ __align__(16) uint16_t Vs[2][kBK * D];  // [key][chunk ^ vswz(key)]
   __shared__ __align__(16) float Cs[2][12];          // of each 16 keys: c, v, 2^-v twice in bf16
@@ -158,10 +158,8 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(2)))
   }
 
   // ---- staging: thread = (key sr of the tile, 16 dims from 16 sc on)
-  const int sid = NL == 2 ? tid : tid & (kBK * TPR - 1);
-  const int sr = sid / TPR, sc = sid % TPR;
-  const bool stage_v = NL == 1 && tid >= kBK * TPR;  // D = 64: the upper half of the block stages V
-  const bool stage_c = sr % 16 == 0 && sc == 0 && !stage_v;
+  const int sr = tid / TPR, sc = tid % TPR;
+  const bool stage_c = sr % 16 == 0 && sc == 0;
   const int32_t* table = a.table + int64_t(qt.b) * a.M;
   const int pmask = (1 << a.c.page_sh) - 1;
   auto key_row = [&](int t) { return min((tile0 + t) * kBK + sr, kend - 1); };
@@ -169,22 +167,22 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(2)))
     const uint32_t page = min(uint32_t(id), uint32_t(a.c.num_pages - 1));
     return ((int64_t(page) * a.c.Hkv + kvh) << a.c.page_sh) + (r & pmask);
   };
-  uint4 raw[NL];
-  int ek = 0, ev = 0;
-  int32_t id = table[key_row(0) >> a.c.page_sh];
-  auto issue = [&](int t) {  // tile t's codes and exponents, and the page of tile t + 1
-    const int64_t at = flat_row(key_row(t), id);
-    if (NL == 2) {
-      raw[0] = *reinterpret_cast<const uint4*>(a.c.K + at * D + 16 * sc);
-      raw[NL - 1] = *reinterpret_cast<const uint4*>(a.c.V + at * D + 16 * sc);
-    } else {
-      raw[0] = *reinterpret_cast<const uint4*>((stage_v ? a.c.V : a.c.K) + at * D + 16 * sc);
-    }
+  // Two tiles are in flight in registers, the tile of parity P in slot P; the page of a tile is
+  // asked for two tiles before its codes, ahead of theirs, so that no wait for it waits for them.
+  uint4 raw[2][2];  // [parity][K, V]
+  int ek[2] = {0, 0}, ev[2] = {0, 0};
+  auto page_of = [&](int t) { return table[key_row(t) >> a.c.page_sh]; };
+  int32_t id[2] = {page_of(0), page_of(1)};
+  auto issue = [&](int t, auto parity) {  // tile t's codes and exponents
+    constexpr int P = decltype(parity)::value;
+    const int64_t at = flat_row(key_row(t), id[P]);
+    id[P] = page_of(t + 2);
+    raw[P][0] = *reinterpret_cast<const uint4*>(a.c.K + at * D + 16 * sc);
+    raw[P][1] = *reinterpret_cast<const uint4*>(a.c.V + at * D + 16 * sc);
     if (stage_c) {
-      ek = a.c.Ks[at >> a.c.block_sh];
-      ev = a.c.Vs[at >> a.c.block_sh];
+      ek[P] = a.c.Ks[at >> a.c.block_sh];
+      ev[P] = a.c.Vs[at >> a.c.block_sh];
     }
-    id = table[key_row(t + 1) >> a.c.page_sh];
   };
   auto vswz = [](int r) { return D == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); };
   auto put = [&](uint16_t* dst, int swz, const uint4& v) {
@@ -192,23 +190,22 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(2)))
     *reinterpret_cast<uint4*>(dst + sr * D + ((2 * sc) ^ swz) * 8) = make_uint4(p0.x, p0.y, p1.x, p1.y);
     *reinterpret_cast<uint4*>(dst + sr * D + ((2 * sc + 1) ^ swz) * 8) = make_uint4(p2.x, p2.y, p3.x, p3.y);
   };
-  auto stage = [&](int t) {  // tile t from its registers into its buffer
-    const int buf = t & 1, k0 = (tile0 + t) * kBK;
+  auto stage = [&](int t, auto parity) {  // tile t from its registers into its buffer
+    constexpr int buf = decltype(parity)::value;
+    const int k0 = (tile0 + t) * kBK;
     if (TYPE == kKvE4m3 && k0 + kBK - 1 > qt.past + qt.first) {
       // Some query of the block does not see some key of the tile: its weight of 0 must not
       // meet a NaN.  The codes go, and fix_nan puts them back where they are seen.
-      if (NL == 2 || stage_v) {
-        uint4& v = raw[NL - 1];
-        if (has_nan_code(v.x) || has_nan_code(v.y) || has_nan_code(v.z) || has_nan_code(v.w)) {
-          v = make_uint4(without_nan(v.x), without_nan(v.y), without_nan(v.z), without_nan(v.w));
-          nan_tile[buf] = k0;
-        }
+      uint4& v = raw[buf][1];
+      if (has_nan_code(v.x) || has_nan_code(v.y) || has_nan_code(v.z) || has_nan_code(v.w)) {
+        v = make_uint4(without_nan(v.x), without_nan(v.y), without_nan(v.z), without_nan(v.w));
+        nan_tile[buf] = k0;
       }
     }
-    if (!stage_v) put(Ks[buf], sr % CPR, raw[0]);
-    if (NL == 2 || stage_v) put(Vs[buf], vswz(sr), raw[NL - 1]);
+    put(Ks[buf], sr % CPR, raw[buf][0]);
+    put(Vs[buf], vswz(sr), raw[buf][1]);
     if (stage_c) {
-      const int k = kv8_exp(ek), v = kv8_exp(ev), u = sr / 16;
+      const int k = kv8_exp(ek[buf]), v = kv8_exp(ev[buf]), u = sr / 16;
       const bool nan = v == kKvNanExp;
       Cs[buf][u] = sl2 * kv8_scale(k);
       Cs[buf][4 + u] = nan ? __uint_as_float(0x7fc00000u) : float(v - 127);
@@ -217,9 +214,12 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(2)))
   };
   if (tid < 2) nan_tile[tid] = -1;
   __syncthreads();
-  issue(0);
-  stage(0);
-  if (n > 1) issue(1);
+  using even = std::integral_constant<int, 0>;
+  using odd = std::integral_constant<int, 1>;
+  issue(0, even{});
+  if (n > 1) issue(1, odd{});
+  stage(0, even{});
+  if (n > 2) issue(2, even{});
   __syncthreads();
 
   // ---- operand addresses: K row 32 kk + j has the swizzle of row j; lane (i = 16 g1 + mm,
@@ -242,8 +242,9 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(2)))
     for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
   float m = kLowest, l = 0.f;
 
-  auto compute = [&](int t) {
-    const int buf = t & 1, k0 = (tile0 + t) * kBK;
+  auto compute = [&](int t, auto parity) {
+    constexpr int buf = decltype(parity)::value;
+    const int k0 = (tile0 + t) * kBK;
     const bool edge = k0 + kBK - 1 > wave_first;  // some of the wave's queries do not see all of the tile
     const uint16_t* ks = Ks[buf];
     f32x16_t st[2];
@@ -252,11 +253,20 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(2)))
 #pragma unroll
       for (int r = 0; r < 16; ++r) st[kk][r] = 0.f;
 #pragma unroll
-    for (int s = 0; s < NS; ++s)
+    for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk)
+      for (int s = 0; s < NS; ++s)
         st[kk] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
             as_bf16x8(*reinterpret_cast<const uint4*>(ks + 32 * kk * D + koff[s])), qf[s], st[kk], 0, 0, 0);
+    // The reads run NS steps ahead of the products (left alone they run one ahead, and
+    // every pair of products waits out the latency of LDS).
+    __builtin_amdgcn_sched_group_barrier(0x100, NS, 0);
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x8, NS, 0);
     // st[kk][r] = s' of (query j, key k0 + 32 kk + 8 (r / 4) + 4 h + r % 4); 16 keys u = 2 kk + r / 8 share a scale
     float c[4], v[4], iv[4];
 #pragma unroll
@@ -338,13 +348,17 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(2)))
     }
   };
 
-  for (int t = 0; t < n; ++t) {
+  auto step = [&](int t, auto parity, auto other) {
     if (t + 1 < n) {
-      stage(t + 1);  // its buffer was read last before the barrier behind tile t - 1
-      if (t + 2 < n) issue(t + 2);
+      stage(t + 1, other);  // its buffer was read last before the barrier behind tile t - 1
+      if (t + 3 < n) issue(t + 3, other);
     }
-    if (wave_on && (tile0 + t) * kBK <= wave_last) compute(t);
+    if (wave_on && (tile0 + t) * kBK <= wave_last) compute(t, parity);
     __syncthreads();
+  };
+  for (int t = 0; t < n; t += 2) {
+    step(t, even{}, odd{});
+    if (t + 1 < n) step(t + 1, odd{}, even{});
   }
 
   // ---- l: the two lane halves hold a share of query j's sum each
@@ -376,8 +390,8 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(2)))
 template <int D, int G>
 __global__ __launch_bounds__(256) void quant_prefill_join_kernel(QuantAttnArgs a, SplitPlan pl) {
   EZ_PROF_WAVE(kProfQuantAttnCombine);
-  constexpr int QT = kRows / G, TPR = D / 4, PER = 256 / TPR;  // rows a pass
-  const int parts = kRows / PER;
+  constexpr int QT = rows_of(D) / G, TPR = D / 4, PER = 256 / TPR;  // rows of a block
+  constexpr int parts = rows_of(D) / PER;
   const int part = int(blockIdx.x) % parts, rest = int(blockIdx.x) / parts;
   const int kvh = rest % a.c.Hkv;
   QueryTile qt;
@@ -388,34 +402,41 @@ __global__ __launch_bounds__(256) void quant_prefill_join_kernel(QuantAttnArgs a
   const int kend = qt.past + min(qt.qlen, qt.first + QT), ntiles = (kend + kBK - 1) / kBK;
   const int per = split_tiles(ntiles, pl.nsplit), used = (ntiles + per - 1) / per;
   const int64_t at = int64_t(qt.t0 + qi) * a.H + kvh * G + row % G, step = a.T * a.H;
-  float m = kLowest;
-  for (int s = 0; s < used; ++s) m = fmaxf(m, pl.ml[(at + s * step) * 2]);
-  float o[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
-  for (int s = 0; s < used; ++s) {
-    const float2 x = *reinterpret_cast<const float2*>(pl.ml + (at + s * step) * 2);
-    const float4 p = *reinterpret_cast<const float4*>(pl.o + (at + s * step) * D + d);
-    const float f = __builtin_amdgcn_exp2f(x.x - m);
-    l = fmaf(f, x.y, l);
-    o[0] = fmaf(f, p.x, o[0]);
-    o[1] = fmaf(f, p.y, o[1]);
-    o[2] = fmaf(f, p.z, o[2]);
-    o[3] = fmaf(f, p.w, o[3]);
-  }
-  const float inv = 1.f / l;
-  *reinterpret_cast<uint2*>(a.out + at * D + d) = make_uint2(cvt_bf2(o[0] * inv, o[1] * inv), cvt_bf2(o[2] * inv, o[3] * inv));
+  float o[4];
+  if (pl.nsplit <= 4) join_parts<4>(reinterpret_cast<const float2*>(pl.ml) + at, reinterpret_cast<const float4*>(pl.o + at * D + d), step,
+             step * (D / 4), used, o);
+  else join_parts<16>(reinterpret_cast<const float2*>(pl.ml) + at, reinterpret_cast<const float4*>(pl.o + at * D + d), step,
+             step * (D / 4), used, o);
+  *reinterpret_cast<uint2*>(a.out + at * D + d) = make_uint2(cvt_bf2(o[0], o[1]), cvt_bf2(o[2], o[3]));
 }
 
 // Query tiles at most (a sequence adds at most one that is not full), and the splits of
-// the keys: as many as give every CU a block, none below four tiles of 64 keys at full length.
-SplitPlan plan(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t kv_len) {
-  const int64_t qt = kRows / (H / Hkv);
-  const int64_t tiles = T / qt + (B < T ? B : T);
-  const int64_t blocks = tiles * Hkv, cus = num_cus();
-  int64_t ns = cus / blocks;
-  const int64_t most = kv_len / (4 * kBK);
-  ns = ns < most ? ns : most;
-  ns = ns < kMaxSplits ? ns : kMaxSplits;
-  return {int(ns < 1 ? 1 : ns), int(tiles), nullptr, nullptr};
+// the keys that a model of the time prefers, in us: a block takes kBlock to begin and end and
+// kTile a key tile; the longest block and the blocks' sum over the CUs each bound the
+// kernel; splits add a join and their partials through memory.  The key tiles of a block
+// are at most those of kv_len, on average those of one prompt whose last row that is, or
+// half where there are several sequences.  (70 tokens on 3000 rows of 32 / 8 heads: 6, 12, 16
+// and 24 splits take 32.7, 28.7, 28.7 and 37 us; nine ragged chunks of 2660 tokens of 16 / 2 heads of 64 on up to
+// 2500 rows 61 us with one, 58 with two.)
+SplitPlan plan(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t kv_len) {
+  const int64_t qt = rows_of(D) / (H / Hkv);
+  const int64_t tiles = (T + (B < T ? B : T) * (qt - 1)) / qt;
+  const double blocks = double(tiles * Hkv), cus = num_cus();
+  const double kTile = D == 64 ? 1.2 : 2.2, kBlock = 7.0, at_once = D == 64 ? 3.0 : 1.0;
+  const double most = double(kv_len) / kBK + 1;
+  const double mean = B == 1 && kv_len > T ? double(kv_len - T / 2) / kBK : most / 2;
+  int best = 1;
+  double least = 1e30;
+  for (int ns = 1; ns <= kMaxSplits && ns <= (kv_len + 2 * kBK - 1) / (2 * kBK); ++ns) {
+    const double longest = most / ns * kTile + kBlock, sum = blocks * (mean * kTile + ns * kBlock / at_once) / cus;
+    const double join = ns > 1 ? 4.0 + double(T * H * D) * 8.0 * ns / 5e6 : 0.0;
+    const double us = (longest > sum ? longest : sum) + join;
+    if (us < least * 0.95) least = us, best = ns;  // more splits where they gain something
+  }
+#ifdef EZ_NS
+  best = EZ_NS;
+#endif
+  return {best, int(tiles), nullptr, nullptr};
 }
 int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
 
@@ -427,7 +448,7 @@ extern "C" size_t ezops_quant_prefill_attn_workspace_size(int64_t B, int64_t T, 
   if (B < 1 || T < 1 || T >= (int64_t(1) << 30) || H < 1 || H > 4096 || Hkv < 1 || H % Hkv || H / Hkv > 16 || D < 1 || D > 128 ||
       kv_len < 1)
     return 0;
-  const ez::SplitPlan pl = ez::plan(B, T, H, Hkv, kv_len);
+  const ez::SplitPlan pl = ez::plan(B, T, H, Hkv, D, kv_len);
   return pl.nsplit == 1 ? 0 : size_t(ez::up256(pl.nsplit * T * H * D * 4) + ez::up256(pl.nsplit * T * H * 8));
 }
 
@@ -449,8 +470,8 @@ extern "C" int ezops_quant_prefill_attn_bf16(const void* q, int64_t q_stride, co
   const int rc = ez::check_attn8(op, a, page_size, block_size, H, max_kv_len);
   if (rc != EZ_OK) return rc;
   ez::finish_args(a, page_size, max_kv_len);
-ez::SplitPlan pl = ez::plan(B, T, H, Hkv, a.cap);
-  const int64_t blocks = int64_t(pl.tiles) * Hkv * pl.nsplit, joins = int64_t(pl.tiles) * Hkv * (ez::kRows * D / 1024);
+ez::SplitPlan pl = ez::plan(B, T, H, Hkv, D, a.cap);
+  const int64_t blocks = int64_t(pl.tiles) * Hkv * pl.nsplit, joins = int64_t(pl.tiles) * Hkv * (ez::rows_of(D) * D / 1024);
   EZ_REQUIRE(blocks < int64_t(1) << 23 && (pl.nsplit == 1 || joins < int64_t(1) << 24), "%s: tokens * heads past one launch", op);
   if (pl.nsplit > 1) {
     const size_t need = ezops_quant_prefill_attn_workspace_size(B, T, H, Hkv, D, a.cap);
@@ -463,7 +484,7 @@ ez::SplitPlan pl = ez::plan(B, T, H, Hkv, a.cap);
   }
 #define EZ_GROUP(DD, TY, GG)                                                                                              \
   do {                                                                                                                    \
-    hipLaunchKernelGGL((ez::quant_prefill_kernel<DD, TY, GG>), dim3(unsigned(blocks)), dim3(ez::kW * ez::kWave), 0, stream, \
+    hipLaunchKernelGGL((ez::quant_prefill_kernel<DD, TY, GG>), dim3(unsigned(blocks)), dim3(ez::waves_of(DD) * ez::kWave), 0, stream, \
                        a, pl);                                                                                            \
     if (pl.nsplit > 1)                                                                                                    \
       hipLaunchKernelGGL((ez::quant_prefill_join_kernel<DD, GG>), dim3(unsigned(joins)), dim3(256), 0, stream, a, pl);    \

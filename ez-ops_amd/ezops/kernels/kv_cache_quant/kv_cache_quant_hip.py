@@ -46,8 +46,6 @@ class KvCacheQuantHipKernel(_CacheRowsKernel):
         dev = _hip.one_gpu(k, v, K_cache, V_cache, K_scale, V_scale, slot_mapping)
         k_rs, v_rs = rows16(k, "k", self._kv), rows16(v, "v", self._kv)
         _hip.check_all(self._specs, K_cache, V_cache, K_scale, V_scale, slot_mapping)
-        aligned(K_cache, "K_cache")
-        aligned(V_cache, "V_cache")
         _hip.call_on(dev, "ezops_kv_cache_quant_bf16", k.data_ptr(), k_rs, v.data_ptr(), v_rs, slot_mapping.data_ptr(),
                      K_cache.data_ptr(), V_cache.data_ptr(), K_scale.data_ptr(), V_scale.data_ptr(), *self._pool, self.T,
                      self.Hkv, self.D)
@@ -59,8 +57,6 @@ class KvCacheDequantHipKernel(_CacheRowsKernel):
     def __call__(self, K_cache, V_cache, K_scale, V_scale, slot_mapping, *, k_out=None, v_out=None):
         dev = _hip.one_gpu(K_cache, V_cache, K_scale, V_scale, slot_mapping, k_out, v_out)
         _hip.check_all(self._specs, K_cache, V_cache, K_scale, V_scale, slot_mapping)
-        aligned(K_cache, "K_cache")
-        aligned(V_cache, "V_cache")
         if k_out is None:
             k_out = torch.empty(self._kv, dtype=torch.bfloat16, device=dev)
         if v_out is None:

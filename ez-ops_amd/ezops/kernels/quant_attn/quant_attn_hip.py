@@ -54,8 +54,6 @@ class QuantPagedAttnDecodeHipKernel(_QuantAttnKernel):
         dev = _hip.one_gpu(q, K_cache, V_cache, K_scale, V_scale, block_table, kv_lens, out)
         q_rs = rows16(q, "q", self._q)
         _hip.check_all(self._specs, K_cache, V_cache, K_scale, V_scale, block_table, kv_lens)
-        aligned(K_cache, "K_cache")
-        aligned(V_cache, "V_cache")
         out = self._out_of(out, dev)
         ws, n = self._workspace(dev, max_kv_len, "ezops_quant_paged_attn_decode_workspace_size", self.B, self.H, self.Hkv,
                                 self.D)
@@ -84,8 +82,6 @@ class QuantPrefillAttnHipKernel(_QuantAttnKernel):
         _hip.check_all(self._specs, K_cache, V_cache, K_scale, V_scale, block_table, cu_seqlens)
         if past_lens is not None:
             _hip.check_all(self._past, past_lens)
-        aligned(K_cache, "K_cache")
-        aligned(V_cache, "V_cache")
         out = self._out_of(out, dev)
         ws, n = self._workspace(dev, max_kv_len, "ezops_quant_prefill_attn_workspace_size", self.B, self.T, self.H, self.Hkv,
                                 self.D)
