@@ -433,9 +433,6 @@ SplitPlan plan(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t 
     const double us = (longest > sum ? longest : sum) + join;
     if (us < least * 0.95) least = us, best = ns;  // more splits where they gain something
   }
-#ifdef EZ_NS
-  best = EZ_NS;
-#endif
   return {best, int(tiles), nullptr, nullptr};
 }
 int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }

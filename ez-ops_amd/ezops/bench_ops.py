@@ -214,7 +214,7 @@ _F1_POS: dict = {}
 
 
 # ---- QK norm + rotary positions with several axes (no reference counterpart).  The other ragged-batch ops are not
-# here: their references read lengths on the host, which no graph takes.
+# here, nor those over the 8-bit cache: their references read lengths or slots on the host, which no graph takes.
 def _mrope(T, H, Hkv, D, sections, label, **kw):
     from .ops.qk_norm_mrope import QkNormMropeOp
 
