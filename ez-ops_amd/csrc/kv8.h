@@ -34,8 +34,8 @@ inline int check_kv8(const char* op, const Kv8Args& a, int64_t page_size, int64_
   EZ_REQUIRE(a.K && a.V && a.Ks && a.Vs, "%s: null pointer", op);
   EZ_REQUIRE(a.type == kKvInt8 || a.type == kKvE4m3, "%s: cache type must be int8 (0) or e4m3 (1)", op);
   EZ_REQUIRE(page_size >= 32 && page_size <= (1 << 20) && (page_size & (page_size - 1)) == 0 && a.num_pages >= 1 &&
-                 a.num_pages < (int64_t(1) << 31),
-             "%s: page_size must be a power of two in [32, 2^20] and num_pages in [1, 2^31)", op);
+                 a.num_pages < (int64_t(1) << 31) && a.num_slots <= (int64_t(1) << 40),
+             "%s: page_size must be a power of two in [32, 2^20] and num_pages in [1, 2^31), 2^40 rows at most", op);
   EZ_REQUIRE(block >= 16 && block <= 256 && block <= page_size && (block & (block - 1)) == 0,
              "%s: block_size must be a power of two in [16, 256], at most page_size", op);
   EZ_REQUIRE(((reinterpret_cast<uintptr_t>(a.K) | reinterpret_cast<uintptr_t>(a.V)) & 15) == 0,

@@ -135,6 +135,7 @@ __device__ __forceinline__ void quant_run(const KvQuantArgs& a, int64_t t, int64
     }
     return uint32_t(__builtin_amdgcn_readfirstlane(int(m)));
   };
+  old = kv8_exp(__builtin_amdgcn_readfirstlane(old));  // here, before a wave that is done may write the new one
   uint32_t m = all_waves(max(m2 & 0xffffu, m2 >> 16));
   const bool finite = m < 0x7f80u;
   if (TYPE == kKvE4m3 && !finite) {  // the finite values alone set the scale
@@ -154,7 +155,6 @@ __device__ __forceinline__ void quant_run(const KvQuantArgs& a, int64_t t, int64
   }
   int e = TYPE == kKvInt8 && !finite ? kKvNanExp : kv8_need<TYPE>(m);
   if (off) {
-    old = kv8_exp(__builtin_amdgcn_readfirstlane(old));
     e = max(e, old);
     if (e > old) turn_rows<D, TYPE>(dst - int64_t(off) * D, off, old, e, part * kWave + lane, WPU * kWave);
   }

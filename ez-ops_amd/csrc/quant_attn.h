@@ -74,18 +74,19 @@ inline std::array<Range, 10> attn8_tensors(const QuantAttnArgs& a, int64_t H) {
            {a.kv_lens, a.B * 4}, {a.cu, (a.B + 1) * 4}, {a.past, a.B * 4}, {a.q, ((a.T - 1) * a.q_rs + row) * 2}}};
 }
 
-inline int check_attn8(const char* op, const QuantAttnArgs& a, int64_t page_size, int64_t block, int64_t H, int64_t max_kv_len) {
+// H, Hkv and D as the caller gave them: those in `a` are 32 bits of them.
+inline int check_attn8(const char* op, const QuantAttnArgs& a, int64_t page_size, int64_t block, int64_t H, int64_t Hkv,
+                       int64_t D, int64_t max_kv_len) {
   EZ_REQUIRE(a.q && a.out && a.table, "%s: null pointer", op);
+  EZ_REQUIRE(D == 64 || D == 128, "%s: head_dim must be 64 or 128", op);
+  EZ_REQUIRE(H >= 1 && Hkv >= 1 && H <= 4096 && H % Hkv == 0,
+             "%s: num_heads must be in [1, 4096] and divisible by num_kv_heads", op);
   const int rc = check_kv8(op, a.c, page_size, block);
   if (rc != EZ_OK) return rc;
   EZ_REQUIRE(a.B >= 1 && a.B <= 65536, "%s: batch must be in [1, 65536]", op);
   EZ_REQUIRE(a.T >= 1 && a.T < (int64_t(1) << 30), "%s: tokens must be in [1, 2^30)", op);
-  const int64_t Hkv = a.c.Hkv;
-  EZ_REQUIRE(H >= 1 && Hkv >= 1 && H <= 4096 && H % Hkv == 0,
-             "%s: num_heads must be in [1, 4096] and divisible by num_kv_heads", op);
   const int64_t G = H / Hkv;
   EZ_REQUIRE(G == 1 || G == 2 || G == 4 || G == 8 || G == 16, "%s: group size must be 1, 2, 4, 8 or 16", op);
-  EZ_REQUIRE(a.c.D == 64 || a.c.D == 128, "%s: head_dim must be 64 or 128", op);
   EZ_REQUIRE(a.M >= 1 && a.M * page_size <= (int64_t(1) << 30),
              "%s: max_pages must be >= 1 and max_pages * page_size at most 2^30", op);
   EZ_REQUIRE(max_kv_len >= 0, "%s: max_kv_len must be >= 0", op);

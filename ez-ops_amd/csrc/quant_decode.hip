@@ -39,7 +39,6 @@ constexpr int kW = 4;              // waves of a block
 constexpr int kT = 32;             // rows of a wave's tile
 constexpr int kMaxSplits = 32;     // chunks of a sequence
 constexpr int kSumSeqs = 1024;     // sequences whose lengths every block sums
-constexpr int kAimMany = 4096;     // rows of a chunk where there are more
 
 struct SplitPlan {
   int target;       // chunks of a kv head to aim at; 0: a block per sequence
@@ -68,8 +67,8 @@ struct Chunk {
 };
 
 // The idx-th chunk of the batch; false behind the last one.  The rows to aim at are all the
-// batch's over the chunks to aim at, so a ragged batch is shared out by rows (above 1024
-// sequences 4096, without the sum).  A sequence without rows has one (which writes its zeros).
+// batch's over the chunks to aim at, so a ragged batch is shared out by rows.  A sequence
+// without rows has one (which writes its zeros).
 __device__ __forceinline__ bool find_chunk(const QuantAttnArgs& a, int target, int idx, Chunk& c) {
   constexpr int kPer = 4;  // lengths of a lane and step
   const int lane = threadIdx.x & (kWave - 1), B = int(a.B);
@@ -90,31 +89,29 @@ __device__ __forceinline__ bool find_chunk(const QuantAttnArgs& a, int target, i
       L[i] = s < B ? seq_len(a, s) : -1;
     }
   };
-  int aim = kAimMany;
-  if (B <= kSumSeqs) {
-    float sum = 0.f;  // up to 2^10 lengths of 2^30
-    for (int b0 = 0; b0 < B; b0 += kPer * kWave) {
-      lengths(b0);
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) sum += float(max(L[i], 0));
-    }
-    // rounded up past the sums' rounding, so that the chunks stay within the blocks
-    const float per = wave_reduce_uniform<false>(sum) * 1.0001f / float(target);
-    aim = (int(per) / (kW * kT) + 1) * (kW * kT);
-  }
+  float sum = 0.f;  // up to 2^10 lengths of 2^30
   for (int b0 = 0; b0 < B; b0 += kPer * kWave) {
-    if (B > kPer * kWave || B > kSumSeqs) lengths(b0);
-    int n[kPer], sum = 0;
+    lengths(b0);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) sum += float(max(L[i], 0));
+  }
+  // Rounded up past the sum's rounding, so that the chunks stay within the blocks; from 2^30
+  // on no sequence is longer.
+  const float per = fminf(wave_reduce_uniform<false>(sum) * 1.0001f / float(target), 0x1p30f);
+  const int aim = (int(per) / (kW * kT) + 1) * (kW * kT);
+  for (int b0 = 0; b0 < B; b0 += kPer * kWave) {
+    if (B > kPer * kWave) lengths(b0);
+    int n[kPer], count = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       n[i] = L[i] < 0 ? 0 : chunk_count(L[i], aim);
-      sum += n[i];
+      count += n[i];
     }
-    const int end = wave_scan(sum);
+    const int end = wave_scan(count);
     const uint64_t hit = __ballot(idx < end);
     if (hit) {
       const int l = __ffsll(static_cast<unsigned long long>(hit)) - 1;
-      int at = idx - (__builtin_amdgcn_readlane(end, l) - __builtin_amdgcn_readlane(sum, l));
+      int at = idx - (__builtin_amdgcn_readlane(end, l) - __builtin_amdgcn_readlane(count, l));
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         const int ni = __builtin_amdgcn_readlane(n[i], l);
@@ -395,17 +392,17 @@ __global__ __launch_bounds__(256) void quant_decode_join_kernel(QuantAttnArgs a,
 // chunks than the join takes at once: 4 x 8192 rows of 32 / 8 heads 38.7 to 35.8 us); with many sequences,
 // chunks of twice the mean length, so that a long one among them is shared out.  None below a
 // tile a wave.  Sequences that are short and fill the card whole stay whole, without a join
-// (64 x 1024 rows 42.7 to 38 us, 200 of up to 1500 79 to 71).
+// (64 x 1024 rows 42.7 to 38 us, 200 of up to 1500 79 to 71), and so do more than 1024.
 SplitPlan plan(int64_t B, int64_t Hkv, int64_t kv_len) {
   const int64_t cus = num_cus();
-  if (kv_len <= kW * kT || (B * Hkv >= 2 * cus && kv_len <= 2048)) return {0, int(B), nullptr, nullptr, nullptr};
+  if (kv_len <= kW * kT || B > kSumSeqs || (B * Hkv >= 2 * cus && kv_len <= 2048)) return {0, int(B), nullptr, nullptr, nullptr};
   int64_t places = 3 * cus / Hkv;
   if (places > 16 * B) places = 2 * cus / Hkv > 16 * B ? 2 * cus / Hkv : 16 * B;
   int64_t target = places - B / 2 > B / 2 ? places - B / 2 : B / 2;
   target = target < 1 ? 1 : target;
   int64_t most = (kv_len + kW * kT - 1) / (kW * kT);  // of a sequence
   most = most < kMaxSplits ? most : kMaxSplits;
-  const int64_t blocks = B <= kSumSeqs && target + B < B * most ? target + B : B * most;
+  const int64_t blocks = target + B < B * most ? target + B : B * most;
   return {int(target), int(blocks), nullptr, nullptr, nullptr};
 }
 int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
@@ -436,7 +433,7 @@ extern "C" int ezops_quant_paged_attn_decode_bf16(const void* q, int64_t q_strid
   a.table = block_table; a.kv_lens = kv_lens;
   a.B = a.T = B; a.M = max_pages; a.H = int(H); a.scale = scale;
   EZ_REQUIRE(kv_lens, "%s: null pointer", op);
-  const int rc = ez::check_attn8(op, a, page_size, block_size, H, max_kv_len);
+  const int rc = ez::check_attn8(op, a, page_size, block_size, H, Hkv, D, max_kv_len);
   if (rc != EZ_OK) return rc;
   ez::finish_args(a, page_size, max_kv_len);
   ez::SplitPlan pl = ez::plan(B, Hkv, a.cap);

@@ -73,14 +73,19 @@ struct QueryTile {
 template <int QT>
 __device__ __forceinline__ bool find_tile(const QuantAttnArgs& a, int idx, QueryTile& q) {
   const int lane = threadIdx.x & (kWave - 1), T = int(a.T), cap = int(a.cap);
-  for (int b0 = 0; b0 < int(a.B); b0 += kWave) {
-    const int b = b0 + lane;
-    int t0 = 0, n = 0, past = 0;
-    if (b < int(a.B)) {
-      t0 = min(max(a.cu[b], 0), T);
-      past = a.past ? min(max(a.past[b], 0), cap) : 0;
-      n = min(min(max(a.cu[b + 1], 0), T) - t0, cap - past);
-    }
+  const int B = int(a.B);
+  int c0 = 0, c1 = 0, p0 = 0;  // of sequence b0 + lane, read a step ahead
+  auto ask = [&](int b) {
+    b = min(b, B - 1);
+    c0 = a.cu[b];
+    c1 = a.cu[b + 1];
+    p0 = a.past ? a.past[b] : 0;
+  };
+  ask(lane);
+  for (int b0 = 0; b0 < B; b0 += kWave) {
+    const int t0 = min(max(c0, 0), T), past = min(max(p0, 0), cap);
+    const int n = b0 + lane < B ? min(min(max(c1, 0), T) - t0, cap - past) : 0;
+    ask(b0 + kWave + lane);
     const int tiles = n > 0 ? (n + QT - 1) / QT : 0;
     const int end = wave_scan(tiles);
     const uint64_t hit = __ballot(idx < end);
@@ -464,7 +469,7 @@ extern "C" int ezops_quant_prefill_attn_bf16(const void* q, int64_t q_stride, co
   a.table = block_table; a.cu = cu_seqlens; a.past = past_lens;
   a.B = B; a.T = T; a.M = max_pages; a.H = int(H); a.scale = scale;
   EZ_REQUIRE(cu_seqlens, "%s: null pointer", op);
-  const int rc = ez::check_attn8(op, a, page_size, block_size, H, max_kv_len);
+  const int rc = ez::check_attn8(op, a, page_size, block_size, H, Hkv, D, max_kv_len);
   if (rc != EZ_OK) return rc;
   ez::finish_args(a, page_size, max_kv_len);
 ez::SplitPlan pl = ez::plan(B, T, H, Hkv, D, a.cap);

@@ -126,6 +126,14 @@ def test_decode_many_sequences(kind):
     decode(Cache(kind, lens, 2, 128, 32, 16, 1), 8)
 
 
+def test_decode_more_sequences_than_are_summed():
+    """300 (several steps of the scan, shared out by rows) and 1100 sequences (whole), a long one among short ones."""
+    for B, long in ((300, 9000), (1100, 3000)):
+        lens = [3 + i % 5 for i in range(B)]
+        lens[B // 2], lens[7], lens[B - 1] = long, 0, 1
+        decode(Cache("int8", lens, 1, 64, 32, 32, B), 2)
+
+
 @pytest.mark.parametrize("kind", KINDS)
 def test_decode_lengths_outside(kind):
     """Lengths below zero and above what the table or the bound holds."""

@@ -114,6 +114,44 @@ def test_c_entries_reject_bad_arguments():
     _refused(_prefill, dict(T=1 << 30), b"tokens")
 
 
+def test_sizes_are_checked_in_64_bits():
+    """Heads and dims whose low 32 bits would pass, and pools whose size would wrap."""
+    for fn in (_decode, _prefill):
+        for kw, text in [(dict(Hkv=(1 << 32) + 2), b"divisible"), (dict(D=(1 << 32) + 64, qs=1 << 40), b"head_dim"),
+                         (dict(H=(1 << 32) + 4, qs=1 << 40), b"num_heads"),
+                         (dict(B=(1 << 32) + 1), b"batch")]:
+            _refused(fn, kw, text)
+    for fn in (_quant, _dequant):
+        for kw, text in [(dict(Hkv=(1 << 32) + 2), b"num_kv_heads"), (dict(D=(1 << 32) + 64), b"head_dim"),
+                         (dict(T=(1 << 32) + 1), b"tokens")]:
+            _refused(fn, kw, text)
+    for fn in (_quant, _dequant, _decode, _prefill):
+        for kw in (dict(P=1 << 20, NP=(1 << 20) + 1), dict(P=(1 << 32) + 64), dict(blk=(1 << 32) + 32), dict(NP=(1 << 32) + 4)):
+            _refused(fn, kw, b"page_size", b"block_size")
+
+
+def test_workspaces_are_checked_before_any_launch():
+    lib = _hip.lib()
+    need = lib.ezops_quant_paged_attn_decode_workspace_size(2, 4, 2, 64, 128)
+    assert need == 0 and lib.ezops_quant_paged_attn_decode_workspace_size(2, 4, 2, 64, 0) == 0
+    need = lib.ezops_quant_paged_attn_decode_workspace_size(2, 4, 2, 64, 4096)
+    assert 0 < need < 1 << 24
+    for kw in (dict(ws=None), dict(nb=need - 1), dict(ws=AT[9] + 8), dict(ws=AT[1]), dict(ws=AT[3] + 64), dict(ws=AT[8])):
+        _refused(_decode, dict(M=64, NP=200, **kw), b"workspace")
+    # a bound on the lengths plans the work: what is enough for it may be too little without it
+    short = lib.ezops_quant_paged_attn_decode_workspace_size(2, 4, 2, 64, 256)
+    assert 0 < short < need
+    _refused(_decode, dict(M=64, NP=200, nb=short), b"workspace too small")
+    need = lib.ezops_quant_prefill_attn_workspace_size(2, 8, 4, 2, 64, 8192)
+    assert need > 0 and lib.ezops_quant_prefill_attn_workspace_size(2, 8, 4, 2, 64, 64) == 0
+    for kw in (dict(ws=None), dict(nb=need - 1), dict(ws=AT[9] + 8), dict(ws=AT[0] + 16), dict(ws=AT[7])):
+        _refused(_prefill, dict(M=128, NP=300, **kw), b"workspace")
+    # many sequences stay whole, so that the workspace does not grow with them
+    for B in (1, 7, 64, 300, 1024):
+        assert lib.ezops_quant_paged_attn_decode_workspace_size(B, 32, 8, 128, 1 << 20) <= (B + 96 + B // 2) * 32 * 520 + B * 64 + 1024
+    assert lib.ezops_quant_paged_attn_decode_workspace_size(1025, 32, 8, 128, 1 << 20) == 0
+
+
 def test_c_entries_reject_overlaps():
     pool, sc = 4 * 2 * 64 * 64, 4 * 2 * 2
     for kw in (dict(K=AT[0]), dict(V=AT[1] - pool + 16), dict(Ks=AT[2] + 8), dict(Vs=AT[0] + 256), dict(K=AT[2] - 16)):
