@@ -24,6 +24,9 @@
 //
 // Where the queries are few (a chunk on a long prefix) the keys are shared out over
 // nsplit blocks; they leave fp32 partials (O, m, l), which a second kernel joins.
+#include <algorithm>
+#include <cmath>
+
 #include "common.h"
 #include "internal.h"
 #include "prof.h"
@@ -417,25 +420,30 @@ __global__ __launch_bounds__(256) void quant_prefill_join_kernel(QuantAttnArgs a
 
 // Query tiles at most (a sequence adds at most one that is not full), and the splits of
 // the keys that a model of the time prefers, in us: a block takes kBlock to begin and end and
-// kTile a key tile; the longest block and the blocks' sum over the CUs each bound the
-// kernel; splits add a join and their partials through memory.  The key tiles of a block
-// are at most those of kv_len, on average those of one prompt whose last row that is, or
-// half where there are several sequences.  (70 tokens on 3000 rows of 32 / 8 heads: 6, 12, 16
-// and 24 splits take 32.7, 28.7, 28.7 and 37 us; nine ragged chunks of 2660 tokens of 16 / 2 heads of 64 on up to
-// 2500 rows 61 us with one, 58 with two.)
+// kTile a key tile; the kernel lasts as long as its longest block, as the blocks' sum over
+// the CUs, and with several sequences, whose blocks come in no order of size, as whole rounds
+// of them; splits add a join and their partials through memory.  The longest block has the
+// key tiles of kv_len, a mean one those of the middle row of one prompt that ends there, or
+// three quarters where there are several sequences (the lengths are on the device).  70
+// tokens on 3000 rows of 32 / 8 heads: 6, 12, 16 and 24 splits take 32.7, 28.7, 28.7 and
+// 37 us; 16 x 16 tokens on 2000 rows 56.8, 49.9 and 58 us with one, two and three; nine
+// ragged chunks of 2660 tokens of 16 / 2 heads of 64 on up to 2500 rows 61 and 58 us with
+// one and two.
 SplitPlan plan(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t kv_len) {
-  const int64_t qt = rows_of(D) / (H / Hkv);
-  const int64_t tiles = (T + (B < T ? B : T) * (qt - 1)) / qt;
-  const double blocks = double(tiles * Hkv), cus = num_cus();
+  const int64_t qt = rows_of(D) / (H / Hkv), seqs = B < T ? B : T;
+  const int64_t tiles = (T + seqs * (qt - 1)) / qt;
+  const double blocks = double(seqs * ((T / seqs + qt - 1) / qt) * Hkv), cus = num_cus();
   const double kTile = D == 64 ? 1.2 : 2.2, kBlock = 7.0, at_once = D == 64 ? 3.0 : 1.0;
   const double most = double(kv_len) / kBK + 1;
-  const double mean = B == 1 && kv_len > T ? double(kv_len - T / 2) / kBK : most / 2;
+  const double mean = seqs > 1 ? most * 0.75 : kv_len > T ? double(kv_len - T / 2) / kBK : most / 2;
   int best = 1;
   double least = 1e30;
   for (int ns = 1; ns <= kMaxSplits && ns <= (kv_len + 2 * kBK - 1) / (2 * kBK); ++ns) {
     const double longest = most / ns * kTile + kBlock, sum = blocks * (mean * kTile + ns * kBlock / at_once) / cus;
+    const double rounds = seqs > 1 ? std::ceil(blocks * ns / (cus * at_once)) : 1.0;
+    const double whole = rounds > 1 ? rounds * (at_once * mean / ns * kTile + kBlock) : 0.0;
     const double join = ns > 1 ? 4.0 + double(T * H * D) * 8.0 * ns / 5e6 : 0.0;
-    const double us = (longest > sum ? longest : sum) + join;
+    const double us = std::max(std::max(longest, sum), whole) + join;
     if (us < least * 0.95) least = us, best = ns;  // more splits where they gain something
   }
   return {best, int(tiles), nullptr, nullptr};
