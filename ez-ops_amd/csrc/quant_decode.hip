@@ -411,6 +411,9 @@ SplitPlan plan(int64_t B, int64_t Hkv, int64_t kv_len) {
   return {int(target), int(blocks), nullptr, nullptr, nullptr};
 }
 int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
+size_t ws_size(const SplitPlan& pl, int64_t B, int64_t H, int64_t Hkv, int64_t D) {
+  return pl.target == 0 ? 0 : size_t(up256(pl.blocks * H * D * 4) + up256(pl.blocks * H * 8) + up256(B * Hkv * 8));
+}
 
 }  // namespace
 }  // namespace ez
@@ -420,8 +423,7 @@ extern "C" size_t ezops_quant_paged_attn_decode_workspace_size(int64_t B, int64_
   if (B < 1 || B > 65536 || H < 1 || H > 4096 || Hkv < 1 || H % Hkv || D < 1 || D > 128 || kv_len < 1 ||
       kv_len > (int64_t(1) << 30))
     return 0;
-  const ez::SplitPlan pl = ez::plan(B, Hkv, kv_len);
-  return pl.target == 0 ? 0 : size_t(ez::up256(pl.blocks * H * D * 4) + ez::up256(pl.blocks * H * 8) + ez::up256(B * Hkv * 8));
+  return ez::ws_size(ez::plan(B, Hkv, kv_len), B, H, Hkv, D);
 }
 
 extern "C" int ezops_quant_paged_attn_decode_bf16(const void* q, int64_t q_stride, const void* K_cache, const void* V_cache,
@@ -445,7 +447,7 @@ extern "C" int ezops_quant_paged_attn_decode_bf16(const void* q, int64_t q_strid
   const int64_t blocks = Hkv * pl.blocks, joins = (B * H * (D / 4) + 255) / 256;
   EZ_REQUIRE(blocks < int64_t(1) << 24, "%s: batch * heads past one launch", op);
   if (pl.target) {
-    const size_t need = ezops_quant_paged_attn_decode_workspace_size(B, H, Hkv, D, a.cap);
+    const size_t need = ez::ws_size(pl, B, H, Hkv, D);
     EZ_REQUIRE(ws && ws_bytes >= need, "%s: workspace too small (%zu < %zu)", op, ws_bytes, need);
     EZ_REQUIRE(ez::kv8_aligned16(ws), "%s: workspace must be 16-byte aligned", op);
     for (const auto& x : ez::attn8_tensors(a, H))

@@ -113,8 +113,11 @@ __device__ __forceinline__ bool find_tile(const QuantAttnArgs& a, int idx, Query
   return false;
 }
 
-// Key tiles of a split of the tile's `n` key tiles, and how many splits have any.
-__device__ __forceinline__ int split_tiles(int n, int nsplit) { return (n + nsplit - 1) / nsplit; }
+// Key tiles of a split of the tile's `n` key tiles; splits behind the last one with any leave.
+// The host plans with a bound on the lengths that may be far above them: three tiles at least
+// (70 tokens on 3000 rows planned for 131072: 37 us with 32 splits, two tiles each).
+constexpr int kMinTiles = 3;
+__device__ __forceinline__ int split_tiles(int n, int nsplit) { return max((n + nsplit - 1) / nsplit, kMinTiles); }
 
 __device__ __forceinline__ bool has_nan_code(uint32_t w) {  // an e4m3 byte of 0x7f or 0xff
   const uint32_t x = (w & 0x7f7f7f7fu) ^ 0x7f7f7f7fu;
@@ -456,6 +459,9 @@ SplitPlan plan(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t 
   return {best, int(tiles), nullptr, nullptr};
 }
 int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
+size_t ws_size(const SplitPlan& pl, int64_t T, int64_t H, int64_t D) {
+  return pl.nsplit == 1 ? 0 : size_t(up256(pl.nsplit * T * H * D * 4) + up256(pl.nsplit * T * H * 8));
+}
 
 }  // namespace
 }  // namespace ez
@@ -465,8 +471,7 @@ extern "C" size_t ezops_quant_prefill_attn_workspace_size(int64_t B, int64_t T, 
   if (B < 1 || T < 1 || T >= (int64_t(1) << 30) || H < 1 || H > 4096 || Hkv < 1 || H % Hkv || H / Hkv > 16 || D < 1 || D > 128 ||
       kv_len < 1)
     return 0;
-  const ez::SplitPlan pl = ez::plan(B, T, H, Hkv, D, kv_len);
-  return pl.nsplit == 1 ? 0 : size_t(ez::up256(pl.nsplit * T * H * D * 4) + ez::up256(pl.nsplit * T * H * 8));
+  return ez::ws_size(ez::plan(B, T, H, Hkv, D, kv_len), T, H, D);
 }
 
 extern "C" int ezops_quant_prefill_attn_bf16(const void* q, int64_t q_stride, const void* K_cache, const void* V_cache,
@@ -491,7 +496,7 @@ ez::SplitPlan pl = ez::plan(B, T, H, Hkv, D, a.cap);
   const int64_t blocks = int64_t(pl.tiles) * Hkv * pl.nsplit, joins = int64_t(pl.tiles) * Hkv * (ez::rows_of(D) * D / 1024);
   EZ_REQUIRE(blocks < int64_t(1) << 23 && (pl.nsplit == 1 || joins < int64_t(1) << 24), "%s: tokens * heads past one launch", op);
   if (pl.nsplit > 1) {
-    const size_t need = ezops_quant_prefill_attn_workspace_size(B, T, H, Hkv, D, a.cap);
+    const size_t need = ez::ws_size(pl, T, H, D);
     EZ_REQUIRE(ws && ws_bytes >= need, "%s: workspace too small (%zu < %zu)", op, ws_bytes, need);
     EZ_REQUIRE(ez::kv8_aligned16(ws), "%s: workspace must be 16-byte aligned", op);
     for (const auto& x : ez::attn8_tensors(a, H))

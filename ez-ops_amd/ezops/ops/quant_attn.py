@@ -47,10 +47,10 @@ class _QuantAttnOp(Op):
             raise ValueError(f"num_heads ({num_heads}) must be divisible by num_kv_heads ({num_kv_heads}) and at most 4096")
         if num_heads // num_kv_heads not in GROUPS:
             raise ValueError(f"GQA group size {num_heads}/{num_kv_heads} not supported (1, 2, 4, 8 or 16)")
-        num_pages = batch * max_pages if num_pages is None else num_pages
-        check_cache(page_size, num_pages, block_size, cache_dtype, head_dim)
         if max_pages < 1 or max_pages * page_size > 1 << 30:
             raise ValueError(f"max_pages ({max_pages}) must be >= 1 and max_pages * page_size at most 2^30")
+        num_pages = batch * max_pages if num_pages is None else num_pages
+        check_cache(page_size, num_pages, block_size, cache_dtype, head_dim)
         self.batch, self.num_heads, self.num_kv_heads, self.head_dim = batch, num_heads, num_kv_heads, head_dim
         self.page_size, self.max_pages, self.num_pages = page_size, max_pages, num_pages
         self.cache_dtype, self.block_size, self.scale = cache_dtype, block_size, _scale(scale, head_dim)

@@ -297,6 +297,38 @@ def test_attention_past_32_bits():
 
 
 @pytest.mark.parametrize("kind", KINDS)
+def test_wide_tables(kind):
+    """Tables for 2^16 and more rows a sequence that hold a few hundred: plans for what could be, work for what is."""
+    c = Cache(kind, [300, 33, 700, 1], 2, 128, 64, 32, 12, extra=1020)
+    decode(c, 8)
+    prefill(c, 8, [20, 33, 1, 0], [280, 0, 699, 1])
+    prefill(Cache(kind, [515], 1, 64, 64, 16, 13, extra=2000), 4, [70], [445])
+
+
+def test_two_streams_at_once():
+    """The same ops on two streams that run together: neither disturbs the other."""
+    c = Cache("e4m3", [3000, 90, 1500], 2, 128, 64, 32, 14)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    dec = QuantPagedAttnDecodeOp(3, 8, 2, 128, 64, c.M, c.pages, **c.how)
+    pre = QuantPrefillAttnOp(3, 40, 8, 2, 128, 64, c.M, c.pages, **c.how)
+    lens, cu, past = torch.tensor(c.lens, **i32), torch.tensor([0, 20, 37, 40], **i32), torch.tensor([2980, 73, 1497], **i32)
+    qs = [(c.q(3, 8), c.q(40, 8)) for _ in range(2)]
+    both = lambda q: (dec(q[0], *c.pools, c.t, lens), pre(q[1], *c.pools, c.t, cu, past))  # noqa: E731
+    want = [both(q) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in qs]
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(both(qs[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out in got[i]:
+            assert torch.equal(out[0], want[i][0]) and torch.equal(out[1], want[i][1])
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_captured_calls(kind):
     """Two graphs of both ops, replayed in turn with eager calls between: every replay equals the eager result."""
     c = Cache(kind, [700, 90, 33], 2, 128, 64, 32, 10)

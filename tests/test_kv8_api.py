@@ -41,7 +41,7 @@ def test_constructor_refusals():
     for args, kw, text in [((0, 4, 2, 64, 64, 4), {}, "batch"), ((65537, 4, 2, 64, 64, 4), {}, "batch"),
                            ((1, 4, 3, 64, 64, 4), {}, "divisible"), ((1, 6, 2, 64, 64, 4), {}, "group size"),
                            ((1, 4, 2, 80, 64, 4), {}, "head_dim"), ((1, 4, 2, 64, 40, 4), {}, "page_size"),
-                           ((1, 4, 2, 64, 64, 0), dict(num_pages=1), "max_pages"),
+                           ((1, 4, 2, 64, 64, 0), dict(num_pages=1), "max_pages"), ((1, 4, 2, 64, 64, 0), {}, "max_pages"),
                            ((1, 4, 2, 64, 64, 1 << 25), {}, "max_pages"), ((1, 4, 2, 64, 64, 4, 0), {}, "num_pages"),
                            ((1, 4, 2, 64, 64, 4), dict(scale=0.0), "scale"),
                            ((1, 4, 2, 64, 64, 4), dict(block_size=128), "block_size"),
