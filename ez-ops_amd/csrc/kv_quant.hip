@@ -9,16 +9,16 @@
 // so every row is rounded against the scale that its block has after the call.
 //
 // Both directions are memory traffic: 2 bytes a value in, 1 out, or the reverse.  A unit
-// is one wave (blocks of up to 64 tokens) or the four waves of a block (128 and 256):
-// the run's rows are read once, whole rows by 16-byte loads, and wait in registers (64
-// at most) for the maximum over all of them.  A wave looks at a window of tokens: one
+// is one wave (blocks of few rows) or the four or eight waves of a block: the run's
+// rows are read once, whole rows by 16-byte loads, and wait in registers (32 at most) for
+// the maximum over all of them.  A wave looks at a window of tokens: one
 // load of 64 slots tells which of them begin a run and how long it is; runs of one token
 // (a decode step) go several to a wave, a row to each 8 or 16 lanes.
 //
-// Measured: 16384 tokens of 8 heads of 128 written in 27 us (3.7 TB/s; the registers of a
-// block of 64 rows leave two waves a SIMD) and read back in 16, which together take 50 us a
-// call on inputs that no cache holds (a large copy of as many bytes 39); 40000 rows read back
-// in 51 us, 5.0 TB/s (copy 5.1); 64 single tokens 3.4 us, a launch and two dependent loads.
+// Measured: 16384 tokens of 8 heads of 128 written in 18 us and read back in 16
+// where the memory-side cache holds some of them; 45 us a call of both on inputs that no
+// cache holds (a large copy of as many bytes 39).  40000 rows read back in 51 us, 5.0 TB/s
+// (copy 5.1); 64 single tokens 3.4 us, a launch and two dependent loads.
 #include "common.h"
 #include "internal.h"
 #include "kv8.h"
@@ -47,8 +47,6 @@ struct KvDequantArgs {
 };
 
 __device__ __forceinline__ bool slot_ok(int64_t s, int64_t n) { return s >= 0 && s < n; }
-
-constexpr int kChunk = 32;  // rows of a wave's registers at a time
 
 __device__ __forceinline__ uint32_t pk_max_u16(uint32_t a, uint32_t b) {
   typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
@@ -95,12 +93,12 @@ __device__ __forceinline__ void turn_rows(uint8_t* rows, int n, int old, int e, 
   }
 }
 
-// Rows [t, t + n) of one head into the block that holds slot `slot`, WPU waves of the
-// block together, `part` of them this one; NC chunks of rows a wave (n <= 32 NC WPU).
-template <int D, int TYPE, int NC, int WPU>
+// Rows [t, t + n) of one head into the block that holds slot `slot`, WPU waves together,
+// `part` of them this one; CH rows a wave (n <= CH WPU).
+template <int D, int TYPE, int CH, int WPU>
 __device__ __forceinline__ void quant_run(const KvQuantArgs& a, int64_t t, int64_t slot, int n, int h, bool is_v, int part,
                                           uint32_t* shared_max) {
-  constexpr int LPR = D / 8, RPI = kWave / LPR, NI = kChunk / RPI;  // lanes of a row, rows and loads
+  constexpr int LPR = D / 8, RPI = kWave / LPR, NI = CH / RPI;  // lanes of a row, rows of a load, loads
   const int lane = threadIdx.x & (kWave - 1);
   const int off = int(slot) & ((1 << a.c.block_sh) - 1);
   const int64_t rs = is_v ? a.v_rs : a.k_rs;
@@ -108,28 +106,24 @@ __device__ __forceinline__ void quant_run(const KvQuantArgs& a, int64_t t, int64
   const int64_t row0 = (((slot >> a.c.page_sh) * a.c.Hkv + h) << a.c.page_sh) + (slot & ((int64_t(1) << a.c.page_sh) - 1));
   uint8_t* sp = (is_v ? a.c.Vs : a.c.Ks) + (row0 >> a.c.block_sh);
   uint8_t* dst = (is_v ? a.c.V : a.c.K) + row0 * D;
-  const int r0 = part * NC * kChunk + lane / LPR;
+  const int r0 = part * CH + lane / LPR;
   int old = off ? int(*sp) : 0;
-  uint4 x[NC][NI];
+  uint4 x[NI];
   uint32_t m2 = 0;
 #pragma unroll
-  for (int c = 0; c < NC; ++c)
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      x[c][i] = make_uint4(0, 0, 0, 0);
-      if (part * NC * kChunk + c * kChunk + i * RPI < n) {
-        const int r = r0 + c * kChunk + i * RPI;
-        if (r < n) x[c][i] = *reinterpret_cast<const uint4*>(src + r * rs);
-      }
+  for (int i = 0; i < NI; ++i) {
+    x[i] = make_uint4(0, 0, 0, 0);
+    if (part * CH + i * RPI < n) {
+      const int r = r0 + i * RPI;
+      if (r < n) x[i] = *reinterpret_cast<const uint4*>(src + r * rs);
     }
+  }
 #pragma unroll
-  for (int c = 0; c < NC; ++c)
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const uint32_t mask = 0x7fff7fffu;
-      const uint4 v = x[c][i];
-      m2 = pk_max_u16(m2, pk_max_u16(pk_max_u16(v.x & mask, v.y & mask), pk_max_u16(v.z & mask, v.w & mask)));
-    }
+  for (int i = 0; i < NI; ++i) {
+    const uint32_t mask = 0x7fff7fffu;
+    const uint4 v = x[i];
+    m2 = pk_max_u16(m2, pk_max_u16(pk_max_u16(v.x & mask, v.y & mask), pk_max_u16(v.z & mask, v.w & mask)));
+  }
   auto all_waves = [&](uint32_t m) {
     m = wave_max_u32(m);
     if constexpr (WPU > 1) {
@@ -146,16 +140,14 @@ __device__ __forceinline__ void quant_run(const KvQuantArgs& a, int64_t t, int64
   if (TYPE == kKvE4m3 && !finite) {  // the finite values alone set the scale
     m = 0;
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
+    for (int i = 0; i < NI; ++i) {
+      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const uint32_t w[4] = {x[c][i].x, x[c][i].y, x[c][i].z, x[c][i].w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t lo = w[k] & 0x7fffu, hi = (w[k] >> 16) & 0x7fffu;
-          m = max(m, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
-        }
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t lo = w[k] & 0x7fffu, hi = (w[k] >> 16) & 0x7fffu;
+        m = max(m, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
       }
+    }
     m = all_waves(m);
   }
   int e = TYPE == kKvInt8 && !finite ? kKvNanExp : kv8_need<TYPE>(m);
@@ -164,14 +156,12 @@ __device__ __forceinline__ void quant_run(const KvQuantArgs& a, int64_t t, int64
     if (e > old) turn_rows<D, TYPE>(dst - int64_t(off) * D, off, old, e, part * kWave + lane, WPU * kWave);
   }
 #pragma unroll
-  for (int c = 0; c < NC; ++c)
-#pragma unroll
-    for (int i = 0; i < NI; ++i)
-      if (part * NC * kChunk + c * kChunk + i * RPI < n) {
-        const int r = r0 + c * kChunk + i * RPI;
-        const uint2 w = to_codes<TYPE>(x[c][i], e, finite);
-        if (r < n) *reinterpret_cast<uint2*>(dst + r * D + lane % LPR * 8) = w;
-      }
+  for (int i = 0; i < NI; ++i)
+    if (part * CH + i * RPI < n) {
+      const int r = r0 + i * RPI;
+      const uint2 w = to_codes<TYPE>(x[i], e, finite);
+      if (r < n) *reinterpret_cast<uint2*>(dst + r * D + lane % LPR * 8) = w;
+    }
   if (lane == 0 && part == 0) *sp = uint8_t(e);
 }
 
@@ -223,11 +213,11 @@ __device__ __forceinline__ void quant_singles(const KvQuantArgs& a, int64_t t, i
   if (c == 0) *sp = uint8_t(e);
 }
 
-template <int D, int TYPE, int NC, int WPU>
-__global__ __launch_bounds__(256) void kv_quant_kernel(KvQuantArgs a, int window) {
+template <int D, int TYPE, int CH, int WPU>
+__global__ __launch_bounds__(WPU > 4 ? WPU * kWave : 256) void kv_quant_kernel(KvQuantArgs a, int window) {
   EZ_PROF_WAVE(kProfKvQuant);
   constexpr int LPR = D / 8, RPI = kWave / LPR;
-  __shared__ uint32_t shared_max[4];
+  __shared__ uint32_t shared_max[WPU];
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t u = WPU == 1 ? int64_t(blockIdx.x) * 4 + wave : int64_t(blockIdx.x);
   const int units = 2 * a.c.Hkv;  // of a window
@@ -277,7 +267,7 @@ __global__ __launch_bounds__(256) void kv_quant_kernel(KvQuantArgs a, int window
         if (more < 64) break;
       }
     }
-    quant_run<D, TYPE, NC, WPU>(a, t, slot, n, h, hv & 1, WPU == 1 ? 0 : wave, shared_max);
+    quant_run<D, TYPE, CH, WPU>(a, t, slot, n, h, hv & 1, WPU == 1 ? 0 : wave, shared_max);
   }
 }
 
@@ -365,20 +355,29 @@ extern "C" int ezops_kv_cache_quant_bf16(const void* k, int64_t k_stride, const 
   a.slots = slot_mapping; a.T = T;
   // Tokens a wave looks at: as many as leave 4096 waves.  In a prompt most tokens begin no
   // run, and a wave that finds none still holds its place for two loads (16384 tokens of
-  // 8 heads in blocks of 64: 82 us with 8 tokens a wave, 47, 33 and 27 with 16, 32 and 64;
+  // 8 heads in blocks of 64: 82 us with 8 tokens a wave, 47, 33 and 27 with 16, 32 and 64, one wave a run;
   // a mixed step of 3500 tokens 10.6, 9.2, 8.8 and 10.0 us at 2, 4, 8 and 16).
   int window = 1;
   while (window < 64 && T * Hkv * 2 / window > 4096) window *= 2;
-  const int64_t units = (T + window - 1) / window * Hkv * 2, blocks = block_size <= 64 ? (units + 3) / 4 : units;
-  EZ_REQUIRE(blocks < int64_t(1) << 24, "%s: tokens * heads past one launch", op);
-#define EZ_RUN(DD, TY, NC, WPU) \
-  hipLaunchKernelGGL((ez::kv_quant_kernel<DD, TY, NC, WPU>), dim3(unsigned(blocks)), dim3(256), 0, stream, a, window)
-#define EZ_GO(DD, TY)                               \
-  do {                                              \
-    if (block_size <= 32) EZ_RUN(DD, TY, 1, 1);     \
-    else if (block_size == 64) EZ_RUN(DD, TY, 2, 1); \
-    else if (block_size == 128) EZ_RUN(DD, TY, 1, 4); \
-    else EZ_RUN(DD, TY, 2, 4);                      \
+  const int64_t units = (T + window - 1) / window * Hkv * 2;
+  // Rows of a wave and waves of a run: 32 registers of values a lane at most, and 16 where
+  // four waves hold a whole block in that (16384 tokens of heads of 128 in blocks of 64: two
+  // waves a SIMD with 64 registers 50.6 us with the read-back, 45 so; three prompts of 5250
+  // in blocks of 256 53.4, with eight waves 51; heads of 64 so 28.4 and 35.5, but 26.6 and 31.3
+  // with the rows of half as many bytes that they have).
+#define EZ_RUN(DD, TY, CH, WPU)                                                                              \
+  do {                                                                                                       \
+    constexpr int threads = (WPU) > 4 ? (WPU) * 64 : 256;                                                    \
+    const int64_t blocks = (WPU) == 1 ? (units + 3) / 4 : units;                                             \
+    EZ_REQUIRE(blocks < (int64_t(1) << 32) / threads, "%s: tokens * heads past one launch", op);             \
+    hipLaunchKernelGGL((ez::kv_quant_kernel<DD, TY, CH, WPU>), dim3(unsigned(blocks)), dim3(threads), 0, stream, a, window); \
+  } while (0)
+#define EZ_GO(DD, TY)                                                                      \
+  do {                                                                                     \
+    if (block_size <= 32) EZ_RUN(DD, TY, 32, 1);                                           \
+    else if (block_size == 64) EZ_RUN(DD, TY, (DD == 64 ? 64 : 16), (DD == 64 ? 1 : 4));   \
+    else if (block_size == 128) EZ_RUN(DD, TY, 32, 4);                                     \
+    else EZ_RUN(DD, TY, (DD == 64 ? 64 : 32), (DD == 64 ? 4 : 8));                         \
   } while (0)
   EZ_KV8_DISPATCH(EZ_GO);
 #undef EZ_GO
