@@ -102,6 +102,31 @@ def test_not_finite(kind):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("block", [16, 32, 64, 128, 256])
+def test_every_block_and_head_size(kind, D, block):
+    """Runs that begin, go on, fill and leave a block, single tokens between them, and values that are not finite."""
+    Hkv, P = 2, 256
+    g = torch.Generator().manual_seed(block + D)
+    lens = [(block // 2 - 1, 0), (1, 3), (2 * block + 5, block - 7), (1, block - 1), (block, 0), (P - 1, 1), (3, 0), (0, 9)]
+    slots = plan(lens, P, torch.randperm(20, generator=g).tolist())
+    T = len(slots)
+    op = KvCacheQuantOp(T, Hkv, D, P, 20, backend="hip", cache_dtype=KINDS[kind], block_size=block)
+    pools = junk_pools(g, op)
+    pools[2][:, :, ::2], pools[3][:, :, 1::2] = 125, 121
+    want = [raw(p).copy() for p in pools]
+    for bad in ((), (0, T // 3, T // 2, T - 1)):
+        k, v = tokens(g, T, Hkv, D, False)
+        for t in bad:
+            k[t, 0, 7], v[t, 1, D - 1], v[t, 0, 0] = float("nan"), float("inf"), -float("inf")
+        for x, c, s in ((k, 0, 2), (v, 1, 3)):
+            kv8.write(n64(x), want[c], want[s], slots, block, kind)
+        op(k, v, *pools, torch.tensor(slots, device=DEV))
+        for name, p, w in zip(("K", "V", "Ks", "Vs"), pools, want):
+            np.testing.assert_array_equal(raw(p), w, err_msg=name)
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_growth_token_by_token(kind):
     """Blocks that grow at nearly every token, as decode steps do it."""
     B, Hkv, D, P, block = 7, 2, 128, 64, 64
