@@ -39,7 +39,6 @@ namespace ez {
 EZ_PROF_DEFINE(quantdecode)
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kW = 4;              // waves of a block
 constexpr int kT = 32;             // rows of a wave's tile
 constexpr int kMaxSplits = 32;     // chunks of a sequence
@@ -239,7 +238,6 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(3)))
 #pragma unroll
     for (int d = 0; d < NDB; ++d) voff[d] = row * D + ((d ^ vswz(row)) * 16) + 8 * (li & 1);
   }
-  const float sl2 = a.scale * kLog2e;
 
   // Lane (li, lg): head li's reference m, its share of the sum, O^T[16 d + 4 lg + r][li] in o[d][r]
   float m = kLowest, l = 0.f;
@@ -253,7 +251,7 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(3)))
 #pragma unroll
     for (int i = 0; i < NL; ++i) *reinterpret_cast<uint4*>(ks + (i * kWave + lane) * 16) = kn[i];
     const int e = kv8_exp(en);
-    const float cv = lane & 2 ? (e == kKvNanExp ? __uint_as_float(0x7fc00000u) : float(e - 127)) : sl2 * kv8_scale(e);
+    const float cv = lane & 2 ? (e == kKvNanExp ? __uint_as_float(0x7fc00000u) : float(e - 127)) : kv8_factor(a.scale, e);
     const int iv = e == kKvNanExp ? 127 : 254 - e;
     at = flat_row(tn, id);
     load_k(tn, at);

@@ -46,7 +46,6 @@ namespace ez {
 EZ_PROF_DEFINE(quantprefill)
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.f;     // log2 headroom of the softmax reference, see below
 // Waves of a block, 32 (query, head) rows each.
 constexpr int waves_of(int64_t D) { return D == 64 ? 4 : 8; }
@@ -166,7 +165,6 @@ __global__ __launch_bounds__(waves_of(D) * kWave) __attribute__((amdgpu_waves_pe
   const int wave_q0 = qt.first + wave * 32 / G;
   const bool wave_on = wave_q0 < qt.qlen;
   const int wave_first = qt.past + wave_q0, wave_last = qt.past + min(qt.first + (wave * 32 + 31) / G, qt.qlen - 1);
-  const float sl2 = a.scale * kLog2e;
 
   bf16x8_t qf[NS];
   {
@@ -225,7 +223,7 @@ __global__ __launch_bounds__(waves_of(D) * kWave) __attribute__((amdgpu_waves_pe
     if (stage_c) {
       const int k = kv8_exp(ek[buf]), v = kv8_exp(ev[buf]), u = sr / 16;
       const bool nan = v == kKvNanExp;
-      Cs[buf][u] = sl2 * kv8_scale(k);
+      Cs[buf][u] = kv8_factor(a.scale, k);
       Cs[buf][4 + u] = nan ? __uint_as_float(0x7fc00000u) : float(v - 127);
       Cs[buf][8 + u] = __uint_as_float(nan ? 0x3f803f80u : uint32_t(254 - v) << 7 | uint32_t(254 - v) << 23);
     }

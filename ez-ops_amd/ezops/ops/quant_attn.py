@@ -13,7 +13,9 @@ rows ``0 .. past_lens[b] + i`` for the sequence's new token ``i`` (prefill; the 
 are in the cache already).  Query head ``h`` reads kv head ``h // (H / Hkv)``;
 ``block_table [B, max_pages]`` (int32) maps logical pages to pool pages.  Ids of pages that
 hold visible rows must lie in the pool (others are read as a page of it); codes and scales
-of rows that no query sees may hold anything.
+of rows that no query sees may hold anything.  Any positive scale of fp32 may be asked for;
+the products of q with a row's codes have to stay below 2^128 (as does a score), past which
+the query's own output is undefined.
 """
 
 import torch

@@ -333,7 +333,8 @@ int ezops_kv_cache_dequant_bf16(const void* K_cache, const void* V_cache, const 
  * that is > 0), one without rows gets zeros.  max_kv_len plans the work.  Page ids outside
  * the pool are clamped into it; codes and scales of rows behind a length may hold
  * anything.  H / Hkv in {1, 2, 4, 8, 16}, D in {64, 128}, B <= 65536, H <= 4096; scale <= 0
- * selects 1/sqrt(D).  workspace: 16-byte aligned,
+ * selects 1/sqrt(D).  Products of q with a row's codes have to stay below 2^128, as scores
+ * do; past that the query's own output is undefined.  workspace: 16-byte aligned,
  * ezops_quant_paged_attn_decode_workspace_size(B, H, Hkv, D, max_kv_len or max_pages *
  * page_size) bytes, need not be zero-filled (NULL where that is 0).
  * No counterpart in the reference (bf16 cache, ezops/ops/attn_decode.py:9-67). */
