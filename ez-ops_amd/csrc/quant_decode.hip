@@ -418,10 +418,9 @@ size_t ws_size(const SplitPlan& pl, int64_t B, int64_t H, int64_t Hkv, int64_t D
 
 extern "C" size_t ezops_quant_paged_attn_decode_workspace_size(int64_t B, int64_t H, int64_t Hkv, int64_t D,
                                                                int64_t kv_len) {
-  if (B < 1 || B > 65536 || H < 1 || H > 4096 || Hkv < 1 || H % Hkv || D < 1 || D > 128 || kv_len < 1 ||
-      kv_len > (int64_t(1) << 30))
-    return 0;
-  return ez::ws_size(ez::plan(B, Hkv, kv_len), B, H, Hkv, D);
+  if (B < 1 || B > 65536 || H < 1 || H > 4096 || Hkv < 1 || H % Hkv || D < 1 || D > 128 || kv_len < 1) return 0;
+  const int64_t most = int64_t(1) << 30;  // rows of a table; the size grows with the bound up to there
+  return ez::ws_size(ez::plan(B, Hkv, kv_len < most ? kv_len : most), B, H, Hkv, D);
 }
 
 extern "C" int ezops_quant_paged_attn_decode_bf16(const void* q, int64_t q_stride, const void* K_cache, const void* V_cache,

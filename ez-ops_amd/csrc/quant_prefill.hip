@@ -437,7 +437,19 @@ __global__ __launch_bounds__(256) void quant_prefill_join_kernel(QuantAttnArgs a
 // 37 us; 16 x 16 tokens on 2000 rows 56.8, 49.9 and 58 us with one, two and three; nine
 // ragged chunks of 2660 tokens of 16 / 2 heads of 64 on up to 2500 rows 61 and 58 us with
 // one and two.
+//
+// kv_len counts in steps of len_step, so that most_splits below sees every plan.
+constexpr int64_t kMaxLen = int64_t(1) << 30;
+int64_t len_step(int64_t n) {  // a sixteenth to an eighth of n, two key tiles at least
+  return std::max(int64_t(2 * kBK), (int64_t(1) << (63 - __builtin_clzll(static_cast<unsigned long long>(n)))) / 8);
+}
+int64_t len_up(int64_t n) {
+  n = std::min(n, kMaxLen);
+  return (n + len_step(n) - 1) / len_step(n) * len_step(n);
+}
+int split_limit(int64_t kv_len) { return int(std::min(int64_t(kMaxSplits), (kv_len + 2 * kBK - 1) / (2 * kBK))); }
 SplitPlan plan(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t kv_len) {
+  kv_len = len_up(kv_len);
   const int64_t qt = rows_of(D) / (H / Hkv), seqs = B < T ? B : T;
   const int64_t tiles = (T + seqs * (qt - 1)) / qt;
   const double blocks = double(seqs * ((T / seqs + qt - 1) / qt) * Hkv), cus = num_cus();
@@ -446,7 +458,7 @@ SplitPlan plan(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t 
   const double mean = seqs > 1 ? most * 0.75 : kv_len > T ? double(kv_len - T / 2) / kBK : most / 2;
   int best = 1;
   double least = 1e30;
-  for (int ns = 1; ns <= kMaxSplits && ns <= (kv_len + 2 * kBK - 1) / (2 * kBK); ++ns) {
+  for (int ns = 1; ns <= split_limit(kv_len); ++ns) {
     const double longest = most / ns * kTile + kBlock, sum = blocks * (mean * kTile + ns * kBlock / at_once) / cus;
     const double rounds = seqs > 1 ? std::ceil(blocks * ns / (cus * at_once)) : 1.0;
     const double whole = rounds > 1 ? rounds * (at_once * mean / ns * kTile + kBlock) : 0.0;
@@ -456,9 +468,17 @@ SplitPlan plan(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t 
   }
   return {best, int(tiles), nullptr, nullptr};
 }
+// The most splits of any bound up to kv_len: the model's choice goes up and down as the bound
+// grows, but a buffer for the largest of several bounds has to be enough for all of them.
+int most_splits(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t kv_len) {
+  int most = 1;
+  for (int64_t n = len_up(kv_len); n > 0 && split_limit(n) > most; n -= len_step(n - 1))
+    most = std::max(most, plan(B, T, H, Hkv, D, n).nsplit);
+  return most;
+}
 int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
-size_t ws_size(const SplitPlan& pl, int64_t T, int64_t H, int64_t D) {
-  return pl.nsplit == 1 ? 0 : size_t(up256(pl.nsplit * T * H * D * 4) + up256(pl.nsplit * T * H * 8));
+size_t ws_size(int nsplit, int64_t T, int64_t H, int64_t D) {
+  return nsplit == 1 ? 0 : size_t(up256(nsplit * T * H * D * 4) + up256(nsplit * T * H * 8));
 }
 
 }  // namespace
@@ -469,7 +489,7 @@ extern "C" size_t ezops_quant_prefill_attn_workspace_size(int64_t B, int64_t T, 
   if (B < 1 || T < 1 || T >= (int64_t(1) << 30) || H < 1 || H > 4096 || Hkv < 1 || H % Hkv || H / Hkv > 16 || D < 1 || D > 128 ||
       kv_len < 1)
     return 0;
-  return ez::ws_size(ez::plan(B, T, H, Hkv, D, kv_len), T, H, D);
+  return ez::ws_size(ez::most_splits(B, T, H, Hkv, D, kv_len), T, H, D);
 }
 
 extern "C" int ezops_quant_prefill_attn_bf16(const void* q, int64_t q_stride, const void* K_cache, const void* V_cache,
@@ -490,11 +510,11 @@ extern "C" int ezops_quant_prefill_attn_bf16(const void* q, int64_t q_stride, co
   const int rc = ez::check_attn8(op, a, page_size, block_size, H, Hkv, D, max_kv_len);
   if (rc != EZ_OK) return rc;
   ez::finish_args(a, page_size, max_kv_len);
-ez::SplitPlan pl = ez::plan(B, T, H, Hkv, D, a.cap);
+  ez::SplitPlan pl = ez::plan(B, T, H, Hkv, D, a.cap);
   const int64_t blocks = int64_t(pl.tiles) * Hkv * pl.nsplit, joins = int64_t(pl.tiles) * Hkv * (ez::rows_of(D) * D / 1024);
   EZ_REQUIRE(blocks < int64_t(1) << 23 && (pl.nsplit == 1 || joins < int64_t(1) << 24), "%s: tokens * heads past one launch", op);
   if (pl.nsplit > 1) {
-    const size_t need = ez::ws_size(pl, T, H, D);
+    const size_t need = ez::ws_size(pl.nsplit, T, H, D);
     EZ_REQUIRE(ws && ws_bytes >= need, "%s: workspace too small (%zu < %zu)", op, ws_bytes, need);
     EZ_REQUIRE(ez::kv8_aligned16(ws), "%s: workspace must be 16-byte aligned", op);
     for (const auto& x : ez::attn8_tensors(a, H))

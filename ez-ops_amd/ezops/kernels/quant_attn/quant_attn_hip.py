@@ -1,6 +1,8 @@
 """HIP attention over the 8-bit KV cache (single tokens, packed prompts); no reference counterpart (its attention reads
 a contiguous bf16 cache, ezops/ops/attn_decode.py:9-67)."""
 
+import operator
+
 import torch
 
 from ... import _hip
@@ -20,7 +22,7 @@ class _QuantAttnKernel(BaseKernel):
         self._out = (("out", self._q, torch.bfloat16),)
         self._type = TYPE_CODES[cache_dtype]
         self._pool = (num_pages, page_size, max_pages, block_size)
-        self._ws_bytes: dict = {}  # by the library, per max_kv_len
+        self._ws_bytes: dict = {}  # by the library, per bound on the lengths
 
     def _out_of(self, out, dev):
         if out is None:
@@ -30,12 +32,12 @@ class _QuantAttnKernel(BaseKernel):
         return out
 
     def _workspace(self, dev, max_kv_len, name, *shape):
-        n = self._ws_bytes.get(max_kv_len)
+        n = operator.index(max_kv_len if 0 < max_kv_len < self.S else self.S)
+        step = 1 << max(7, n.bit_length() - 4)
+        bound = -(-n // step) * step  # a size is enough for smaller bounds: a few of them serve all
+        n = self._ws_bytes.get(bound)
         if n is None:
-            n = _hip.size(name, *shape, max_kv_len if 0 < max_kv_len < self.S else self.S)
-            if len(self._ws_bytes) >= 1024:
-                self._ws_bytes.clear()
-            self._ws_bytes[max_kv_len] = n
+            n = self._ws_bytes[bound] = _hip.size(name, *shape, bound)
         # from torch's allocator at every call: stream-ordered, and a captured graph keeps its own
         return (torch.empty(n, dtype=torch.uint8, device=dev) if n else None), n
 

@@ -335,8 +335,9 @@ int ezops_kv_cache_dequant_bf16(const void* K_cache, const void* V_cache, const 
  * anything.  H / Hkv in {1, 2, 4, 8, 16}, D in {64, 128}, B <= 65536, H <= 4096; scale <= 0
  * selects 1/sqrt(D).  Products of q with a row's codes have to stay below 2^128, as scores
  * do; past that the query's own output is undefined.  workspace: 16-byte aligned,
- * ezops_quant_paged_attn_decode_workspace_size(B, H, Hkv, D, max_kv_len or max_pages *
- * page_size) bytes, need not be zero-filled (NULL where that is 0).
+ * ezops_quant_paged_attn_decode_workspace_size(B, H, Hkv, D, kv_len) bytes, need not be
+ * zero-filled (NULL where that is 0); kv_len: max_kv_len where that is > 0, else max_pages *
+ * page_size, or more: the size for a bound is enough for every smaller one too.
  * No counterpart in the reference (bf16 cache, ezops/ops/attn_decode.py:9-67). */
 size_t ezops_quant_paged_attn_decode_workspace_size(int64_t B, int64_t H, int64_t Hkv, int64_t D,
                                                     int64_t kv_len);
@@ -353,7 +354,8 @@ int ezops_quant_paged_attn_decode_bf16(const void* q, int64_t q_stride, const vo
  * cu_seqlens[b] .. cu_seqlens[b+1]-1 (clamped into [0, T]; the offsets must not decrease),
  * its token i stands at cache row past_lens[b] + i (past_lens NULL = 0) and sees the rows
  * up to that one.  Rows of no sequence, and of tokens at or past max_pages * page_size or
- * max_kv_len (where that is > 0), are not written. */
+ * max_kv_len (where that is > 0), are not written.  workspace as above, by
+ * ezops_quant_prefill_attn_workspace_size with the call's B and T. */
 size_t ezops_quant_prefill_attn_workspace_size(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t D,
                                                int64_t kv_len);
 int ezops_quant_prefill_attn_bf16(const void* q, int64_t q_stride, const void* K_cache,
