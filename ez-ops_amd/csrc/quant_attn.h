@@ -28,9 +28,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 // kept within (0, FLT_MAX], so that a masked score of -inf stays one and a score of 0 too
 // (0 * -inf and inf * 0 are NaN).  Where it is subnormal it is off by less than 2^-148, and
 // times a sum q . codes of less than 2^128 by less than 2^-20; past fp32 the scores saturate.
-__device__ __forceinline__ float kv8_factor(float scale, int e) {
-  const float c = scale * kv8_scale(e) * kLog2e;  // the power first: exact where the scale is subnormal and it is large
-  return e == kKvNanExp ? c : fminf(fmaxf(c, 0x1p-149f), 0x1.fffffep127f);
+__device__ __forceinline__ float kv8_factor(float scale, int e) {  // e as kv8_exp gives it
+  // the power first: exact where the scale is subnormal and it is large
+  const float c = scale * __uint_as_float(uint32_t(e) << 23) * kLog2e;
+  return e == kKvNanExp ? __uint_as_float(0x7fc00000u) : __builtin_amdgcn_fmed3f(c, 0x1p-149f, 0x1.fffffep127f);
 }
 
 constexpr float kLowest = -3e38f;  // softmax reference before any row: finite, so that differences are
