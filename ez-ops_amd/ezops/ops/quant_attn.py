@@ -18,6 +18,8 @@ the products of q with a row's codes have to stay below 2^128 (as does a score),
 the query's own output is undefined.
 """
 
+import operator
+
 import torch
 
 from ..registry import get_kernel
@@ -32,6 +34,17 @@ def cache_rows(cache, scale, table, block_size):
     x = cache.view(torch.uint8)[table].view(cache.dtype).float()
     x = x * exp2_of(read_exp(scale[table])).repeat_interleave(block_size, -1)[..., None]
     return x.transpose(0, 1).flatten(1, 2)
+
+
+MAX_ROWS = 1 << 30  # of a block table
+
+
+def bound(max_kv_len):
+    """A caller's bound on the lengths as the kernels take it; 0 for none."""
+    n = operator.index(max_kv_len)
+    if n < 0:
+        raise ValueError(f"max_kv_len ({max_kv_len}) must be >= 0")
+    return min(n, MAX_ROWS)
 
 
 class _QuantAttnOp(Op):
@@ -49,7 +62,7 @@ class _QuantAttnOp(Op):
             raise ValueError(f"num_heads ({num_heads}) must be divisible by num_kv_heads ({num_kv_heads}) and at most 4096")
         if num_heads // num_kv_heads not in GROUPS:
             raise ValueError(f"GQA group size {num_heads}/{num_kv_heads} not supported (1, 2, 4, 8 or 16)")
-        if max_pages < 1 or max_pages * page_size > 1 << 30:
+        if max_pages < 1 or max_pages * page_size > MAX_ROWS:
             raise ValueError(f"max_pages ({max_pages}) must be >= 1 and max_pages * page_size at most 2^30")
         num_pages = batch * max_pages if num_pages is None else num_pages
         check_cache(page_size, num_pages, block_size, cache_dtype, head_dim)
@@ -116,7 +129,7 @@ class QuantPagedAttnDecodeOp(_QuantAttnOp):
         """q [B, H, D] (rows may lie apart), kv_lens [B] int32 -> out [B, H, D]; a sequence of no rows gets zeros.
         max_kv_len: the caller's bound on the lengths (0 = max_pages * page_size), which plans the work; longer ones are
         cut off there."""
-        return self._kernel(q, K_cache, V_cache, K_scale, V_scale, block_table, kv_lens, max_kv_len, out=out)
+        return self._kernel(q, K_cache, V_cache, K_scale, V_scale, block_table, kv_lens, bound(max_kv_len), out=out)
 
     def gen_data(self, device=None):
         dev, q, pools, table = self._gen(device)
@@ -131,7 +144,7 @@ class QuantPagedAttnDecodeOp(_QuantAttnOp):
 
     def _ref_forward(self, q, K_cache, V_cache, K_scale, V_scale, block_table, kv_lens, max_kv_len: int = 0, *, out=None):
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
-        cap = min(max_kv_len or 1 << 30, self.max_pages * self.page_size)
+        cap = min(max_kv_len or MAX_ROWS, self.max_pages * self.page_size)
         for b, n in enumerate(kv_lens.tolist()):
             n = min(max(n, 0), cap)
             out[b] = self._attend(q[b:b + 1], K_cache, V_cache, K_scale, V_scale, block_table[b], n - 1)[0] if n else 0
@@ -161,7 +174,7 @@ class QuantPrefillAttnOp(_QuantAttnOp):
         bound on past + new tokens of a sequence (0 = none), which plans the work; tokens past it are not written
         either."""
         return self._kernel(q, K_cache, V_cache, K_scale, V_scale, block_table, cu_seqlens, past_lens,
-                            max_kv_len=max_kv_len, out=out)
+                            max_kv_len=bound(max_kv_len), out=out)
 
     def gen_data(self, device=None):
         """The rows shared out evenly, each sequence on a few cached rows where there is room."""
@@ -182,7 +195,7 @@ class QuantPrefillAttnOp(_QuantAttnOp):
     def _ref_forward(self, q, K_cache, V_cache, K_scale, V_scale, block_table, cu_seqlens, past_lens=None, *,
                      max_kv_len: int = 0, out=None):
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
-        cap = min(max_kv_len or 1 << 30, self.max_pages * self.page_size)
+        cap = min(max_kv_len or MAX_ROWS, self.max_pages * self.page_size)
         cu = [min(max(0, x), self.num_tokens) for x in cu_seqlens.tolist()]
         past = past_lens.tolist() if past_lens is not None else [0] * self.batch
         for b, (s, e) in enumerate(zip(cu, cu[1:])):
