@@ -82,9 +82,8 @@ __device__ __forceinline__ void kv8_f32x4(uint32_t w, float (&f)[4]) {
 
 // ---- fp32 values in units of their scale -> codes, round to nearest even, saturating.
 // Not finite: 0x7f in e4m3 (it has no infinities; the conversion itself makes 0xff of a
-// NaN), which callers that know their values finite leave out (CHECK false); int8 has no
-// such code (its block's exponent says so).
-template <int TYPE, bool CHECK>
+// NaN); int8 has no such code (its block's exponent says so).
+template <int TYPE>
 __device__ __forceinline__ uint32_t kv8_codes(const float (&y)[4]) {
   if constexpr (TYPE == kKvE4m3) {
     float c[4];
@@ -92,11 +91,9 @@ __device__ __forceinline__ uint32_t kv8_codes(const float (&y)[4]) {
     for (int i = 0; i < 4; ++i) c[i] = fminf(fmaxf(y[i], -448.f), 448.f);
     uint32_t w = uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false));
     w = uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], int(w), true));
-    if constexpr (CHECK) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (!(fabsf(y[i]) < INFINITY)) w = (w & ~(0xffu << (8 * i))) | (0x7fu << (8 * i));
-    }
+    for (int i = 0; i < 4; ++i)
+      if (!(fabsf(y[i]) < INFINITY)) w = (w & ~(0xffu << (8 * i))) | (0x7fu << (8 * i));
     return w;
   } else {
     uint32_t w = 0;

@@ -76,7 +76,7 @@ __device__ __forceinline__ uint2 to_codes(const uint4& x, int e, bool finite) {
 #pragma unroll
   for (int k = 0; k < 8; ++k) f[k] = TYPE == kKvInt8 && e == kKvNanExp ? 0.f : f[k] * inv;
   const float lo[4] = {f[0], f[1], f[2], f[3]}, hi[4] = {f[4], f[5], f[6], f[7]};
-  return make_uint2(kv8_codes<TYPE, true>(lo), kv8_codes<TYPE, true>(hi));
+  return make_uint2(kv8_codes<TYPE>(lo), kv8_codes<TYPE>(hi));
 }
 
 // The n rows a block held before, from scale `old` to the larger e: 4 codes a lane, `of` lanes.
@@ -89,7 +89,7 @@ __device__ __forceinline__ void turn_rows(uint8_t* rows, int n, int old, int e, 
     kv8_f32x4<TYPE>(held[i], y);
 #pragma unroll
     for (int k = 0; k < 4; ++k) y[k] *= r;
-    held[i] = kv8_codes<TYPE, true>(y);
+    held[i] = kv8_codes<TYPE>(y);
   }
 }
 
