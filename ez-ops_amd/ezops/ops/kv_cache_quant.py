@@ -24,10 +24,10 @@ that leave their range.
 
 Token ``t`` goes to slot ``slot_mapping[t]`` (int64, page * page_size + offset, as
 PagedBatchPlanOp makes it); slots outside the pool are skipped.  The tokens that a block
-gets in one call stand next to one another in ascending slots (as a plan has them), and
-nothing is kept of rows of that block behind the last of them; a block whose tokens are
-not in one run, or a slot used twice, is left with undefined rows and scale, other blocks
-are not touched.  Values of magnitude 2^67 and more saturate and such below 2^-61 become
+gets in one call have to be one run, consecutive tokens in consecutive slots (as a plan
+has them), and nothing is kept of rows of that block behind the last of them; a block whose
+tokens are not (a row or a token left out between them, another order), or a slot used
+twice, is left with undefined rows and scale, other blocks are not touched.  Values of magnitude 2^67 and more saturate and such below 2^-61 become
 zero.  A k or v that is not finite is a NaN code (0x7f) of its own in an e4m3 cache; int8 has no
 such code, and its block reads as NaN until its first row is written again.
 """

@@ -34,7 +34,7 @@ extern "C" {
 #endif
 
 /* Raised with every entry that is added or changed; 3: batch plan, QK norm with
- * several position axes, linear attention. */
+ * several position axes, linear attention; 4: KV cache held in 8 bits. */
 #define EZOPS_HIP_ABI_VERSION 4
 #define EZOPS_EINVAL (-22)
 #define EZOPS_ENOSYS (-38) /* feature not compiled into this build */
@@ -306,12 +306,12 @@ int ezops_linear_attn_decode_bf16(const void* q, int64_t q_stride, const void* k
  * [67, 187] with max|x| <= TOP 2^(e - 127), TOP = 127 or 448; e = need where the block's
  * first row is among them, else max(need, e as it was), and where that grows, the rows
  * held before become round(code 2^(e_old - e)); code = round(x 2^(127 - e)), to nearest
- * even, saturating.  The tokens of a block must be consecutive with ascending slots; else,
- * or where a slot comes twice, the rows and the scale of that block (and nothing else) are
- * undefined.  Not finite: NaN code 0x7f (e4m3), or e = 255 for the block (int8).  D in {64,
- * 128}; page_size a power of two in [32, 2^20], block_size one in [16, 256] and at most
- * page_size; k, v and the caches 16-byte aligned; caches and scales must not overlap each
- * other or an input.
+ * even, saturating.  The tokens of a block must be one run, consecutive tokens in
+ * consecutive slots; else (a row or token left out between them), or where a slot comes
+ * twice, the rows and the scale of that block (and nothing else) are undefined.  Not
+ * finite: NaN code 0x7f (e4m3), or e = 255 for the block (int8).  D in {64, 128}; page_size
+ * a power of two in [32, 2^20], block_size one in [16, 256] and at most page_size; k, v and
+ * the caches 16-byte aligned; caches and scales must not overlap each other or an input.
  * No counterpart in the reference (bf16 cache, ezops/ops/attn_decode.py:60-61). */
 int ezops_kv_cache_quant_bf16(const void* k, int64_t k_stride, const void* v, int64_t v_stride,
                               const int64_t* slot_mapping, void* K_cache, void* V_cache,
