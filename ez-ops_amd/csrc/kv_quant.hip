@@ -18,7 +18,10 @@
 // Measured: 16384 tokens of 8 heads of 128 written in 18 us and read back in 16
 // where the memory-side cache holds some of them; 45 us a call of both on inputs that no
 // cache holds (a large copy of as many bytes 39).  40000 rows read back in 51 us, 5.0 TB/s
-// (copy 5.1); 64 single tokens 3.4 us, a launch and two dependent loads.
+// (copy 5.1).  64 single tokens 3.3 us, a launch and two dependent loads, where no scale grows;
+// where one does, the 8 or 16 lanes of the row turn the block's earlier rows 4 bytes each at a
+// time: all 64 at the last row of their block 17 us in blocks of 32 rows, 130 to 140 in blocks of
+// 256, 155 to 195 with heads of 64.
 #include "common.h"
 #include "internal.h"
 #include "kv8.h"
@@ -166,7 +169,7 @@ __device__ __forceinline__ void quant_run(const KvQuantArgs& a, int64_t t, int64
 }
 
 // Runs of one token: the lanes of a row (D / 8) take one each, so a wave takes RPI of them
-// at a time.  `i` is the lane that holds the token's slot, `on` whether these lanes have one.
+// at a time.  Token `t` goes to `slot`, where these lanes have one (`on`).
 template <int D, int TYPE>
 __device__ __forceinline__ void quant_singles(const KvQuantArgs& a, int64_t t, int64_t slot, bool on, int h, bool is_v) {
   constexpr int LPR = D / 8;
@@ -353,18 +356,23 @@ extern "C" int ezops_kv_cache_quant_bf16(const void* k, int64_t k_stride, const 
   a.k = static_cast<const uint16_t*>(k); a.k_rs = k_stride;
   a.v = static_cast<const uint16_t*>(v); a.v_rs = v_stride;
   a.slots = slot_mapping; a.T = T;
-  // Tokens a wave looks at: as many as leave 4096 waves.  In a prompt most tokens begin no
-  // run, and a wave that finds none still holds its place for two loads (16384 tokens of
-  // 8 heads in blocks of 64: 82 us with 8 tokens a wave, 47, 33 and 27 with 16, 32 and 64, one wave a run;
-  // a mixed step of 3500 tokens 10.6, 9.2, 8.8 and 10.0 us at 2, 4, 8 and 16).
+  // Tokens that the waves of a unit look at: doubled up to 64 while there are more than 4096
+  // units (a window, a kv head, K or V), so that 2049 to 4096 are left.  In a prompt most
+  // tokens begin no run, and a wave that finds none still holds its place for two loads; few
+  // tokens want many waves.  The kernel alone, 8 heads of 128, at 8, 16, 32 and 64 tokens:
+  // 16384 tokens in blocks of 32 rows 34, 26, 18 and 17 us, of 64 33, 24, 20 and 17.5, of 256 65,
+  // 44, 33 and 27 (the rule: 64); a mixed step of 3684 tokens in blocks of 16 7.5, 6.9, 7.8 and
+  // 10.2, of 64 10.8, 8.6, 8.0 and 8.4 (16).  Between these it is not the best: 4096 tokens of one
+  // prompt 8.8 us at its 16, 5.9 at 32; 1024 5.8 at its 4, 4.4 at 16.
   int window = 1;
   while (window < 64 && T * Hkv * 2 / window > 4096) window *= 2;
   const int64_t units = (T + window - 1) / window * Hkv * 2;
   // Rows of a wave and waves of a run: 32 registers of values a lane at most, and 16 where
   // four waves hold a whole block in that (16384 tokens of heads of 128 in blocks of 64: two
   // waves a SIMD with 64 registers 50.6 us with the read-back, 45 so; three prompts of 5250
-  // in blocks of 256 53.4, with eight waves 51; heads of 64 so 28.4 and 35.5, but 26.6 and 31.3
-  // with the rows of half as many bytes that they have).
+  // in blocks of 256 53.4, with eight waves 51).  Rows of heads of 64 have half the bytes: the
+  // same two cases 28.4 and 35.5 us with as many waves, 26.6 and 31.3 with one and four, 64
+  // rows each.
 #define EZ_RUN(DD, TY, CH, WPU)                                                                              \
   do {                                                                                                       \
     constexpr int threads = (WPU) > 4 ? (WPU) * 64 : 256;                                                    \

@@ -15,22 +15,24 @@
 // that sums the weights.  w is rounded to bf16 for the product; l sums the rounded
 // weights, so that rounding cancels in o / l but for its spread.
 //
-// A block owns 256 rows of one kv head: (query, head of the group) pairs, 256 / G
-// queries, 32 rows a wave; all share the K / V tiles of 64 keys.  A tile is read once
-// from memory in 8 bits (16 bytes a thread and tensor, two tiles ahead in registers),
-// widened to bf16 on its way into one of two LDS buffers, so the widening is done
-// once for the 8 waves.  Operand layouts (lane 32 h + j): S^T = K Q^T, then O^T = V^T P^T
+// A block owns 256 rows of one kv head (128 with heads of 64): (query, head of the group)
+// pairs, 256 / G queries, 32 rows to each of 8 (4) waves; all share the K / V tiles of 64
+// keys.  A tile is read once from memory in 8 bits (16 bytes a thread and tensor, two tiles
+// ahead in registers), widened to bf16 on its way into one of two LDS buffers, so the
+// widening is done once for all waves.  Operand layouts (lane 32 h + j): S^T = K Q^T, then O^T = V^T P^T
 // with the weights staying in their lane; V^T by transposing LDS reads.
 //
 // Where the queries are few (a chunk on a long prefix) the keys are shared out over
 // nsplit blocks; they leave fp32 partials (O, m, l), which a second kernel joins.
 //
-// Measured: 2048 tokens on 30000 rows, 32 / 8 heads of 128, e4m3: 1.02 ms, 1020 TFLOP/s; a
-// fresh prompt of 4096 tokens, int8: 145 us, 945 TFLOP/s (a large bf16 matrix product: 1220);
-// 8192 tokens of 16 / 2 heads of 64 600.  By the counters the matrix cores are busy 44% and the
-// vector units 51% of a CU's time at 4096 tokens, hardly at once: a tile's exponentials take
-// as long as its products, the two waves of a SIMD meet at each tile's barrier, and a
-// second tile's scores do not fit the registers (228 of 256).
+// Measured (two cards): 2048 tokens on 30000 rows, 32 / 8 heads of 128, e4m3: 1.03 and 1.08 ms,
+// 1010 and 970 TFLOP/s; a fresh prompt of 4096 tokens, int8: 145 and 153 us, 950 and 900 (a large
+// bf16 matrix product: 1220).  By the counters the matrix cores are busy 44% and the vector units
+// 51% of a CU's time at 4096 tokens, hardly at once: a tile's exponentials take as long as its
+// products, the two waves of a SIMD meet at each tile's barrier, and a second tile's scores do
+// not fit the registers (228 of 256).  8192 tokens of 16 / 2 heads of 64: 204 us, 670 TFLOP/s;
+// with as many exponentials for half the products the vector units are busy 76% of the time,
+// the matrix cores 34%.
 #include <algorithm>
 #include <cmath>
 
@@ -314,8 +316,9 @@ __global__ __launch_bounds__(waves_of(D) * kWave) __attribute__((amdgpu_waves_pe
     }
     mx = halves_max(mx);
     // The reference m moves, and O and l are rescaled, only where a row's maximum passes
-    // it by more than kLazy: weights stay below 2^kLazy, exact in fp32 and of the same
-    // relative precision in bf16, and most tiles skip the rescale.
+    // it by more than kLazy, and most tiles skip the rescale.  Weights, which carry the scale
+    // of v, stay below 2^(kLazy + 60), and the sums of their products with codes far below
+    // 2^127: fp32 and bf16 hold them with the same relative precision at any size.
     if (__builtin_amdgcn_ballot_w64(mx > m + kLazy)) {
       const float mn = fmaxf(m, mx);
       const float alpha = __builtin_amdgcn_exp2f(m - mn);
