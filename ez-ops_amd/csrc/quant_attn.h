@@ -27,7 +27,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 // Factor of the scores of a block with exponent e, scale log2(e) 2^(e - 127): NaN for 255, else
 // kept within (0, FLT_MAX], so that a masked score of -inf stays one and a score of 0 too
 // (0 * -inf and inf * 0 are NaN).  Where it is subnormal it is off by less than 2^-148, and
-// times a sum q . codes of less than 2^128 by less than 2^-20; past fp32 the scores saturate.
+// times a sum q . codes of less than 2^128 by less than 2^-20.  Callers keep it below 2^128
+// where a row is not all zeros.
 __device__ __forceinline__ float kv8_factor(float scale, int e) {  // e as kv8_exp gives it
   // the power first: exact where the scale is subnormal and it is large
   const float c = scale * __uint_as_float(uint32_t(e) << 23) * kLog2e;

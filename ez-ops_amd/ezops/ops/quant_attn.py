@@ -13,9 +13,10 @@ rows ``0 .. past_lens[b] + i`` for the sequence's new token ``i`` (prefill; the 
 are in the cache already).  Query head ``h`` reads kv head ``h // (H / Hkv)``;
 ``block_table [B, max_pages]`` (int32) maps logical pages to pool pages.  Ids of pages that
 hold visible rows must lie in the pool (others are read as a page of it); codes and scales
-of rows that no query sees may hold anything.  Any positive scale of fp32 may be asked for;
-the products of q with a row's codes have to stay below 2^128 (as does a score), past which
-the query's own output is undefined.
+of rows that no query sees may hold anything.  The scale is any positive
+number of fp32.  Products of q with a row's codes have to stay below 2^128, and so do scores
+and, unless all of a row's codes are 0, ``1.45 * scale * 2^(e - 127)`` of its block; past that the
+query's own output is undefined.
 """
 
 import operator

@@ -333,8 +333,9 @@ int ezops_kv_cache_dequant_bf16(const void* K_cache, const void* V_cache, const 
  * that is > 0), one without rows gets zeros.  max_kv_len plans the work.  Page ids outside
  * the pool are clamped into it; codes and scales of rows behind a length may hold
  * anything.  H / Hkv in {1, 2, 4, 8, 16}, D in {64, 128}, B <= 65536, H <= 4096; scale <= 0
- * selects 1/sqrt(D).  Products of q with a row's codes have to stay below 2^128, as scores
- * do; past that the query's own output is undefined.  workspace: 16-byte aligned,
+ * selects 1/sqrt(D).  Products of q with a row's codes have to stay below 2^128, and so do
+ * scores and, unless all of a row's codes are 0, 1.45 scale 2^(e - 127) of its block; past that
+ * the query's own output is undefined.  workspace: 16-byte aligned,
  * ezops_quant_paged_attn_decode_workspace_size(B, H, Hkv, D, kv_len) bytes, need not be
  * zero-filled (NULL where that is 0); kv_len: max_kv_len where that is > 0, else max_pages *
  * page_size, or more: the size for a bound is enough for every smaller one too.
